@@ -56,6 +56,10 @@ CU_SOURCES = [
     "rotate_aggregate.cu",
     "edge_chain.cu",
     "checks.cu",
+    "rotary.cu",
+    "group_norm.cu",
+    "route.cu",
+    "adamw.cu",
 ]
 HEADERS = ["common.cuh", "launch.cuh"]
 

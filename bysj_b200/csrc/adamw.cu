@@ -1,0 +1,339 @@
+// One AdamW step over many tensors for sm_100a, states in 32 or 8 bits.
+//
+//   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+//   p = decay p - size m / (correct sqrt(v) + eps)
+//
+// Work is counted in blocks of 256 elements, the unit that shares one scale
+// of an 8-bit state.  The tensor table travels in the kernel's parameters
+// (no copy to the device); a warp finds the tensor of its block by a binary
+// search and takes 8 elements per lane.  Every tensor's states begin at a
+// block boundary of the shared state buffers, so the table holds no state
+// pointers and their loads are always aligned.
+//
+// Each product and sum is rounded to fp32 on its own (no fused
+// multiply-add), so a step gives the same bits as the formula evaluated one
+// operation at a time.
+//
+// 8-bit states.  m keeps a sign and a 7-bit magnitude with 3 mantissa bits
+// (a relative rounding of at most 1/16 down to 2^-16 of the block's
+// largest); sqrt(v) an 8-bit code with 4 mantissa bits (1/32).  The step
+// divides by sqrt(v), so its root is what is kept: 2^-16 there spans 2^-32 of
+// v.  A positive v never becomes 0: its code is at least 1, so a rounded
+// second moment can only shorten a step, not divide by eps.  The scale is the
+// block's largest magnitude itself and value(top) = 1, so that element is
+// kept exactly and a decay by beta is carried by the scale.
+#include "launch.cuh"
+
+namespace bysj {
+namespace {
+
+constexpr int kStateBlock = BYSJ_ADAMW_BLOCK;
+constexpr int kPerLane = kStateBlock / kWarp;
+constexpr int kTopM = 127, kMantM = 3;
+constexpr int kTopV = 255, kMantV = 4;
+
+struct AdamEntry {
+  void* param;
+  const void* grad;
+  int64_t n;
+  int64_t state_block;  // first block in the state buffers
+  int64_t work_block;   // first block of this launch's work list
+};
+
+template <int CAP>
+struct AdamArgs {
+  AdamEntry entry[CAP];
+  int count;
+  int64_t work_blocks;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  float* master;
+  const float* grad_scale;
+  bysj_adamw_hyper h;
+};
+
+// Kernel parameters hold 32,764 bytes; most models need far fewer entries and
+// a shorter parameter block costs less to launch.
+constexpr int kSmallTable = 96;
+constexpr int kLargeTable = 800;
+
+__device__ __forceinline__ float load_f32(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float load_f32(const __nv_bfloat16* p) {
+  return __bfloat162float(*p);
+}
+__device__ __forceinline__ void store_value(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_value(__nv_bfloat16* p, float v) {
+  *p = __float2bfloat16_rn(v);
+}
+
+template <int TOP, int MANT>
+__device__ __forceinline__ float code_value(int code) {
+  const float v = __int_as_float((code - TOP + (127 << MANT)) << (23 - MANT));
+  return code > 0 ? v : 0.0f;
+}
+
+// Code of ratio in [0, 1]: the bits of the float rounded to MANT mantissa
+// bits (to nearest, ties to even), counted down from TOP; may come out <= 0.
+template <int TOP, int MANT>
+__device__ __forceinline__ int ratio_code(float ratio) {
+  constexpr int kShift = 23 - MANT;
+  const int bits = __float_as_int(ratio);
+  const int code = (bits + ((1 << (kShift - 1)) - 1) + ((bits >> kShift) & 1)) >> kShift;
+  return min(code - (127 << MANT) + TOP, TOP);
+}
+
+// Largest magnitude over the warp's block; for non-negative floats the order
+// of the bits is the order of the values (NaN above all).
+__device__ __forceinline__ float block_max(const float (&v)[kPerLane]) {
+  unsigned best = 0;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i)
+    best = max(best, static_cast<unsigned>(__float_as_int(v[i])) & 0x7fffffffu);
+  return __uint_as_float(__reduce_max_sync(kFull, best));
+}
+
+__device__ __forceinline__ float inverse_scale(float scale) {
+  return scale > 0.0f ? __frcp_rn(scale) : 0.0f;
+}
+
+__device__ __forceinline__ int encode_m(float m, float inv) {
+  const float size = fabsf(m);
+  const float ratio = __fmul_rn(size, inv);
+  int code = ratio_code<kTopM, kMantM>(ratio);
+  // below the smallest code's value (1.25 2^-16): to it or to 0, the nearer
+  if (code < 1) code = ratio >= 0.5f * 1.25f / 65536.0f ? 1 : 0;
+  return m < 0.0f ? code + 128 : code;
+}
+
+__device__ __forceinline__ int encode_v(float root, float inv) {
+  const int code = ratio_code<kTopV, kMantV>(__fmul_rn(root, inv));
+  return root > 0.0f ? max(code, 1) : 0;
+}
+
+template <typename T, int BITS, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kBlock)
+    adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
+  const int lane = lane_id();
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
+  const float scale = a.grad_scale != nullptr ? __ldg(a.grad_scale) : 1.0f;
+  const bool scaled = a.grad_scale != nullptr;
+  for (int64_t work = global_warp(); work < a.work_blocks; work += warps) {
+    int lo = 0, hi = a.count - 1;  // last entry whose work_block <= work
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (a.entry[mid].work_block <= work) lo = mid;
+      else hi = mid - 1;
+    }
+    const int64_t local = work - a.entry[lo].work_block;
+    const int64_t block = a.entry[lo].state_block + local;
+    const int64_t begin = local * kStateBlock;
+    const int64_t left = a.entry[lo].n - begin;
+    T* param = static_cast<T*>(a.entry[lo].param) + begin;
+    const T* grad = static_cast<const T*>(a.entry[lo].grad) + begin;
+    const int64_t state = block * kStateBlock;
+    float p[kPerLane], g[kPerLane], m[kPerLane], v[kPerLane];
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int j = lane + i * kWarp;
+      const bool in = j < left;
+      g[i] = in ? load_f32(grad + j) : 0.0f;
+      if constexpr (MASTER) p[i] = a.master[state + j];
+      else p[i] = in ? load_f32(param + j) : 0.0f;
+      if constexpr (BITS == 32) {
+        m[i] = static_cast<const float*>(a.exp_avg)[state + j];
+        v[i] = static_cast<const float*>(a.exp_avg_sq)[state + j];
+      } else {
+        const int cm = static_cast<const uint8_t*>(a.exp_avg)[state + j];
+        const int cv = static_cast<const uint8_t*>(a.exp_avg_sq)[state + j];
+        const float size = __fmul_rn(code_value<kTopM, kMantM>(cm & 127), a.exp_avg_scale[block]);
+        const float root = __fmul_rn(code_value<kTopV, kMantV>(cv), a.exp_avg_sq_scale[block]);
+        m[i] = cm & 128 ? -size : size;
+        v[i] = __fmul_rn(root, root);
+      }
+    }
+    float root[kPerLane];
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const float gi = scaled ? __fmul_rn(g[i], scale) : g[i];
+      m[i] = __fadd_rn(__fmul_rn(m[i], a.h.beta1), __fmul_rn(gi, a.h.one_minus_beta1));
+      v[i] = __fadd_rn(__fmul_rn(v[i], a.h.beta2),
+                       __fmul_rn(__fmul_rn(gi, a.h.one_minus_beta2), gi));
+      root[i] = __fsqrt_rn(v[i]);
+      const float den = __fadd_rn(__fmul_rn(root[i], a.h.correct), a.h.eps);
+      p[i] = __fsub_rn(__fmul_rn(p[i], a.h.decay), __fmul_rn(__fdiv_rn(m[i], den), a.h.size));
+    }
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int j = lane + i * kWarp;
+      if (j < left) {
+        store_value(param + j, p[i]);
+        if constexpr (MASTER) a.master[state + j] = p[i];
+      }
+    }
+    if constexpr (BITS == 32) {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        const int j = lane + i * kWarp;
+        static_cast<float*>(a.exp_avg)[state + j] = m[i];
+        static_cast<float*>(a.exp_avg_sq)[state + j] = v[i];
+      }
+    } else {
+      const float sm = block_max(m), sv = block_max(root);
+      const float im = inverse_scale(sm), iv = inverse_scale(sv);
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        const int j = lane + i * kWarp;
+        static_cast<uint8_t*>(a.exp_avg)[state + j] = static_cast<uint8_t>(encode_m(m[i], im));
+        static_cast<uint8_t*>(a.exp_avg_sq)[state + j] =
+            static_cast<uint8_t>(encode_v(root[i], iv));
+      }
+      if (lane == 0) {
+        a.exp_avg_scale[block] = sm;
+        a.exp_avg_sq_scale[block] = sv;
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kBlock)
+    adamw_values_kernel(const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const float* scale_m,
+                        const float* scale_v, int64_t count, float* out_m, float* out_v) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < count;
+       i += step) {
+    const int cm = exp_avg[i], cv = exp_avg_sq[i];
+    const float size = __fmul_rn(code_value<kTopM, kMantM>(cm & 127), scale_m[i / kStateBlock]);
+    const float root = __fmul_rn(code_value<kTopV, kMantV>(cv), scale_v[i / kStateBlock]);
+    out_m[i] = cm & 128 ? -size : size;
+    out_v[i] = __fmul_rn(root, root);
+  }
+}
+
+template <typename T, int BITS, bool MASTER, int CAP>
+int launch_chunk(const bysj_adamw_tensor* tensors, int64_t count, AdamArgs<CAP>& a,
+                 cudaStream_t s) {
+  a.count = 0;
+  a.work_blocks = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (tensors[i].n == 0) continue;
+    AdamEntry& e = a.entry[a.count++];
+    e.param = tensors[i].param;
+    e.grad = tensors[i].grad;
+    e.n = tensors[i].n;
+    e.state_block = tensors[i].first_block;
+    e.work_block = a.work_blocks;
+    a.work_blocks += (tensors[i].n + kStateBlock - 1) / kStateBlock;
+  }
+  if (a.work_blocks == 0) return BYSJ_OK;
+  int64_t blocks = (a.work_blocks + kWarpsPerBlock - 1) / kWarpsPerBlock;
+  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 16;
+  if (blocks > cap) blocks = cap;
+  adamw_kernel<T, BITS, MASTER, CAP><<<static_cast<unsigned>(blocks), kBlock, 0, s>>>(a);
+  return launch_check("adamw_kernel");
+}
+
+template <typename T, int BITS, bool MASTER, int CAP>
+int launch_all(const bysj_adamw_tensor* tensors, int64_t count, const AdamArgs<1>& base,
+               cudaStream_t s) {
+  AdamArgs<CAP> a;
+  a.exp_avg = base.exp_avg;
+  a.exp_avg_sq = base.exp_avg_sq;
+  a.exp_avg_scale = base.exp_avg_scale;
+  a.exp_avg_sq_scale = base.exp_avg_sq_scale;
+  a.master = base.master;
+  a.grad_scale = base.grad_scale;
+  a.h = base.h;
+  for (int64_t at = 0; at < count; at += CAP) {
+    const int64_t part = count - at < CAP ? count - at : CAP;
+    const int st = launch_chunk<T, BITS, MASTER, CAP>(tensors + at, part, a, s);
+    if (st != BYSJ_OK) return st;
+  }
+  return BYSJ_OK;
+}
+
+template <typename T>
+int launch_type(const bysj_adamw_tensor* tensors, int64_t count, int bits,
+                const AdamArgs<1>& base, cudaStream_t s) {
+  const bool master = base.master != nullptr, small = count <= kSmallTable;
+  if (bits == 32) {
+    if (master)
+      return small ? launch_all<T, 32, true, kSmallTable>(tensors, count, base, s)
+                   : launch_all<T, 32, true, kLargeTable>(tensors, count, base, s);
+    return small ? launch_all<T, 32, false, kSmallTable>(tensors, count, base, s)
+                 : launch_all<T, 32, false, kLargeTable>(tensors, count, base, s);
+  }
+  if (master)
+    return small ? launch_all<T, 8, true, kSmallTable>(tensors, count, base, s)
+                 : launch_all<T, 8, true, kLargeTable>(tensors, count, base, s);
+  return small ? launch_all<T, 8, false, kSmallTable>(tensors, count, base, s)
+               : launch_all<T, 8, false, kLargeTable>(tensors, count, base, s);
+}
+
+}  // namespace
+}  // namespace bysj
+
+using namespace bysj;
+
+extern "C" {
+
+int bysj_adamw_step(const bysj_adamw_tensor* tensors, int64_t n_tensors, int dtype,
+                    int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
+                    float* exp_avg_sq_scale, float* master, const float* grad_scale,
+                    const bysj_adamw_hyper* hyper, void* stream) {
+  clear_error();
+  if (dtype != BYSJ_F32 && dtype != BYSJ_BF16)
+    return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw: unknown dtype %d", dtype);
+  if (state_bits != 8 && state_bits != 32)
+    return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw: states have 8 or 32 bits");
+  if (n_tensors < 0 || (n_tensors > 0 && tensors == nullptr) || hyper == nullptr)
+    return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw: no tensors or hyper parameters");
+  int64_t elements = 0;
+  for (int64_t i = 0; i < n_tensors; ++i) {
+    if (tensors[i].n < 0 || tensors[i].first_block < 0)
+      return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw: tensor %lld has an invalid size",
+                  (long long)i);
+    if (tensors[i].n > 0 && (tensors[i].param == nullptr || tensors[i].grad == nullptr))
+      return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw: tensor %lld is NULL", (long long)i);
+    elements += tensors[i].n;
+  }
+  if (elements == 0) return BYSJ_OK;
+  if (exp_avg == nullptr || exp_avg_sq == nullptr ||
+      (state_bits == 8 && (exp_avg_scale == nullptr || exp_avg_sq_scale == nullptr)))
+    return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw: NULL state");
+  AdamArgs<1> base{};
+  base.exp_avg = exp_avg;
+  base.exp_avg_sq = exp_avg_sq;
+  base.exp_avg_scale = exp_avg_scale;
+  base.exp_avg_sq_scale = exp_avg_sq_scale;
+  base.master = master;
+  base.grad_scale = grad_scale;
+  base.h = *hyper;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == BYSJ_F32 ? launch_type<float>(tensors, n_tensors, state_bits, base, s)
+                           : launch_type<__nv_bfloat16>(tensors, n_tensors, state_bits, base, s);
+}
+
+int bysj_adamw_state_values(const uint8_t* exp_avg, const uint8_t* exp_avg_sq,
+                            const float* exp_avg_scale, const float* exp_avg_sq_scale,
+                            int64_t blocks, float* exp_avg_values, float* exp_avg_sq_values,
+                            void* stream) {
+  clear_error();
+  if (blocks < 0) return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw values: invalid size");
+  if (blocks == 0) return BYSJ_OK;
+  if (exp_avg == nullptr || exp_avg_sq == nullptr || exp_avg_scale == nullptr ||
+      exp_avg_sq_scale == nullptr || exp_avg_values == nullptr || exp_avg_sq_values == nullptr)
+    return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw values: NULL pointer");
+  const int64_t count = blocks * kStateBlock;
+  int64_t grid = (count + kBlock - 1) / kBlock;
+  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 16;
+  if (grid > cap) grid = cap;
+  adamw_values_kernel<<<static_cast<unsigned>(grid), kBlock, 0,
+                        static_cast<cudaStream_t>(stream)>>>(
+      exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, count, exp_avg_values,
+      exp_avg_sq_values);
+  return launch_check("adamw_values_kernel");
+}
+
+}  // extern "C"

@@ -9,8 +9,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <optional>
 #include <tuple>
+#include <vector>
 
 #include "../../include/bysj_b200.h"
 
@@ -804,6 +806,337 @@ std::tuple<Tensor, Tensor, Tensor> gie_zonal_scatter_backward(Tensor grad_output
   return {gz, gr, gi};
 }
 
+// ---- rotary positions ----------------------------------------------------------
+
+// [tokens, heads, dim] with channel stride 1 and any other strides.
+int heads_dtype(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.dim() == 3, name, " must have shape (tokens, heads, dim)");
+  TORCH_CHECK(t.size(2) <= 1 || t.stride(2) == 1, name, " channels must be contiguous");
+  if (t.scalar_type() == torch::kFloat32) return BYSJ_F32;
+  TORCH_CHECK(t.scalar_type() == torch::kBFloat16, name, " must be float32 or bfloat16");
+  return BYSJ_BF16;
+}
+
+bysj_rotary_side rotary_side(const Tensor& x, const Tensor& y, const OptTensor& saved) {
+  bysj_rotary_side side{};
+  side.x = x.data_ptr();
+  side.y = y.data_ptr();
+  side.heads = x.size(1);
+  side.x_token_stride = x.stride(0);
+  side.x_head_stride = x.stride(1);
+  if (saved) {
+    side.saved = saved->data_ptr();
+    side.saved_token_stride = saved->stride(0);
+    side.saved_head_stride = saved->stride(1);
+  }
+  return side;
+}
+
+// Turns q and k; with saved_q / saved_k (the forward inputs) also returns the
+// gradient of float positions.
+std::tuple<Tensor, Tensor, OptTensor> rotary_axes(Tensor q, Tensor k, Tensor positions,
+                                                  Tensor inv_freq,
+                                                  std::vector<int64_t> sections,
+                                                  bool interleaved, bool inverse,
+                                                  OptTensor saved_q, OptTensor saved_k) {
+  const int dt = heads_dtype(q, "rotary q");
+  TORCH_CHECK(heads_dtype(k, "rotary k") == dt, "rotary q and k must have one dtype");
+  TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2),
+              "rotary q and k must have the same tokens and dim");
+  cuda_tensor(positions, "rotary positions");
+  const bool integers = positions.scalar_type() == torch::kInt64;
+  TORCH_CHECK(integers || positions.scalar_type() == torch::kFloat32,
+              "rotary positions must be float32 or int64");
+  const int64_t axes = static_cast<int64_t>(sections.size());
+  TORCH_CHECK(positions.dim() == 2 && positions.size(0) == q.size(0) && positions.size(1) == axes,
+              "rotary positions must have shape (tokens, axes)");
+  f32(inv_freq, "rotary inv_freq");
+  int64_t pairs = 0;
+  for (int64_t s : sections) pairs += s;
+  TORCH_CHECK(inv_freq.numel() == pairs, "rotary inv_freq must hold one value for each pair");
+  TORCH_CHECK(saved_q.has_value() == saved_k.has_value(), "rotary saved inputs come in pairs");
+  for (const Tensor* t : {&k, &positions, &inv_freq})
+    same_device(q, *t, "rotary input");
+  if (saved_q) {
+    TORCH_CHECK(heads_dtype(*saved_q, "rotary saved q") == dt && saved_q->sizes() == q.sizes() &&
+                    heads_dtype(*saved_k, "rotary saved k") == dt && saved_k->sizes() == k.sizes(),
+                "rotary saved inputs must match the gradients");
+    same_device(q, saved_q, "rotary saved q");
+    same_device(q, saved_k, "rotary saved k");
+  }
+  c10::cuda::CUDAGuard guard(q.device());
+  Tensor yq = torch::empty(q.sizes(), q.options()), yk = torch::empty(k.sizes(), k.options());
+  OptTensor gp;
+  if (saved_q) gp = torch::empty(positions.sizes(), positions.options());
+  const bysj_rotary_side qs = rotary_side(q, yq, saved_q), ks = rotary_side(k, yk, saved_k);
+  check(bysj_rotary_axes(&qs, &ks, dt, positions.data_ptr(), integers,
+                         pairs ? inv_freq.data_ptr<float>() : nullptr, sections.data(),
+                         static_cast<int>(axes), q.size(0), q.size(2), interleaved, inverse,
+                         gp ? gp->data_ptr<float>() : nullptr, stream_of(q)),
+        "rotary_axes");
+  return {yq, yk, gp};
+}
+
+// ---- group norm -----------------------------------------------------------------
+
+struct NormShape {
+  int64_t rows, channels, frames, inner;
+};
+
+NormShape group_norm_shape(const Tensor& x, const OptTensor& offsets, const OptTensor& weight,
+                           const OptTensor& bias) {
+  TORCH_CHECK(x.dim() >= 2, "group norm input must have at least two dimensions");
+  NormShape s{};
+  s.channels = x.size(-1);
+  TORCH_CHECK(s.channels > 0, "group norm channels must be positive");
+  s.rows = x.numel() / s.channels;
+  s.frames = x.size(0);
+  s.inner = 1;
+  if (offsets) {
+    i64(*offsets, "group norm offsets");
+    same_device(x, offsets, "group norm offsets");
+    TORCH_CHECK(offsets->dim() == 1 && offsets->numel() >= 1,
+                "group norm offsets must be a one-dimensional prefix sum");
+    s.frames = offsets->numel() - 1;
+    for (int64_t d = 1; d < x.dim() - 1; ++d) s.inner *= x.size(d);
+    if (s.inner == 0) s.inner = 1;
+  }
+  for (const OptTensor* t : {&weight, &bias}) {
+    if (!t->has_value()) continue;
+    f32(**t, "group norm weight and bias");
+    same_device(x, *t, "group norm weight and bias");
+    TORCH_CHECK((*t)->numel() == s.channels, "group norm weight and bias must have shape (channels,)");
+  }
+  return s;
+}
+
+std::tuple<Tensor, Tensor, Tensor> group_norm_forward(Tensor x, int64_t groups, OptTensor weight,
+                                                      OptTensor bias, double eps,
+                                                      int64_t activation, OptTensor offsets) {
+  const int dt = value_dtype(x, "group norm input");
+  const NormShape s = group_norm_shape(x, offsets, weight, bias);
+  c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = torch::empty_like(x);
+  Tensor stats = torch::empty({2, s.frames, groups}, x.options().dtype(torch::kFloat32));
+  Tensor mean = stats.select(0, 0), rstd = stats.select(0, 1);
+  Tensor ws = workspace(
+      x, bysj_group_norm_forward_workspace_size(s.rows, s.channels, groups, s.frames));
+  check(bysj_group_norm_forward(x.data_ptr(), dt, s.rows, s.channels, groups,
+                                opt_ptr<int64_t>(offsets), s.frames, s.inner,
+                                opt_ptr<float>(weight), opt_ptr<float>(bias),
+                                static_cast<float>(eps), static_cast<int>(activation),
+                                y.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(),
+                                ws.data_ptr(), static_cast<size_t>(ws.numel()), stream_of(x)),
+        "group_norm_forward");
+  return {y, mean, rstd};
+}
+
+std::tuple<Tensor, OptTensor, OptTensor> group_norm_backward(
+    Tensor grad_out, Tensor x, int64_t groups, OptTensor weight, OptTensor bias, Tensor mean,
+    Tensor rstd, int64_t activation, OptTensor offsets, bool want_weight, bool want_bias) {
+  const int dt = value_dtype(x, "group norm input");
+  TORCH_CHECK(value_dtype(grad_out, "group norm grad_out") == dt && grad_out.sizes() == x.sizes(),
+              "group norm grad_out must match the input");
+  const NormShape s = group_norm_shape(x, offsets, weight, bias);
+  f32(mean, "group norm mean");
+  f32(rstd, "group norm rstd");
+  TORCH_CHECK(mean.numel() == s.frames * groups && rstd.numel() == mean.numel(),
+              "group norm saved statistics have an invalid shape");
+  c10::cuda::CUDAGuard guard(x.device());
+  Tensor gx = torch::empty_like(x);
+  OptTensor gw, gb;
+  if (want_weight) gw = torch::empty({s.channels}, mean.options());
+  if (want_bias) gb = torch::empty({s.channels}, mean.options());
+  Tensor ws = workspace(
+      x, bysj_group_norm_backward_workspace_size(s.rows, s.channels, groups, s.frames));
+  check(bysj_group_norm_backward(
+            grad_out.data_ptr(), x.data_ptr(), dt, s.rows, s.channels, groups,
+            opt_ptr<int64_t>(offsets), s.frames, s.inner, opt_ptr<float>(weight),
+            opt_ptr<float>(bias), mean.data_ptr<float>(), rstd.data_ptr<float>(),
+            static_cast<int>(activation), gx.data_ptr(), gw ? gw->data_ptr<float>() : nullptr,
+            gb ? gb->data_ptr<float>() : nullptr, ws.data_ptr(),
+            static_cast<size_t>(ws.numel()), stream_of(x)),
+        "group_norm_backward");
+  return {gx, gw, gb};
+}
+
+// ---- expert router ----------------------------------------------------------------
+
+// Returns weights, experts, counts, balance, z, and for the backward pass
+// z_scale, denom and share.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> route_forward(
+    Tensor logits, int64_t k, OptTensor mask, OptTensor offsets, bool renormalize) {
+  const int dt = value_dtype(logits, "router logits");
+  TORCH_CHECK(logits.dim() == 2, "router logits must have shape (tokens, experts)");
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  if (mask) {
+    cuda_tensor(*mask, "router mask");
+    TORCH_CHECK(mask->scalar_type() == torch::kBool && mask->dim() == 1 &&
+                    mask->size(0) == tokens,
+                "router mask must be a bool tensor of shape (tokens,)");
+    same_device(logits, mask, "router mask");
+  }
+  int64_t frames = 1;
+  if (offsets) {
+    i64(*offsets, "router offsets");
+    same_device(logits, offsets, "router offsets");
+    TORCH_CHECK(offsets->dim() == 1 && offsets->numel() >= 1,
+                "router offsets must be a one-dimensional prefix sum");
+    frames = offsets->numel() - 1;
+  }
+  c10::cuda::CUDAGuard guard(logits.device());
+  const auto f32o = logits.options().dtype(torch::kFloat32);
+  const auto i64o = logits.options().dtype(torch::kInt64);
+  Tensor weights = torch::empty({tokens, k}, f32o), chosen = torch::empty({tokens, k}, i64o);
+  Tensor counts = offsets ? torch::empty({frames, experts}, i64o)
+                          : torch::empty({experts}, i64o);
+  Tensor balance = torch::empty({}, f32o), z = torch::empty({}, f32o);
+  Tensor z_scale = torch::empty({}, f32o), denom = torch::empty({tokens}, f32o);
+  Tensor share = torch::empty({frames, experts}, f32o);
+  Tensor ws = workspace(logits, bysj_route_forward_workspace_size(tokens, experts, frames));
+  check(bysj_route_forward(logits.data_ptr(), dt, tokens, experts, k,
+                           mask ? reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>())
+                                : nullptr,
+                           opt_ptr<int64_t>(offsets), frames, renormalize,
+                           weights.data_ptr<float>(), chosen.data_ptr<int64_t>(),
+                           counts.data_ptr<int64_t>(), balance.data_ptr<float>(),
+                           z.data_ptr<float>(), z_scale.data_ptr<float>(),
+                           denom.data_ptr<float>(), share.data_ptr<float>(), ws.data_ptr(),
+                           static_cast<size_t>(ws.numel()), stream_of(logits)),
+        "route_forward");
+  return {weights, chosen, counts, balance, z, z_scale, denom, share};
+}
+
+Tensor route_backward(Tensor logits, int64_t k, OptTensor offsets, bool renormalize,
+                      Tensor weights, Tensor experts, Tensor denom, Tensor share, Tensor z_scale,
+                      OptTensor grad_weights, OptTensor grad_balance, OptTensor grad_z) {
+  const int dt = value_dtype(logits, "router logits");
+  const int64_t tokens = logits.size(0), n_experts = logits.size(1);
+  f32(weights, "router weights");
+  i64(experts, "router experts");
+  f32(denom, "router denom");
+  f32(share, "router share");
+  f32(z_scale, "router z_scale");
+  TORCH_CHECK(weights.numel() == tokens * k && experts.numel() == tokens * k &&
+                  denom.numel() == tokens && z_scale.numel() == 1 &&
+                  share.numel() == (offsets ? offsets->numel() - 1 : 1) * n_experts,
+              "router saved tensors have an invalid shape");
+  if (grad_weights) {
+    f32(*grad_weights, "router grad_weights");
+    TORCH_CHECK(grad_weights->numel() == tokens * k, "router grad_weights must match the weights");
+  }
+  if (grad_balance) f32(*grad_balance, "router grad_balance");
+  if (grad_z) f32(*grad_z, "router grad_z");
+  c10::cuda::CUDAGuard guard(logits.device());
+  Tensor grad = torch::empty_like(logits);
+  check(bysj_route_backward(logits.data_ptr(), dt, tokens, n_experts, k,
+                            opt_ptr<int64_t>(offsets), share.numel() / n_experts, renormalize,
+                            weights.data_ptr<float>(), experts.data_ptr<int64_t>(),
+                            denom.data_ptr<float>(), share.data_ptr<float>(),
+                            z_scale.data_ptr<float>(), opt_ptr<float>(grad_weights),
+                            opt_ptr<float>(grad_balance), opt_ptr<float>(grad_z),
+                            grad.data_ptr(), stream_of(logits)),
+        "route_backward");
+  return grad;
+}
+
+// ---- AdamW ---------------------------------------------------------------------------
+
+// One step over the parameters that have a gradient.  begins[i]: element at
+// which tensor i's states begin (a multiple of BYSJ_ADAMW_BLOCK).
+void adamw_step(const std::vector<Tensor>& params, const std::vector<OptTensor>& grads,
+                const std::vector<int64_t>& begins, Tensor exp_avg, Tensor exp_avg_sq,
+                OptTensor exp_avg_scale, OptTensor exp_avg_sq_scale, OptTensor master,
+                OptTensor grad_scale, double beta1, double beta2, double decay, double size,
+                double correct, double eps) {
+  TORCH_CHECK(params.size() == grads.size() && params.size() == begins.size(),
+              "AdamW needs one gradient (or None) for each parameter");
+  cuda_tensor(exp_avg, "AdamW exp_avg");
+  cuda_tensor(exp_avg_sq, "AdamW exp_avg_sq");
+  const bool bytes = exp_avg.scalar_type() == torch::kUInt8;
+  TORCH_CHECK((bytes || exp_avg.scalar_type() == torch::kFloat32) &&
+                  exp_avg_sq.scalar_type() == exp_avg.scalar_type() &&
+                  exp_avg_sq.numel() == exp_avg.numel(),
+              "AdamW states must be float32 or uint8 buffers of one length");
+  const int64_t length = exp_avg.numel();
+  if (bytes) {
+    TORCH_CHECK(exp_avg_scale && exp_avg_sq_scale, "AdamW 8-bit states need their scales");
+    for (const OptTensor* t : {&exp_avg_scale, &exp_avg_sq_scale}) {
+      f32(**t, "AdamW scales");
+      TORCH_CHECK((*t)->numel() * BYSJ_ADAMW_BLOCK == length, "AdamW scales: one for each block");
+    }
+  }
+  if (master) {
+    f32(*master, "AdamW master");
+    TORCH_CHECK(master->numel() == length, "AdamW master must have the states' length");
+  }
+  if (grad_scale) f32(*grad_scale, "AdamW grad_scale");
+  for (const OptTensor* t : {&exp_avg_scale, &exp_avg_sq_scale, &master, &grad_scale})
+    same_device(exp_avg, *t, "AdamW state");
+  const bysj_adamw_hyper hyper{
+      static_cast<float>(beta1), static_cast<float>(1.0 - beta1), static_cast<float>(beta2),
+      static_cast<float>(1.0 - beta2), static_cast<float>(decay), static_cast<float>(size),
+      static_cast<float>(correct), static_cast<float>(eps)};
+  std::vector<bysj_adamw_tensor> table[2];
+  for (size_t i = 0; i < params.size(); ++i) {
+    if (!grads[i]) continue;
+    const Tensor &p = params[i], &g = *grads[i];
+    const int dt = value_dtype(p, "AdamW parameter");
+    TORCH_CHECK(g.scalar_type() == p.scalar_type() && g.numel() == p.numel() &&
+                    g.device() == p.device() && p.device() == exp_avg.device() &&
+                    g.is_contiguous(),
+                "AdamW gradient ", i, " must be contiguous with the parameter's dtype, size and "
+                "device");
+    const int64_t begin = begins[i], n = p.numel();
+    TORCH_CHECK(begin >= 0 && begin % BYSJ_ADAMW_BLOCK == 0 &&
+                    begin + (n + BYSJ_ADAMW_BLOCK - 1) / BYSJ_ADAMW_BLOCK * BYSJ_ADAMW_BLOCK <=
+                        length,
+                "AdamW parameter ", i, " does not fit the state buffers");
+    table[dt == BYSJ_BF16].push_back(
+        {p.data_ptr(), g.data_ptr(), n, begin / BYSJ_ADAMW_BLOCK});
+  }
+  c10::cuda::CUDAGuard guard(exp_avg.device());
+  for (int i = 0; i < 2; ++i) {
+    if (table[i].empty()) continue;
+    check(bysj_adamw_step(table[i].data(), static_cast<int64_t>(table[i].size()),
+                          i ? BYSJ_BF16 : BYSJ_F32, bytes ? 8 : 32, exp_avg.data_ptr(),
+                          exp_avg_sq.data_ptr(),
+                          bytes ? exp_avg_scale->data_ptr<float>() : nullptr,
+                          bytes ? exp_avg_sq_scale->data_ptr<float>() : nullptr,
+                          master ? master->data_ptr<float>() : nullptr,
+                          grad_scale ? grad_scale->data_ptr<float>() : nullptr, &hyper,
+                          stream_of(exp_avg)),
+          "adamw_step");
+  }
+}
+
+std::tuple<Tensor, Tensor> adamw_state_values(Tensor exp_avg, Tensor exp_avg_sq,
+                                              Tensor exp_avg_scale, Tensor exp_avg_sq_scale) {
+  for (const Tensor* t : {&exp_avg, &exp_avg_sq}) {
+    cuda_tensor(*t, "AdamW state");
+    TORCH_CHECK(t->scalar_type() == torch::kUInt8 && t->numel() == exp_avg.numel() &&
+                    t->numel() % BYSJ_ADAMW_BLOCK == 0,
+                "AdamW 8-bit states must be uint8 buffers of whole blocks");
+  }
+  const int64_t blocks = exp_avg.numel() / BYSJ_ADAMW_BLOCK;
+  for (const Tensor* t : {&exp_avg_scale, &exp_avg_sq_scale}) {
+    f32(*t, "AdamW scales");
+    TORCH_CHECK(t->numel() == blocks, "AdamW scales: one for each block");
+    same_device(exp_avg, *t, "AdamW scales");
+  }
+  same_device(exp_avg, exp_avg_sq, "AdamW state");
+  c10::cuda::CUDAGuard guard(exp_avg.device());
+  Tensor m = torch::empty({exp_avg.numel()}, exp_avg_scale.options());
+  Tensor v = torch::empty_like(m);
+  check(bysj_adamw_state_values(exp_avg.data_ptr<uint8_t>(), exp_avg_sq.data_ptr<uint8_t>(),
+                                exp_avg_scale.data_ptr<float>(),
+                                exp_avg_sq_scale.data_ptr<float>(), blocks, m.data_ptr<float>(),
+                                v.data_ptr<float>(), stream_of(exp_avg)),
+        "adamw_state_values");
+  return {m, v};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -852,5 +1185,23 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("force_assembly_dst_add", &force_assembly_dst_add, py::arg("grad_edge"),
         py::arg("dst_offsets"), py::arg("summed_partial"));
   m.def("group_by_key", &group_by_key, py::arg("keys"), py::arg("n_keys"));
+  m.def("rotary_axes", &rotary_axes, py::arg("q"), py::arg("k"), py::arg("positions"),
+        py::arg("inv_freq"), py::arg("sections"), py::arg("interleaved") = false,
+        py::arg("inverse") = false, py::arg("saved_q") = py::none(),
+        py::arg("saved_k") = py::none());
+  m.def("group_norm_forward", &group_norm_forward, py::arg("x"), py::arg("groups"),
+        py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("activation"),
+        py::arg("offsets"));
+  m.def("group_norm_backward", &group_norm_backward, py::arg("grad_out"), py::arg("x"),
+        py::arg("groups"), py::arg("weight"), py::arg("bias"), py::arg("mean"), py::arg("rstd"),
+        py::arg("activation"), py::arg("offsets"), py::arg("want_weight"), py::arg("want_bias"));
+  m.def("route_forward", &route_forward, py::arg("logits"), py::arg("k"), py::arg("mask"),
+        py::arg("offsets"), py::arg("renormalize"));
+  m.def("route_backward", &route_backward, py::arg("logits"), py::arg("k"), py::arg("offsets"),
+        py::arg("renormalize"), py::arg("weights"), py::arg("experts"), py::arg("denom"),
+        py::arg("share"), py::arg("z_scale"), py::arg("grad_weights"), py::arg("grad_balance"),
+        py::arg("grad_z"));
+  m.def("adamw_step", &adamw_step);
+  m.def("adamw_state_values", &adamw_state_values);
   m.def("library_version", []() { return bysj_version(); });
 }

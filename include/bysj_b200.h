@@ -465,6 +465,154 @@ BYSJ_API int bysj_gie_zonal_scatter_backward_gated(
     float* grad_zonal, float* grad_radial, float* grad_inv, void* workspace,
     size_t workspace_bytes, void* stream, const uint32_t* gate);
 
+/* ------------------------------------------------------------------------
+ * Operators of a training step.  No reference counterpart (the reference
+ * serves inference); they follow the same conventions as the entries above.
+ * ------------------------------------------------------------------------ */
+
+/* rotary_axes: rotary positions with several axes, applied to the heads of
+ * one or two tensors (queries and keys) in one launch.
+ *   theta[t, p] = positions[t, axis(p)] * inv_freq[p],  p = 0 .. pairs-1
+ *   y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin
+ * pairs = sum of sections[0 .. axes-1]; the first sections[0] pairs turn with
+ * axis 0, the next with axis 1, ...  Pair p is channels (p, p + pairs), or
+ * (2p, 2p + 1) when interleaved; channels from 2 pairs on are copied.
+ * x: [tokens, heads, dim] with the given element strides (channel stride 1);
+ * y: contiguous.  positions: [tokens, axes] float32, or int64 (rounded to
+ * float32).  inverse turns by -theta (the gradient of x).
+ * grad_positions (NULL, or float32 [tokens, axes]; only with inverse) is the
+ * gradient of float positions: saved is then the forward input of each side,
+ *   grad[t, a] = sum_{p in a} inv_freq[p] sum_h (gx2 x1 - gx1 x2),
+ * gx the unrounded gradient written to y.
+ * sections is read on the host.  A side with heads == 0 is skipped. */
+#define BYSJ_ROTARY_MAX_AXES 4
+typedef struct bysj_rotary_side {
+  const void* x;
+  void* y;
+  const void* saved;
+  int64_t heads;
+  int64_t x_token_stride, x_head_stride;
+  int64_t saved_token_stride, saved_head_stride;
+} bysj_rotary_side;
+BYSJ_API int bysj_rotary_axes(const bysj_rotary_side* q, const bysj_rotary_side* k, int dtype,
+                              const void* positions, int integer_positions,
+                              const float* inv_freq, const int64_t* sections, int axes,
+                              int64_t tokens, int64_t dim, int interleaved, int inverse,
+                              float* grad_positions, void* stream);
+
+/* group_norm: normalisation over the rows of a frame and the channels of a
+ * group, channels last, with an affine map and an activation.
+ * x / y: [rows, channels] in `dtype`.  Frame b holds the rows
+ * [offsets[b] * inner, offsets[b+1] * inner) (offsets: device int64
+ * [frames + 1]; NULL: frames of rows / frames rows each, inner unused).
+ *   mean, var over rows of the frame and channels of the group (biased)
+ *   z = (x - mean) rstd w[c] + b[c],  rstd = 1 / sqrt(var + eps),  y = act(z)
+ * weight / bias float32 [channels] or NULL; mean / rstd float32
+ * [frames, groups] are outputs for the backward pass; an empty frame has
+ * mean 0 and rstd 0. */
+BYSJ_API size_t bysj_group_norm_forward_workspace_size(int64_t rows, int64_t channels,
+                                                       int64_t groups, int64_t frames);
+BYSJ_API int bysj_group_norm_forward(const void* x, int dtype, int64_t rows, int64_t channels,
+                                     int64_t groups, const int64_t* offsets, int64_t frames,
+                                     int64_t inner, const float* weight, const float* bias,
+                                     float eps, int activation, void* y, float* mean,
+                                     float* rstd, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+/* dz = dy act'(z), d = dz w:
+ *   grad_x = rstd (d - mean(d) - xhat mean(d xhat)),
+ *   grad_weight[c] = sum dz xhat,  grad_bias[c] = sum dz  (either may be NULL). */
+BYSJ_API size_t bysj_group_norm_backward_workspace_size(int64_t rows, int64_t channels,
+                                                        int64_t groups, int64_t frames);
+BYSJ_API int bysj_group_norm_backward(const void* grad_out, const void* x, int dtype,
+                                      int64_t rows, int64_t channels, int64_t groups,
+                                      const int64_t* offsets, int64_t frames, int64_t inner,
+                                      const float* weight, const float* bias, const float* mean,
+                                      const float* rstd, int activation, void* grad_x,
+                                      float* grad_weight, float* grad_bias, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* route_experts: top-k router with per-expert counts and auxiliary losses.
+ *   p = softmax(logits[t]);  experts[t] = the k largest logits, ties to the
+ *   lowest index, NaN largest, -inf never chosen (slot -1, weight 0)
+ *   weights = p at the chosen experts, divided by their sum if renormalize
+ * A token is valid when its mask byte is non-zero (mask NULL: all) and some
+ * logit is not -inf; an invalid token's logits have no effect: experts -1,
+ * weights 0.  Frame s (offsets int64 [frames + 1], or NULL: one frame) with
+ * n_s valid tokens:
+ *   counts[s, e]  = slots of its tokens that chose e
+ *   balance = mean over s with n_s > 0 of
+ *             experts / (k n_s^2) sum_e counts[s, e] sum_{t in s} p[t, e]
+ *   z       = mean over valid tokens of logsumexp(logits[t])^2
+ * balance, z: one float each.  For the backward pass: z_scale = 2 / (number
+ * of valid tokens), 0 if none (one float); denom[t] = sum_e exp(logit -
+ * largest logit); share[s, e] = d balance / d p[t, e] for t in s.
+ * n_experts <= BYSJ_ROUTE_MAX_EXPERTS, 1 <= k <= min(n_experts, 32). */
+#define BYSJ_ROUTE_MAX_EXPERTS 1024
+#define BYSJ_ROUTE_MAX_K 32
+BYSJ_API size_t bysj_route_forward_workspace_size(int64_t tokens, int64_t n_experts,
+                                                  int64_t frames);
+BYSJ_API int bysj_route_forward(const void* logits, int dtype, int64_t tokens,
+                                int64_t n_experts, int64_t k, const uint8_t* mask,
+                                const int64_t* offsets, int64_t frames, int renormalize,
+                                float* weights, int64_t* experts, int64_t* counts,
+                                float* balance, float* z, float* z_scale, float* denom,
+                                float* share, void* workspace, size_t workspace_bytes,
+                                void* stream);
+/* grad_logits (dtype of logits) from grad_weights [tokens, k], grad_balance
+ * and grad_z (device float32 scalars); any of the three may be NULL (zero). */
+BYSJ_API int bysj_route_backward(const void* logits, int dtype, int64_t tokens,
+                                 int64_t n_experts, int64_t k, const int64_t* offsets,
+                                 int64_t frames, int renormalize, const float* weights,
+                                 const int64_t* experts, const float* denom,
+                                 const float* share, const float* z_scale,
+                                 const float* grad_weights, const float* grad_balance,
+                                 const float* grad_z, void* grad_logits, void* stream);
+
+/* adamw: one decoupled-weight-decay Adam step over many tensors.
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = decay p - size m / (correct sqrt(v) + eps)
+ * g = grad * *grad_scale (device float32, NULL: 1).  Every operation is
+ * rounded to float32 on its own, so results do not depend on contraction.
+ * Tensor i has n elements (params / grads contiguous, dtype `dtype`); its
+ * states and master copy begin at element BYSJ_ADAMW_BLOCK * first_block of
+ * the shared buffers exp_avg, exp_avg_sq and master (NULL, or float32: then p
+ * is read from and written to it and params get the rounded copy).  The
+ * elements up to the next block boundary belong to the tensor and stay zero.
+ * state_bits 32: float32 states, scales unused.  state_bits 8: one byte per
+ * element and one float32 scale per block of BYSJ_ADAMW_BLOCK elements:
+ *   m: bit 7 sign, low 7 bits a magnitude code with 3 mantissa bits
+ *   sqrt(v): an 8-bit code with 4 mantissa bits
+ * code c > 0 stands for scale * value(c), value(top) = 1, each step one unit
+ * in the last mantissa bit (value = float with the bits
+ * (c - top + (127 << mantissa)) << (23 - mantissa)); code 0 for 0.
+ * tensors is read on the host. */
+#define BYSJ_ADAMW_BLOCK 256
+typedef struct bysj_adamw_tensor {
+  void* param;
+  const void* grad;
+  int64_t n;
+  int64_t first_block;
+} bysj_adamw_tensor;
+typedef struct bysj_adamw_hyper {
+  float beta1, one_minus_beta1, beta2, one_minus_beta2;
+  float decay;   /* 1 - lr weight_decay */
+  float size;    /* lr / (1 - beta1^step) */
+  float correct; /* 1 / sqrt(1 - beta2^step) */
+  float eps;
+} bysj_adamw_hyper;
+BYSJ_API int bysj_adamw_step(const bysj_adamw_tensor* tensors, int64_t n_tensors, int dtype,
+                             int state_bits, void* exp_avg, void* exp_avg_sq,
+                             float* exp_avg_scale, float* exp_avg_sq_scale, float* master,
+                             const float* grad_scale, const bysj_adamw_hyper* hyper,
+                             void* stream);
+/* The float32 values that 8-bit states stand for (blocks * BYSJ_ADAMW_BLOCK
+ * elements each): m = scale value, v = (scale value)^2. */
+BYSJ_API int bysj_adamw_state_values(const uint8_t* exp_avg, const uint8_t* exp_avg_sq,
+                                     const float* exp_avg_scale,
+                                     const float* exp_avg_sq_scale, int64_t blocks,
+                                     float* exp_avg_values, float* exp_avg_sq_values,
+                                     void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif
