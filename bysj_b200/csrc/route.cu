@@ -9,12 +9,22 @@
 //   dlogit_e = p_e (a_e - sum_j p_j a_j) + 2 / n grad_z lse p_e
 //   and, for renormalised weights w, + w_i (gw_i - sum_j w_j gw_j) at expert i.
 //
-// One warp per token with the row in registers.  Largest logits are found in
-// an order-preserving integer form by warp-wide integer reductions; ties go to
-// the lowest index.  P and the counts are sums of integers: p is rounded to a
-// multiple of 2^-shift (shift such that all tokens fit 62 bits, 40 at most),
-// so integer atomics give the same sum in any order, with an absolute error
-// of 2^-shift a token, below that of a float sum.
+// A group of L lanes holds a token's row in registers (M logits a lane), so a
+// warp routes 32 / L tokens at once.  The row's order is that of unsigned keys
+// with the column in the low bits: a key is unique, ties fall to the lowest
+// column, and the next largest below `prev` is the maximum of key - prev in
+// wrapping arithmetic (the keys still to come wrap to the top), one
+// add-and-max instruction a logit and slot.  A bfloat16 logit and its column
+// fit 32 bits; a float32 key drops as many mantissa bits as the column needs,
+// and a warp in which two neighbours of the order agree in what is left, or in
+// which a NaN occurs, orders its tokens again by full value and column.
+//
+// P and the counts are sums of integers.  A lane adds its columns' p over the
+// tokens of a piece (the part of a frame inside a CTA's range) in float32; a
+// CTA adds its warps in their order, rounds to a multiple of 2^-shift (shift
+// such that all tokens fit 62 bits, 40 at most) and adds that to the frame's
+// total.  Integer atomics give the same sum in any order, so results repeat
+// bit for bit.
 #include "launch.cuh"
 
 namespace bysj {
@@ -37,11 +47,20 @@ struct RouteArgs {
   float* denom;
   float* share;
   unsigned long long* mass;    // [frames][experts] sum of p in units of 2^-shift
+  unsigned long long* taken;   // [frames][experts] slots
   unsigned long long* number;  // [frames] valid tokens
   unsigned* poison;            // a probability was not a number
+  unsigned* ticket;
+  int64_t zeroed;              // words from mass on that start at 0
   double* square;              // [CTAs] sum of lse^2
+  double* part;                // [CTAs of the losses kernel]
   int shift;
   int ctas;
+  int64_t tokens_per_cta;
+  bool fused_losses;
+  unsigned column_mask;        // key bits that hold the column
+  int k_magic;                 // it / k == (it k_magic) >> 16 for it < 32 k
+  size_t stage_bytes;
   const float* grad_weights;
   const float* grad_balance;
   const float* grad_z;
@@ -57,13 +76,27 @@ __device__ __forceinline__ void store_value(__nv_bfloat16* p, float v) {
   *p = __float2bfloat16_rn(v);
 }
 
-// Unsigned key in the order of the logits, with 0 for -inf (never chosen) and
-// NaN above all; + 0.0f makes the two zeros equal.
-__device__ __forceinline__ unsigned order_key(float v) {
-  if (v == -INFINITY) return 0u;
-  if (isnan(v)) return 0xffffffffu;
-  const unsigned b = __float_as_uint(v + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+template <int V>
+__device__ __forceinline__ void store_vec(float* p, const float (&v)[V]) {
+  if constexpr (V == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else p[0] = v[0];
+}
+template <int V>
+__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&v)[V]) {
+  if constexpr (V == 8) {
+    __nv_bfloat162 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+  } else {
+    p[0] = __float2bfloat16_rn(v[0]);
+  }
+}
+template <int V, typename T>
+__device__ __forceinline__ void copy_vec(T* to, const T* from) {
+  if constexpr (V * sizeof(T) == 16)
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+  else *to = *from;
 }
 
 // Frame of token t: the last whose offset is <= t.
@@ -78,105 +111,97 @@ __device__ __forceinline__ int64_t frame_of(const RouteArgs& a, int64_t t) {
   return lo;
 }
 
-__device__ __forceinline__ float warp_max(float v) { return xor_max(v, 1); }
-__device__ __forceinline__ float warp_sum(float v) { return xor_sum(v, 1); }
+__device__ __forceinline__ int64_t frame_end(const RouteArgs& a, int64_t s) {
+  return a.offsets == nullptr || s + 1 >= a.frames ? a.tokens : __ldg(a.offsets + s + 1);
+}
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(kBlock) route_forward_kernel(RouteArgs a) {
-  __shared__ double s_square[kWarpsPerBlock];
-  const int lane = lane_id();
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
-  const float unit = static_cast<float>(int64_t{1} << a.shift);
-  double square = 0.0;
-  for (int64_t t = global_warp(); t < a.tokens; t += warps) {
-    const T* row = static_cast<const T*>(a.logits) + t * a.experts;
-    const bool on = a.mask == nullptr || __ldg(a.mask + t) != 0;
-    float x[NV];
-    unsigned key[NV];
-    float top = -INFINITY;
-    unsigned any = 0;
+// The logits of one token that a lane holds: NV vectors of V, element i of
+// vector v at column (v L + l) V + i, as loaded (a bfloat16 row in flight
+// takes half the registers).
+template <typename T, int V, int NV, int L>
+struct Row {
+  RowVec<T, V> v[NV];
+  __device__ __forceinline__ void load(const T* row, int l, int experts, bool on) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = lane + i * kWarp;
-      x[i] = on && e < a.experts ? load_f32(row + e) : -INFINITY;
-      key[i] = order_key(x[i]);
-      any |= key[i];
-      top = fmaxf(top, x[i]);
-    }
-    top = warp_max(top);
-    const bool valid = __any_sync(kFull, any != 0);
-    if (!valid) {
-      for (int i = lane; i < a.k; i += kWarp) {
-        a.weights[t * a.k + i] = 0.0f;
-        a.chosen[t * a.k + i] = -1;
-      }
-      if (lane == 0) a.denom[t] = 1.0f;
-      continue;
-    }
-    float total = 0.0f, p[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      p[i] = x[i] == -INFINITY ? 0.0f : expf(x[i] - top);
-      total += p[i];
-    }
-    total = warp_sum(total);
-    const int64_t s = frame_of(a, t);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = lane + i * kWarp;
-      p[i] /= total;
-      if (e < a.experts && p[i] != 0.0f) {
-        if (isnan(p[i])) atomicOr(a.poison, 1u);
-        else atomicAdd(a.mass + s * a.experts + e, static_cast<unsigned long long>(
-                                                       __float2ull_rn(p[i] * unit)));
-      }
-    }
-    // k times the largest remaining key, the lowest index among equals; lane i
-    // keeps slot i
-    float mine = 0.0f, picked = 0.0f;
-    int64_t index = -1;
-    for (int slot = 0; slot < a.k; ++slot) {
-      unsigned best = 0;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) best = max(best, key[i]);
-      best = __reduce_max_sync(kFull, best);
-      if (best == 0) break;
-      unsigned where = 0xffffffffu;
-#pragma unroll
-      for (int i = NV - 1; i >= 0; --i)
-        if (key[i] == best) where = lane + i * kWarp;
-      where = __reduce_min_sync(kFull, where);
-      float value = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (lane + i * kWarp == static_cast<int>(where)) {
-          key[i] = 0;
-          value = p[i];
-          atomicAdd(reinterpret_cast<unsigned long long*>(a.counts) + s * a.experts + where, 1ull);
-        }
-      value = __shfl_sync(kFull, value, where & 31);
-      picked += value;
-      if (lane == slot) {
-        mine = value;
-        index = where;
-      }
-    }
-    if (lane < a.k) {
-      a.weights[t * a.k + lane] = a.renormalize && index >= 0 ? mine / picked : mine;
-      a.chosen[t * a.k + lane] = index;
-    }
-    if (lane == 0) {
-      a.denom[t] = total;
-      atomicAdd(a.number + s, 1ull);
-      const float lse = top + logf(total);
-      square += static_cast<double>(lse) * lse;
+    for (int n = 0; n < NV; ++n) {
+      const int c = (n * L + l) * V;
+      if (on && c < experts) v[n].load(row, n * L + l);
+      else fill(v[n]);
     }
   }
-  if (lane == 0) s_square[threadIdx.x / kWarp] = square;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kWarpsPerBlock; ++i) square += s_square[i];
-    a.square[blockIdx.x] = square;
+  __device__ __forceinline__ float get(int i) const { return v[i / V].get(i % V); }
+  __device__ static constexpr int column(int i, int l) { return ((i / V) * L + l) * V + i % V; }
+  // -inf: what lies beyond the row's end, or belongs to a token left out
+  __device__ static __forceinline__ void fill(RowVec<float, 4>& r) {
+    r.r = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  }
+  __device__ static __forceinline__ void fill(RowVec<float, 1>& r) { r.r = -INFINITY; }
+  __device__ static __forceinline__ void fill(RowVec<__nv_bfloat16, 8>& r) {
+    r.r = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+  }
+  __device__ static __forceinline__ void fill(RowVec<__nv_bfloat16, 1>& r) { r.r = 0xff80u; }
+};
+
+template <int L>
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+  for (int s = 1; s < L; s <<= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, s));
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int s = 1; s < L; s <<= 1) v += __shfl_xor_sync(kFull, v, s);
+  return v;
+}
+template <int L>
+__device__ __forceinline__ unsigned row_max(unsigned v) {
+#pragma unroll
+  for (int s = 1; s < L; s <<= 1) v = max(v, __shfl_xor_sync(kFull, v, s));
+  return v;
+}
+
+// Bits of a float in the order of the values; + 0.0f makes the two zeros equal.
+__device__ __forceinline__ unsigned order_bits(float v) {
+  const unsigned b = __float_as_uint(v + 0.0f);
+  return b ^ (static_cast<unsigned>(static_cast<int>(b) >> 31) | 0x80000000u);
+}
+constexpr unsigned kBarred = 0x007fffffu;  // order_bits(-inf)
+
+// Exact order for a warp's rows: the next in (value, then column) after
+// (prev, at); NaN is largest.  Slow: two reductions a slot.
+template <typename T, int V, int NV, int L>
+__device__ __noinline__ void pick_exact(const Row<T, V, NV, L>& row, int l, int experts, int k,
+                                        unsigned* picks) {
+  constexpr int M = V * NV;
+  unsigned prev = 0;
+  int at = -1;
+  for (int slot = 0; slot < k; ++slot) {
+    unsigned best = 0;
+    int where = 0x7fffffff;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const int c = row.column(i, l);
+      const float x = row.get(i);
+      const unsigned key = c >= experts ? 0u : isnan(x) ? 0xffffffffu : order_bits(x);
+      const bool left = slot == 0 || key < prev || (key == prev && c > at);
+      if (left && (key > best || (key == best && c < where))) {
+        best = key;
+        where = c;
+      }
+    }
+#pragma unroll
+    for (int s = 1; s < L; s <<= 1) {
+      const unsigned other = __shfl_xor_sync(kFull, best, s);
+      const int there = __shfl_xor_sync(kFull, where, s);
+      if (other > best || (other == best && there < where)) {
+        best = other;
+        where = there;
+      }
+    }
+    if (l == 0) picks[slot] = best <= kBarred ? 0xffffffffu : static_cast<unsigned>(where);
+    prev = best;
+    at = where;
   }
 }
 
@@ -190,119 +215,452 @@ __device__ __forceinline__ double block_sum(double v, double* scratch) {
   return total;
 }
 
-__global__ void __launch_bounds__(kBlock) route_losses_kernel(RouteArgs a) {
+// share, counts and the losses from the totals, by CTA `cta` of `ctas`; reads
+// through L2, where the other CTAs' totals are.
+__device__ void route_losses(const RouteArgs& a, int cta, int ctas) {
   __shared__ double scratch[kWarpsPerBlock];
-  double used = 0.0, valid = 0.0, square = 0.0, balance = 0.0;
+  __shared__ bool s_join;
+  double used = 0.0, valid = 0.0;
   for (int64_t s = threadIdx.x; s < a.frames; s += kBlock) {
-    used += a.number[s] > 0;
-    valid += static_cast<double>(a.number[s]);
+    const unsigned long long n = __ldcg(a.number + s);
+    used += n > 0;
+    valid += static_cast<double>(n);
   }
-  for (int i = threadIdx.x; i < a.ctas; i += kBlock) square += a.square[i];
   used = block_sum(used, scratch);
   valid = block_sum(valid, scratch);
-  square = block_sum(square, scratch);
   const double unit = 1.0 / static_cast<double>(int64_t{1} << a.shift);
-  for (int64_t i = threadIdx.x; i < a.frames * a.experts; i += kBlock) {
-    const double n = static_cast<double>(a.number[i / a.experts]);
+  double balance = 0.0;
+  for (int64_t i = static_cast<int64_t>(cta) * kBlock + threadIdx.x; i < a.frames * a.experts;
+       i += static_cast<int64_t>(ctas) * kBlock) {
+    const double n = static_cast<double>(__ldcg(a.number + i / a.experts));
+    const unsigned long long taken = __ldcg(a.taken + i);
     const double share =
-        n > 0.0 ? a.experts * static_cast<double>(a.counts[i]) / (a.k * n * n * used) : 0.0;
+        n > 0.0 ? a.experts * static_cast<double>(taken) / (a.k * n * n * used) : 0.0;
     a.share[i] = static_cast<float>(share);
-    balance += share * (static_cast<double>(a.mass[i]) * unit);
+    a.counts[i] = static_cast<int64_t>(taken);
+    balance += share * (static_cast<double>(__ldcg(a.mass + i)) * unit);
   }
   balance = block_sum(balance, scratch);
+  if (ctas > 1) {  // join the CTAs' parts in their order
+    if (threadIdx.x == 0) {
+      __stcg(a.part + cta, balance);
+      __threadfence();
+      s_join = atomicAdd(a.ticket, 1u) + 1 == static_cast<unsigned>(ctas);
+      __threadfence();
+    }
+    __syncthreads();
+    if (!s_join) return;
+    balance = 0.0;
+    for (int i = threadIdx.x; i < ctas; i += kBlock) balance += __ldcg(a.part + i);
+    balance = block_sum(balance, scratch);
+  }
+  double square = 0.0;
+  for (int i = threadIdx.x; i < a.ctas; i += kBlock) square += __ldcg(a.square + i);
+  square = block_sum(square, scratch);
   if (threadIdx.x == 0) {
-    *a.balance = *a.poison ? NAN : static_cast<float>(balance);
+    *a.balance = __ldcg(a.poison) ? NAN : static_cast<float>(balance);
     *a.z = valid > 0.0 ? static_cast<float>(square / valid) : 0.0f;
     *a.z_scale = valid > 0.0 ? static_cast<float>(2.0 / valid) : 0.0f;
   }
 }
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(kBlock) route_backward_kernel(RouteArgs a) {
-  const int lane = lane_id();
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
-  const float gb = a.grad_balance ? __ldg(a.grad_balance) : 0.0f;
-  const float gz = a.grad_z ? __ldg(a.grad_z) * *a.z_scale : 0.0f;
-  for (int64_t t = global_warp(); t < a.tokens; t += warps) {
-    const T* row = static_cast<const T*>(a.logits) + t * a.experts;
-    T* out = static_cast<T*>(a.grad_logits) + t * a.experts;
-    const int64_t first = a.chosen[t * a.k];
-    if (first < 0) {  // not a valid token
-      for (int e = lane; e < a.experts; e += kWarp) store_value(out + e, 0.0f);
+// Shared memory of the forward kernel, per CTA: counts [E], one row of mass a
+// warp [warps][E], and per warp the picks and their values [32 / L][k].
+template <typename T, int V, int NV, int L>
+__global__ void __launch_bounds__(kBlock) route_forward_kernel(RouteArgs a) {
+  constexpr int M = V * NV, R = kWarp / L;
+  using RowT = Row<T, V, NV, L>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int E = a.experts, k = a.k, items = R * k;
+  unsigned* s_count = reinterpret_cast<unsigned*>(smem);
+  float* s_mass = reinterpret_cast<float*>(s_count + E);
+  unsigned* s_pick = reinterpret_cast<unsigned*>(s_mass + kWarpsPerBlock * E);
+  const int lane = lane_id(), warp = threadIdx.x / kWarp, l = lane % L, g = lane / L;
+  unsigned* picks = s_pick + warp * 2 * items;
+  float* values = reinterpret_cast<float*>(picks + items);
+  __shared__ double s_square[kWarpsPerBlock];
+  __shared__ int s_valid[kWarpsPerBlock];
+  __shared__ bool s_last;
+  const T* logits = static_cast<const T*>(a.logits);
+  const float unit = static_cast<float>(int64_t{1} << a.shift);
+  const int64_t t0 = a.tokens_per_cta * blockIdx.x;
+  const int64_t t1 = min(t0 + a.tokens_per_cta, a.tokens);
+
+  if (gridDim.x == 1) {  // alone: no memset ran before
+    for (int64_t i = threadIdx.x; i < a.zeroed; i += kBlock) a.mass[i] = 0;
+  }
+  for (int i = threadIdx.x; i < E; i += kBlock) s_count[i] = 0;
+  __syncthreads();
+
+  double square = 0.0;
+  int64_t s = t0 < t1 ? frame_of(a, t0) : 0;
+  for (int64_t lo = t0; lo < t1; ++s) {
+    const int64_t hi = min(frame_end(a, s), t1);
+    if (hi <= lo) {
+      if (s + 1 >= a.frames) break;
       continue;
     }
-    const float top = load_f32(row + first), total = a.denom[t];
-    const int64_t s = frame_of(a, t);
-    float p[NV], cot[NV], direct[NV];
+    float mass[M];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = lane + i * kWarp;
-      const float x = e < a.experts ? load_f32(row + e) : -INFINITY;
-      p[i] = x == -INFINITY ? 0.0f : expf(x - top) / total;
-      cot[i] = e < a.experts ? gb * a.share[s * a.experts + e] : 0.0f;
-      direct[i] = 0.0f;
-    }
-    if (a.grad_weights != nullptr) {
-      const float gw = lane < a.k ? a.grad_weights[t * a.k + lane] : 0.0f;
-      const float w = lane < a.k ? a.weights[t * a.k + lane] : 0.0f;
-      const int index = lane < a.k ? static_cast<int>(a.chosen[t * a.k + lane]) : -1;
-      const float along = a.renormalize ? warp_sum(w * gw) : 0.0f;
-      for (int slot = 0; slot < a.k; ++slot) {
-        const int e = __shfl_sync(kFull, index, slot);
-        const float g = __shfl_sync(kFull, a.renormalize ? w * (gw - along) : gw, slot);
+    for (int i = 0; i < M; ++i) mass[i] = 0.0f;
+    int valid_rows = 0;
+    auto fetch = [&](int64_t base, RowT& row) {
+      const int64_t t = base + g;
+      const bool on = t < hi && (a.mask == nullptr || __ldg(a.mask + t) != 0);
+      row.load(logits + t * E, l, E, on);
+    };
+    RowT next;
+    fetch(lo + warp * R, next);
+    for (int64_t base = lo + warp * R; base < hi; base += kWarpsPerBlock * R) {
+      const RowT row = next;
+      if (base + kWarpsPerBlock * R < hi) fetch(base + kWarpsPerBlock * R, next);
+      float top = row.get(0);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (lane + i * kWarp == e) {
-            if (a.renormalize) direct[i] = g;
-            else cot[i] += g;
+      for (int i = 1; i < M; ++i) top = fmaxf(top, row.get(i));
+      top = row_max<L>(top);
+      const float ref = top > -INFINITY ? top : 0.0f;
+      float e[M], total = 0.0f;
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        e[i] = __expf(row.get(i) - ref);
+        total += e[i];
+      }
+      total = row_sum<L>(total);
+      const bool valid = total != 0.0f;  // NaN counts; 0: every logit is -inf
+      const float inv = valid ? 1.0f / total : 0.0f;
+#pragma unroll
+      for (int i = 0; i < M; ++i) mass[i] = fmaf(e[i], inv, mass[i]);
+
+      // the order: V columns of a vector lie side by side, so one subtraction
+      // gives the column part of each key
+      unsigned key[M];
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const int c = RowT::column(i, l);
+        const unsigned bits = order_bits(row.get(i));
+        key[i] = c < E ? (bits & ~a.column_mask) | (a.column_mask - c) : 0u;
+      }
+      unsigned prev = 0;
+      bool unclear = isnan(total);
+      constexpr bool kExact = sizeof(T) == 2;
+      const int rounds = kExact ? k : k + 1;  // one more: is the last one clear?
+      for (int slot = 0; slot < rounds; ++slot) {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < M; ++i) m = __viaddmax_u32(key[i], 0u - prev, m);
+        const unsigned best = row_max<L>(m) + prev;
+        if constexpr (!kExact)
+          unclear |= slot > 0 && best < prev && (best | a.column_mask) == (prev | a.column_mask) &&
+                     (best | a.column_mask) > (kBarred | a.column_mask);
+        if (l == 0 && slot < k)
+          picks[g * k + slot] = (best | a.column_mask) <= (kBarred | a.column_mask)
+                                    ? 0xffffffffu
+                                    : a.column_mask - (best & a.column_mask);
+        prev = best;
+      }
+      if (__any_sync(kFull, unclear)) pick_exact<T, V, NV, L>(row, l, E, k, picks + g * k);
+      __syncwarp();
+
+      // weights and indices, the warp's R k slots side by side
+      for (int it0 = 0; it0 < items; it0 += kWarp) {
+        const int it = it0 + lane;
+        const int r = min((it * a.k_magic) >> 16, R - 1);
+        const float ref_r = __shfl_sync(kFull, ref, r * L), inv_r = __shfl_sync(kFull, inv, r * L);
+        const int64_t t = base + r;
+        if (it < items) {
+          const unsigned c = picks[it];
+          float p = 0.0f;
+          if (t < hi && c != 0xffffffffu) {
+            p = __expf(load_f32(logits + t * E + c) - ref_r) * inv_r;
+            atomicAdd(s_count + c, 1u);
           }
+          values[it] = p;
+        }
+      }
+      __syncwarp();
+      for (int it = lane; it < items; it += kWarp) {
+        const int r = (it * a.k_magic) >> 16;
+        const int64_t t = base + r;
+        if (t < hi) {
+          float w = values[it];
+          const unsigned c = picks[it];
+          if (a.renormalize && c != 0xffffffffu) {
+            float sum = 0.0f;
+            for (int j = 0; j < k; ++j) sum += values[r * k + j];
+            w /= sum;
+          }
+          a.weights[base * k + it] = w;
+          a.chosen[base * k + it] = c == 0xffffffffu ? int64_t{-1} : static_cast<int64_t>(c);
+        }
+      }
+      if (l == 0 && base + g < hi) {
+        a.denom[base + g] = total;
+        if (valid) {
+          const float lse = ref + logf(total);
+          square += static_cast<double>(lse) * lse;
+          ++valid_rows;
+        }
+      }
+      __syncwarp();
+    }
+
+    // flush the piece into its frame's totals
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      mass[i] = xor_sum(mass[i], L);
+      const int c = RowT::column(i, l);
+      if (g == 0 && c < E) s_mass[warp * E + c] = mass[i];
+    }
+    for (int o = L; o < kWarp; o <<= 1) valid_rows += __shfl_xor_sync(kFull, valid_rows, o);
+    if (lane == 0) s_valid[warp] = valid_rows;
+    __syncthreads();
+    for (int c = threadIdx.x; c < E; c += kBlock) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarpsPerBlock; ++w) sum += s_mass[w * E + c];
+      if (isnan(sum)) atomicOr(a.poison, 1u);
+      else if (sum != 0.0f)
+        atomicAdd(a.mass + s * E + c, static_cast<unsigned long long>(__float2ull_rn(sum * unit)));
+      if (s_count[c] != 0) {
+        atomicAdd(a.taken + s * E + c, static_cast<unsigned long long>(s_count[c]));
+        s_count[c] = 0;
       }
     }
-    float along = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) along += p[i] * cot[i];
-    along = warp_sum(along);
-    const float pull = gz * (top + logf(total)) - along;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = lane + i * kWarp;
-      if (e < a.experts) store_value(out + e, p[i] * (cot[i] + pull) + direct[i]);
+    if (threadIdx.x == 0) {
+      int n = 0;
+      for (int w = 0; w < kWarpsPerBlock; ++w) n += s_valid[w];
+      if (n != 0) atomicAdd(a.number + s, static_cast<unsigned long long>(n));
     }
+    __syncthreads();
+    lo = hi;
+  }
+
+  square = xor_sum(square, 1);
+  if (lane == 0) s_square[warp] = square;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    square = 0.0;
+    for (int w = 0; w < kWarpsPerBlock; ++w) square += s_square[w];
+    __stcg(a.square + blockIdx.x, square);
+  }
+  if (!a.fused_losses) return;
+  // the last CTA to arrive turns the totals into the losses
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(a.ticket, 1u) + 1 == gridDim.x;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  route_losses(a, 0, 1);
+}
+
+__global__ void __launch_bounds__(kBlock) route_losses_kernel(RouteArgs a) {
+  route_losses(a, blockIdx.x, gridDim.x);
+}
+
+// Shared memory, per CTA: the cotangents share[s, e] grad_balance [E]; per warp
+// the slots' products [32 / L][k] and the rows on their way out [32 / L][E].
+template <typename T, int V, int NV, int L>
+__global__ void __launch_bounds__(kBlock) route_backward_kernel(RouteArgs a) {
+  constexpr int M = V * NV, R = kWarp / L;
+  using RowT = Row<T, V, NV, L>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int E = a.experts, k = a.k, items = R * k;
+  const int lane = lane_id(), warp = threadIdx.x / kWarp, l = lane % L, g = lane / L;
+  T* stage = reinterpret_cast<T*>(smem) + warp * R * E;
+  float* s_cot = reinterpret_cast<float*>(smem + a.stage_bytes);
+  float* values = s_cot + E + warp * items;
+  const T* logits = static_cast<const T*>(a.logits);
+  T* out = static_cast<T*>(a.grad_logits);
+  const float gb = a.grad_balance ? __ldg(a.grad_balance) : 0.0f;
+  const float gz = a.grad_z ? __ldg(a.grad_z) * __ldg(a.z_scale) : 0.0f;
+  const int64_t t0 = a.tokens_per_cta * blockIdx.x;
+  const int64_t t1 = min(t0 + a.tokens_per_cta, a.tokens);
+  int64_t s = t0 < t1 ? frame_of(a, t0) : 0;
+  for (int64_t lo = t0; lo < t1; ++s) {
+    const int64_t hi = min(frame_end(a, s), t1);
+    if (hi <= lo) {
+      if (s + 1 >= a.frames) break;
+      continue;
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < E; c += kBlock) s_cot[c] = gb * __ldg(a.share + s * E + c);
+    __syncthreads();
+    float cot[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const int c = RowT::column(i, l);
+      cot[i] = c < E ? s_cot[c] : 0.0f;
+    }
+    for (int64_t base = lo + warp * R; base < hi; base += kWarpsPerBlock * R) {
+      const int64_t t = base + g;
+      const bool in = t < hi;
+      RowT row;
+      row.load(logits + t * E, l, E, in);
+      const bool valid = in && __ldg(a.chosen + t * k) >= 0;
+      const float total = in ? __ldg(a.denom + t) : 1.0f;
+      const float inv = 1.0f / total;
+      float top = row.get(0);
+#pragma unroll
+      for (int i = 1; i < M; ++i) top = fmaxf(top, row.get(i));
+      top = row_max<L>(top);
+      const float ref = top > -INFINITY ? top : 0.0f;
+      float along_w = 0.0f;
+      if (a.grad_weights != nullptr) {
+        for (int it0 = 0; it0 < items; it0 += kWarp) {
+          const int it = it0 + lane;
+          if (it < items && base + ((it * a.k_magic) >> 16) < hi)
+            values[it] = __ldg(a.weights + base * k + it) * __ldg(a.grad_weights + base * k + it);
+          else if (it < items)
+            values[it] = 0.0f;
+        }
+        __syncwarp();
+        for (int j = 0; j < k; ++j) along_w += values[g * k + j];
+      }
+      // p_e a_e and its sum; a weight that is p itself adds gw p at its expert
+      float p[M], pc[M], along = 0.0f;
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        p[i] = __expf(row.get(i) - ref) * inv;
+        pc[i] = p[i] * cot[i];
+        along += pc[i];
+      }
+      along = row_sum<L>(along);
+      if (!a.renormalize) along += along_w;
+      const float pull = gz * (ref + logf(total)) - along;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int c = (n * L + l) * V;
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          v[i] = fmaf(p[n * V + i], pull, pc[n * V + i]);
+          if (!valid) v[i] = 0.0f;
+        }
+        if (c < E) store_vec<V>(stage + g * E + c, v);
+      }
+      if (a.grad_weights != nullptr) {
+        __syncwarp();
+        // the chosen experts once more, with the weights' part
+        for (int it0 = 0; it0 < items; it0 += kWarp) {
+          const int it = it0 + lane;
+          const int r = min((it * a.k_magic) >> 16, R - 1);
+          const float ref_r = __shfl_sync(kFull, ref, r * L);
+          const float inv_r = __shfl_sync(kFull, inv, r * L);
+          const float pull_r = __shfl_sync(kFull, pull, r * L);
+          const float along_r = __shfl_sync(kFull, along_w, r * L);
+          if (it < items && base + r < hi) {
+            const int64_t c = __ldg(a.chosen + base * k + it);
+            if (c >= 0) {
+              const float gw = __ldg(a.grad_weights + base * k + it);
+              const float pe = __expf(load_f32(logits + (base + r) * E + c) - ref_r) * inv_r;
+              const float value =
+                  a.renormalize
+                      ? fmaf(pe, s_cot[c] + pull_r,
+                             __ldg(a.weights + base * k + it) * (gw - along_r))
+                      : pe * (s_cot[c] + gw + pull_r);
+              store_value(stage + r * E + c, value);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (in) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+          const int c = (n * L + l) * V;
+          if (c < E) copy_vec<V>(out + t * E + c, stage + g * E + c);
+        }
+      }
+      __syncwarp();
+    }
+    lo = hi;
   }
 }
 
-int route_ctas(int64_t tokens) {
-  int64_t blocks = (tokens + kWarpsPerBlock - 1) / kWarpsPerBlock;
-  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 8;
-  if (blocks > cap) blocks = cap;
-  return blocks < 1 ? 1 : static_cast<int>(blocks);
+// Launch shapes by the number of experts: L lanes a token and M logits a lane.
+// Few lanes a token mean few shuffles a slot; M = 16 keeps keys, exponentials
+// and masses in registers.  Rows whose length is not a multiple of the vector
+// width, or that are not aligned to 16 bytes, are read one logit at a time.
+using RouteKernel = void (*)(RouteArgs);
+struct RouteShape {
+  RouteKernel kernel;
+  int lanes;
+};
+
+template <typename T, int V, int NV, int L, bool BACKWARD>
+RouteShape route_shape() {
+  if constexpr (BACKWARD) return {route_backward_kernel<T, V, NV, L>, L};
+  else return {route_forward_kernel<T, V, NV, L>, L};
 }
 
-// The zeroed part comes first: mass, number, poison.
-size_t carve_workspace(RouteArgs& a, void* workspace, size_t* zeroed) {
+template <typename T, bool BACKWARD>
+RouteShape route_pick(int experts, bool vectors) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  if (vectors) {
+    if (experts <= 16) return route_shape<T, V, 1, 16 / V, BACKWARD>();
+    if (experts <= 32) return route_shape<T, V, 8 / V, 4, BACKWARD>();
+    if (experts <= 64) return route_shape<T, V, 16 / V, 4, BACKWARD>();
+    if (experts <= 128) return route_shape<T, V, 16 / V, 8, BACKWARD>();
+    if (experts <= 256) return route_shape<T, V, 16 / V, 16, BACKWARD>();
+    if (experts <= 512) return route_shape<T, V, 16 / V, 32, BACKWARD>();
+    return route_shape<T, V, 32 / V, 32, BACKWARD>();
+  }
+  if (experts <= 16) return route_shape<T, 1, 4, 4, BACKWARD>();
+  if (experts <= 64) return route_shape<T, 1, 8, 8, BACKWARD>();
+  if (experts <= 256) return route_shape<T, 1, 16, 16, BACKWARD>();
+  if (experts <= 512) return route_shape<T, 1, 16, 32, BACKWARD>();
+  return route_shape<T, 1, 32, 32, BACKWARD>();
+}
+
+RouteShape route_pick_any(int dtype, int experts, const void* a, const void* b, bool backward) {
+  const int v = dtype == BYSJ_F32 ? 4 : 8;
+  const bool vectors = experts % v == 0 && aligned16(a) && aligned16(b);
+  if (dtype == BYSJ_F32)
+    return backward ? route_pick<float, true>(experts, vectors)
+                    : route_pick<float, false>(experts, vectors);
+  return backward ? route_pick<__nv_bfloat16, true>(experts, vectors)
+                  : route_pick<__nv_bfloat16, false>(experts, vectors);
+}
+
+// A CTA's tokens: at least 64, so that its flush into the frames' totals is
+// small beside them, and at most four CTAs for each SM.
+int route_ctas(int64_t tokens) {
+  int64_t ctas = (tokens + 63) / 64;
+  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 4;
+  if (ctas > cap) ctas = cap;
+  return ctas < 1 ? 1 : static_cast<int>(ctas);
+}
+
+// One CTA's worth of losses rides along in the forward kernel; more cells than
+// this get a kernel of their own.
+constexpr int64_t kFusedLossCells = 16384;
+
+int loss_ctas(int64_t cells) {
+  const int64_t ctas = (cells + 8 * kBlock - 1) / (8 * kBlock);
+  const int64_t cap = current_device_info().sm_count;
+  return static_cast<int>(ctas < cap ? ctas : cap);
+}
+
+// The zeroed part comes first, in whole 8-byte words.
+size_t carve_workspace(RouteArgs& a, void* workspace) {
   Carver carve(workspace);
-  a.mass = carve.take<unsigned long long>(static_cast<size_t>(a.frames) * a.experts);
-  a.number = carve.take<unsigned long long>(static_cast<size_t>(a.frames));
-  a.poison = carve.take<unsigned>(1);
-  *zeroed = carve.need;
+  const size_t cells = static_cast<size_t>(a.frames) * a.experts;
+  a.zeroed = static_cast<int64_t>(2 * cells + a.frames + 1);
+  a.mass = carve.take<unsigned long long>(static_cast<size_t>(a.zeroed));
+  a.taken = a.mass + cells;
+  a.number = a.taken + cells;
+  a.poison = reinterpret_cast<unsigned*>(a.number + a.frames);
+  a.ticket = a.poison + 1;
   a.square = carve.take<double>(static_cast<size_t>(a.ctas));
+  a.part = carve.take<double>(static_cast<size_t>(current_device_info().sm_count));
   return carve.need;
 }
 
-using RouteKernel = void (*)(RouteArgs);
-
-template <typename T, bool BACKWARD>
-RouteKernel route_pick(int experts) {
-#define BYSJ_ROUTE_CASE(NV) \
-  if (experts <= NV * kWarp) return BACKWARD ? route_backward_kernel<T, NV> : route_forward_kernel<T, NV>;
-  BYSJ_ROUTE_CASE(1)
-  BYSJ_ROUTE_CASE(2)
-  BYSJ_ROUTE_CASE(4)
-  BYSJ_ROUTE_CASE(8)
-  BYSJ_ROUTE_CASE(16)
-  BYSJ_ROUTE_CASE(32)
-#undef BYSJ_ROUTE_CASE
-  return nullptr;
+void plan_tokens(RouteArgs& a) {
+  a.ctas = route_ctas(a.tokens);
+  a.tokens_per_cta = (a.tokens + a.ctas - 1) / a.ctas;
+  a.k_magic = 65536 / a.k + 1;
 }
 
 int check_sizes(int dtype, int64_t tokens, int64_t n_experts, int64_t k, const int64_t* offsets,
@@ -334,8 +692,7 @@ size_t bysj_route_forward_workspace_size(int64_t tokens, int64_t n_experts, int6
   a.experts = static_cast<int>(n_experts);
   a.frames = frames;
   a.ctas = route_ctas(tokens);
-  size_t zeroed = 0;
-  return carve_workspace(a, nullptr, &zeroed);
+  return carve_workspace(a, nullptr);
 }
 
 int bysj_route_forward(const void* logits, int dtype, int64_t tokens, int64_t n_experts,
@@ -352,23 +709,16 @@ int bysj_route_forward(const void* logits, int dtype, int64_t tokens, int64_t n_
                       denom == nullptr)))
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "route: NULL pointer");
   RouteArgs a{};
+  a.tokens = tokens;
   a.experts = static_cast<int>(n_experts);
+  a.k = static_cast<int>(k);
   a.frames = frames;
-  a.ctas = route_ctas(tokens);
-  size_t zeroed = 0;
-  const size_t need = carve_workspace(a, workspace, &zeroed);
+  plan_tokens(a);
+  const size_t need = carve_workspace(a, workspace);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(BYSJ_ERR_WORKSPACE, "route: workspace of %zu bytes needed, %zu given", need,
                 workspace_bytes);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = cuda_check(cudaMemsetAsync(workspace, 0, zeroed, s), "route: zero workspace");
-  if (st == BYSJ_OK && frames > 0)
-    st = cuda_check(cudaMemsetAsync(counts, 0, sizeof(int64_t) * frames * n_experts, s),
-                    "route: zero counts");
-  if (st) return st;
   a.logits = logits;
-  a.tokens = tokens;
-  a.k = static_cast<int>(k);
   a.mask = mask;
   a.offsets = offsets;
   a.renormalize = renormalize;
@@ -382,12 +732,24 @@ int bysj_route_forward(const void* logits, int dtype, int64_t tokens, int64_t n_
   a.share = share;
   a.shift = 40;
   while ((tokens >> (62 - a.shift)) != 0) --a.shift;
-  const RouteKernel kernel = dtype == BYSJ_F32 ? route_pick<float, false>(a.experts)
-                                               : route_pick<__nv_bfloat16, false>(a.experts);
-  kernel<<<a.ctas, kBlock, 0, s>>>(a);
-  st = launch_check("route_forward_kernel");
+  a.column_mask = 0xffffu;
+  if (dtype == BYSJ_F32) a.column_mask = static_cast<unsigned>(next_pow2(n_experts)) - 1;
+  a.fused_losses = frames * n_experts <= kFusedLossCells;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a.ctas > 1) {
+    st = cuda_check(cudaMemsetAsync(a.mass, 0, sizeof(unsigned long long) * a.zeroed, s),
+                    "route: zero workspace");
+    if (st) return st;
+  }
+  const RouteShape shape = route_pick_any(dtype, a.experts, logits, logits, false);
+  const size_t smem = sizeof(unsigned) * (a.experts * (1 + kWarpsPerBlock) +
+                                          kWarpsPerBlock * 2 * (kWarp / shape.lanes) * a.k);
+  st = allow_dynamic_smem(reinterpret_cast<const void*>(shape.kernel), smem);
   if (st) return st;
-  route_losses_kernel<<<1, kBlock, 0, s>>>(a);
+  shape.kernel<<<a.ctas, kBlock, smem, s>>>(a);
+  st = launch_check("route_forward_kernel");
+  if (st || a.fused_losses) return st;
+  route_losses_kernel<<<loss_ctas(frames * n_experts), kBlock, 0, s>>>(a);
   return launch_check("route_losses_kernel");
 }
 
@@ -398,7 +760,7 @@ int bysj_route_backward(const void* logits, int dtype, int64_t tokens, int64_t n
                         const float* grad_balance, const float* grad_z, void* grad_logits,
                         void* stream) {
   clear_error();
-  const int st = check_sizes(dtype, tokens, n_experts, k, offsets, frames);
+  int st = check_sizes(dtype, tokens, n_experts, k, offsets, frames);
   if (st) return st;
   if (tokens == 0) return BYSJ_OK;
   if (logits == nullptr || weights == nullptr || experts == nullptr || denom == nullptr ||
@@ -421,9 +783,14 @@ int bysj_route_backward(const void* logits, int dtype, int64_t tokens, int64_t n
   a.grad_balance = grad_balance;
   a.grad_z = grad_z;
   a.grad_logits = grad_logits;
-  const RouteKernel kernel = dtype == BYSJ_F32 ? route_pick<float, true>(a.experts)
-                                               : route_pick<__nv_bfloat16, true>(a.experts);
-  kernel<<<route_ctas(tokens), kBlock, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  plan_tokens(a);
+  const RouteShape shape = route_pick_any(dtype, a.experts, logits, grad_logits, true);
+  const size_t rows = static_cast<size_t>(kWarpsPerBlock) * (kWarp / shape.lanes);
+  a.stage_bytes = (rows * a.experts * (dtype == BYSJ_F32 ? 4 : 2) + 15) / 16 * 16;
+  const size_t smem = a.stage_bytes + sizeof(float) * (a.experts + rows * a.k);
+  st = allow_dynamic_smem(reinterpret_cast<const void*>(shape.kernel), smem);
+  if (st) return st;
+  shape.kernel<<<a.ctas, kBlock, smem, static_cast<cudaStream_t>(stream)>>>(a);
   return launch_check("route_backward_kernel");
 }
 
