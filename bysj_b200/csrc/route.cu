@@ -12,12 +12,14 @@
 // A group of L lanes holds a token's row in registers (M logits a lane), so a
 // warp routes 32 / L tokens at once.  The row's order is that of unsigned keys
 // with the column in the low bits: a key is unique, ties fall to the lowest
-// column, and the next largest below `prev` is the maximum of key - prev in
-// wrapping arithmetic (the keys still to come wrap to the top), one
-// add-and-max instruction a logit and slot.  A bfloat16 logit and its column
-// fit 32 bits; a float32 key drops as many mantissa bits as the column needs,
-// and a warp in which two neighbours of the order agree in what is left, or in
-// which a NaN occurs, orders its tokens again by full value and column.
+// column.  A bfloat16 logit and its column fit 32 bits; a float32 key drops as
+// many mantissa bits as the column needs, and a warp in which two neighbours
+// of the order agree in what is left, or in which a NaN occurs, orders its
+// tokens again by full value and column.  For k = 3 .. 8 each lane sorts its
+// keys in lists of eight and keeps the upper half of bitonic merges, first of
+// its own lists, then with the other lanes of the group; for other k the next
+// largest below `prev` is the maximum of key - prev in wrapping arithmetic
+// (the keys still to come wrap to the top), one add-and-max a logit and slot.
 //
 // P and the counts are sums of integers.  A lane adds its columns' p over the
 // tokens of a piece (the part of a frame inside a CTA's range) in float32; a
@@ -58,7 +60,6 @@ struct RouteArgs {
   int ctas;
   int64_t tokens_per_cta;
   bool fused_losses;
-  unsigned column_mask;        // key bits that hold the column
   int k_magic;                 // it / k == (it k_magic) >> 16 for it < 32 k
   size_t stage_bytes;
   const float* grad_weights;
@@ -99,6 +100,21 @@ __device__ __forceinline__ void copy_vec(T* to, const T* from) {
   else *to = *from;
 }
 
+// V cotangents from column c on (0 beyond the row's end).
+template <int V>
+__device__ __forceinline__ void load_cot(const float* s, int c, int experts, float (&v)[V]) {
+  if constexpr (V >= 4) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const float4 q = c < experts ? *reinterpret_cast<const float4*>(s + c + i)
+                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
+    }
+  } else {
+    v[0] = c < experts ? s[c] : 0.0f;
+  }
+}
+
 // Frame of token t: the last whose offset is <= t.
 __device__ __forceinline__ int64_t frame_of(const RouteArgs& a, int64_t t) {
   if (a.offsets == nullptr) return 0;
@@ -130,6 +146,26 @@ struct Row {
     }
   }
   __device__ __forceinline__ float get(int i) const { return v[i / V].get(i % V); }
+  // Largest of the lane's logits (a NaN yields to a number).
+  __device__ __forceinline__ float top() const {
+    if constexpr (sizeof(T) == 2 && V == 8) {  // two at a time
+      __nv_bfloat162 m = pair(0);
+#pragma unroll
+      for (int w = 1; w < 4 * NV; ++w) m = __hmax2(m, pair(w));
+      return fmaxf(__low2float(m), __high2float(m));
+    } else {
+      float m = get(0);
+#pragma unroll
+      for (int i = 1; i < V * NV; ++i) m = fmaxf(m, get(i));
+      return m;
+    }
+  }
+  // Logits 2 w and 2 w + 1 of a bfloat16 row.
+  __device__ __forceinline__ __nv_bfloat162 pair(int w) const {
+    const uint4& r = v[w / 4].r;
+    const uint32_t u = w % 4 == 0 ? r.x : w % 4 == 1 ? r.y : w % 4 == 2 ? r.z : r.w;
+    return *reinterpret_cast<const __nv_bfloat162*>(&u);
+  }
   __device__ static constexpr int column(int i, int l) { return ((i / V) * L + l) * V + i % V; }
   // -inf: what lies beyond the row's end, or belongs to a token left out
   __device__ static __forceinline__ void fill(RowVec<float, 4>& r) {
@@ -161,18 +197,94 @@ __device__ __forceinline__ unsigned row_max(unsigned v) {
   return v;
 }
 
-// Bits of a float in the order of the values; + 0.0f makes the two zeros equal.
-__device__ __forceinline__ unsigned order_bits(float v) {
-  const unsigned b = __float_as_uint(v + 0.0f);
-  return b ^ (static_cast<unsigned>(static_cast<int>(b) >> 31) | 0x80000000u);
-}
+// Keys.  order_bits: the bits of a float in the order of the values (+ 0.0f
+// makes the two zeros equal).  A key replaces the bits under `mask` by
+// mask - column; column (n L + l) V + i has the lane l in bits of its own, so
+// a lane orders its own keys without them and adds them before it meets others.
 constexpr unsigned kBarred = 0x007fffffu;  // order_bits(-inf)
+
+template <typename T, int V, int NV, int L>
+struct Keys {
+  static constexpr int M = V * NV;
+  static constexpr unsigned kMask = sizeof(T) == 2 ? 0xffffu : M * L - 1;
+  static constexpr unsigned kLane = (L - 1) * V;  // the lane's bits of a column
+  static constexpr unsigned kBar = kBarred | kMask;
+  __device__ static __forceinline__ unsigned order_bits(float v) {
+    const unsigned b = __float_as_uint(v + 0.0f);
+    return b ^ (static_cast<unsigned>(static_cast<int>(b) >> 31) | 0x80000000u);
+  }
+  // Keys of a lane's row, without the lane's own bits.
+  __device__ static __forceinline__ void make(const Row<T, V, NV, L>& row, unsigned (&key)[M]) {
+    if constexpr (sizeof(T) == 2 && V == 8) {  // two at a time, off the integer pipe where it goes
+#pragma unroll
+      for (int w = 0; w < M / 2; ++w) {
+        const __nv_bfloat162 z = __hadd2(row.pair(w), __float2bfloat162_rn(0.0f));
+        const unsigned b = *reinterpret_cast<const unsigned*>(&z);
+        const unsigned o = b ^ (((b >> 15) & 0x00010001u) * 0x7fffu | 0x80008000u);
+        key[2 * w] = o * 65536u + rest(2 * w);
+        key[2 * w + 1] = (o & 0xffff0000u) | rest(2 * w + 1);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < M; ++i) key[i] = (order_bits(row.get(i)) & ~kMask) | rest(i);
+    }
+  }
+  __device__ static constexpr unsigned rest(int i) {
+    return (kMask - (i / V) * L * V - i % V) & ~kLane;
+  }
+  __device__ static __forceinline__ unsigned lane_part(int l) {
+    return kLane - static_cast<unsigned>(l * V);
+  }
+  __device__ static __forceinline__ bool barred(unsigned key) { return (key | kMask) <= kBar; }
+  __device__ static __forceinline__ int column(unsigned key) {
+    return static_cast<int>(kMask - (key & kMask));
+  }
+  // The logit of a key: in the key itself for bfloat16, else read again.
+  __device__ static __forceinline__ float logit(unsigned key, const T* row) {
+    if constexpr (sizeof(T) == 2) {
+      const unsigned b = key & 0xffff0000u;
+      return __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : b ^ 0xffff0000u);
+    } else {
+      return load_f32(row + column(key));
+    }
+  }
+};
+
+// Comparators of sorting networks, larger first.
+__device__ __forceinline__ void order2(unsigned& a, unsigned& b) {
+  const unsigned hi = max(a, b);
+  b = min(a, b);
+  a = hi;
+}
+__device__ __forceinline__ void sort8(unsigned (&v)[8]) {  // odd-even merge sort
+  order2(v[0], v[1]); order2(v[2], v[3]); order2(v[4], v[5]); order2(v[6], v[7]);
+  order2(v[0], v[2]); order2(v[1], v[3]); order2(v[4], v[6]); order2(v[5], v[7]);
+  order2(v[1], v[2]); order2(v[5], v[6]);
+  order2(v[0], v[4]); order2(v[1], v[5]); order2(v[2], v[6]); order2(v[3], v[7]);
+  order2(v[2], v[4]); order2(v[3], v[5]);
+  order2(v[1], v[2]); order2(v[3], v[4]); order2(v[5], v[6]);
+}
+__device__ __forceinline__ void merge8(unsigned (&v)[8]) {  // a bitonic list in order
+#pragma unroll
+  for (int s = 4; s > 0; s >>= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((i & s) == 0) order2(v[i], v[i + s]);
+}
+
+// exp(x - ref) on the transcendental pipe: the rounding of the product adds
+// |x - ref| 2^-24 relative to the 2 units of ex2.  The difference comes first,
+// so rows of any magnitude (all at the type's lowest value, say) are safe.
+__device__ __forceinline__ float exp_from(float x, float ref) {
+  return ex2_ftz((x - ref) * 1.4426950408889634f);
+}
 
 // Exact order for a warp's rows: the next in (value, then column) after
 // (prev, at); NaN is largest.  Slow: two reductions a slot.
 template <typename T, int V, int NV, int L>
 __device__ __noinline__ void pick_exact(const Row<T, V, NV, L>& row, int l, int experts, int k,
                                         unsigned* picks) {
+  using Key = Keys<T, V, NV, L>;
   constexpr int M = V * NV;
   unsigned prev = 0;
   int at = -1;
@@ -183,7 +295,7 @@ __device__ __noinline__ void pick_exact(const Row<T, V, NV, L>& row, int l, int 
     for (int i = 0; i < M; ++i) {
       const int c = row.column(i, l);
       const float x = row.get(i);
-      const unsigned key = c >= experts ? 0u : isnan(x) ? 0xffffffffu : order_bits(x);
+      const unsigned key = c >= experts ? 0u : isnan(x) ? 0xffffffffu : Key::order_bits(x);
       const bool left = slot == 0 || key < prev || (key == prev && c > at);
       if (left && (key > best || (key == best && c < where))) {
         best = key;
@@ -199,7 +311,8 @@ __device__ __noinline__ void pick_exact(const Row<T, V, NV, L>& row, int l, int 
         where = there;
       }
     }
-    if (l == 0) picks[slot] = best <= kBarred ? 0xffffffffu : static_cast<unsigned>(where);
+    if (l == 0)
+      picks[slot] = best <= kBarred ? 0u : (best & ~Key::kMask) | (Key::kMask - where);
     prev = best;
     at = where;
   }
@@ -266,10 +379,12 @@ __device__ void route_losses(const RouteArgs& a, int cta, int ctas) {
 
 // Shared memory of the forward kernel, per CTA: counts [E], one row of mass a
 // warp [warps][E], and per warp the picks and their values [32 / L][k].
-template <typename T, int V, int NV, int L>
-__global__ void __launch_bounds__(kBlock) route_forward_kernel(RouteArgs a) {
+// TOP 8: networks, k <= 8; TOP 0: a pass a slot.
+template <typename T, int V, int NV, int L, int TOP>
+__global__ void __launch_bounds__(kBlock, 2) route_forward_kernel(RouteArgs a) {
   constexpr int M = V * NV, R = kWarp / L;
   using RowT = Row<T, V, NV, L>;
+  using Key = Keys<T, V, NV, L>;
   extern __shared__ __align__(16) unsigned char smem[];
   const int E = a.experts, k = a.k, items = R * k;
   unsigned* s_count = reinterpret_cast<unsigned*>(smem);
@@ -283,6 +398,7 @@ __global__ void __launch_bounds__(kBlock) route_forward_kernel(RouteArgs a) {
   __shared__ bool s_last;
   const T* logits = static_cast<const T*>(a.logits);
   const float unit = static_cast<float>(int64_t{1} << a.shift);
+  const unsigned lane_part = Key::lane_part(l);
   const int64_t t0 = a.tokens_per_cta * blockIdx.x;
   const int64_t t1 = min(t0 + a.tokens_per_cta, a.tokens);
 
@@ -314,94 +430,173 @@ __global__ void __launch_bounds__(kBlock) route_forward_kernel(RouteArgs a) {
     for (int64_t base = lo + warp * R; base < hi; base += kWarpsPerBlock * R) {
       const RowT row = next;
       if (base + kWarpsPerBlock * R < hi) fetch(base + kWarpsPerBlock * R, next);
-      float top = row.get(0);
-#pragma unroll
-      for (int i = 1; i < M; ++i) top = fmaxf(top, row.get(i));
-      top = row_max<L>(top);
+      const int64_t t = base + g;
+      const float top = row_max<L>(row.top());
       const float ref = top > -INFINITY ? top : 0.0f;
-      float e[M], total = 0.0f;
+      float total = 0.0f, inv;
+      {
+        float e[M];
 #pragma unroll
-      for (int i = 0; i < M; ++i) {
-        e[i] = __expf(row.get(i) - ref);
-        total += e[i];
+        for (int i = 0; i < M; ++i) {
+          e[i] = exp_from(row.get(i), ref);
+          total += e[i];
+        }
+        total = row_sum<L>(total);
+        inv = total != 0.0f ? 1.0f / total : 0.0f;  // 0: every logit is -inf
+#pragma unroll
+        for (int i = 0; i < M; ++i) mass[i] = fmaf(e[i], inv, mass[i]);
       }
-      total = row_sum<L>(total);
-      const bool valid = total != 0.0f;  // NaN counts; 0: every logit is -inf
-      const float inv = valid ? 1.0f / total : 0.0f;
-#pragma unroll
-      for (int i = 0; i < M; ++i) mass[i] = fmaf(e[i], inv, mass[i]);
-
-      // the order: V columns of a vector lie side by side, so one subtraction
-      // gives the column part of each key
-      unsigned key[M];
-#pragma unroll
-      for (int i = 0; i < M; ++i) {
-        const int c = RowT::column(i, l);
-        const unsigned bits = order_bits(row.get(i));
-        key[i] = c < E ? (bits & ~a.column_mask) | (a.column_mask - c) : 0u;
-      }
-      unsigned prev = 0;
       bool unclear = isnan(total);
       constexpr bool kExact = sizeof(T) == 2;
-      const int rounds = kExact ? k : k + 1;  // one more: is the last one clear?
-      for (int slot = 0; slot < rounds; ++slot) {
-        unsigned m = 0;
+      if constexpr (TOP == 8) {
+        unsigned list[8];
+        int above = 0;  // keys that reach the last pick's kept bits
+        {
+          unsigned key[M];
+          Key::make(row, key);
 #pragma unroll
-        for (int i = 0; i < M; ++i) m = __viaddmax_u32(key[i], 0u - prev, m);
-        const unsigned best = row_max<L>(m) + prev;
-        if constexpr (!kExact)
-          unclear |= slot > 0 && best < prev && (best | a.column_mask) == (prev | a.column_mask) &&
-                     (best | a.column_mask) > (kBarred | a.column_mask);
-        if (l == 0 && slot < k)
-          picks[g * k + slot] = (best | a.column_mask) <= (kBarred | a.column_mask)
-                                    ? 0xffffffffu
-                                    : a.column_mask - (best & a.column_mask);
-        prev = best;
-      }
-      if (__any_sync(kFull, unclear)) pick_exact<T, V, NV, L>(row, l, E, k, picks + g * k);
-      __syncwarp();
-
-      // weights and indices, the warp's R k slots side by side
-      for (int it0 = 0; it0 < items; it0 += kWarp) {
-        const int it = it0 + lane;
-        const int r = min((it * a.k_magic) >> 16, R - 1);
-        const float ref_r = __shfl_sync(kFull, ref, r * L), inv_r = __shfl_sync(kFull, inv, r * L);
-        const int64_t t = base + r;
-        if (it < items) {
-          const unsigned c = picks[it];
-          float p = 0.0f;
-          if (t < hi && c != 0xffffffffu) {
-            p = __expf(load_f32(logits + t * E + c) - ref_r) * inv_r;
-            atomicAdd(s_count + c, 1u);
+          for (int i = 0; i < 8; ++i) list[i] = i < M ? key[i < M ? i : 0] : 0u;
+          sort8(list);
+#pragma unroll
+          for (int n = 8; n < M; n += 8) {
+            unsigned other[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) other[i] = key[n + i];
+            sort8(other);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) list[i] = max(list[i], other[7 - i]);
+            merge8(list);
           }
-          values[it] = p;
-        }
-      }
-      __syncwarp();
-      for (int it = lane; it < items; it += kWarp) {
-        const int r = (it * a.k_magic) >> 16;
-        const int64_t t = base + r;
-        if (t < hi) {
-          float w = values[it];
-          const unsigned c = picks[it];
-          if (a.renormalize && c != 0xffffffffu) {
-            float sum = 0.0f;
-            for (int j = 0; j < k; ++j) sum += values[r * k + j];
-            w /= sum;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) list[i] |= lane_part;
+#pragma unroll
+          for (int d = 1; d < L; d <<= 1) {
+            unsigned other[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) other[i] = __shfl_xor_sync(kFull, list[7 - i], d);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) list[i] = max(list[i], other[i]);
+            merge8(list);
           }
-          a.weights[base * k + it] = w;
-          a.chosen[base * k + it] = c == 0xffffffffu ? int64_t{-1} : static_cast<int64_t>(c);
+          if constexpr (!kExact) {
+            unsigned last = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i == k - 1) last = list[i] & ~Key::kMask;
+#pragma unroll
+            for (int i = 0; i < M; ++i) above += key[i] >= last;
+            if (last <= kBarred) above = 0;  // barred either way
+          }
         }
+        if constexpr (!kExact) {
+#pragma unroll
+          for (int d = 1; d < L; d <<= 1) above += __shfl_xor_sync(kFull, above, d);
+          unclear |= above > k;
+#pragma unroll
+          for (int i = 1; i < 8; ++i)
+            unclear |= i < k && !Key::barred(list[i]) &&
+                       (list[i] | Key::kMask) == (list[i - 1] | Key::kMask);
+        }
+        if (__any_sync(kFull, unclear)) {
+          pick_exact<T, V, NV, L>(row, l, E, k, picks + g * k);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) list[i] = i < k ? picks[g * k + i] : 0u;
+          __syncwarp();
+        }
+        // slots l, l + L, ... of the row are this lane's to finish
+        constexpr int kMine = L >= 8 ? 1 : 8 / L;
+        unsigned mine[kMine];
+        float w[kMine], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          mine[i] = 0u;
+#pragma unroll
+          for (int q = 0; q < (L < 8 ? L : 8); ++q)
+            if (l == q) mine[i] = list[i * L + q];
+          const bool on = l + i * L < k && t < hi && !Key::barred(mine[i]);
+          if (!on) mine[i] = 0u;
+          w[i] = on ? exp_from(Key::logit(mine[i], logits + t * E), ref) * inv : 0.0f;
+          sum += w[i];
+          if (on) atomicAdd(s_count + Key::column(mine[i]), 1u);
+        }
+        if (a.renormalize) {
+          sum = row_sum<L>(sum);
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+            if (mine[i] != 0u) w[i] /= sum;
+        }
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          if (l + i * L < k && t < hi) {
+            const int64_t at = t * k + l + i * L;
+            a.weights[at] = w[i];
+            a.chosen[at] = mine[i] == 0u ? int64_t{-1} : Key::column(mine[i]);
+          }
+        }
+      } else {
+        unsigned key[M];
+        Key::make(row, key);
+#pragma unroll
+        for (int i = 0; i < M; ++i) key[i] |= lane_part;
+        unsigned prev = 0;
+        const int rounds = kExact ? k : k + 1;  // one more: is the last one clear?
+        for (int slot = 0; slot < rounds; ++slot) {
+          unsigned m = 0;
+#pragma unroll
+          for (int i = 0; i < M; ++i) m = __viaddmax_u32(key[i], 0u - prev, m);
+          const unsigned best = row_max<L>(m) + prev;
+          if constexpr (!kExact)
+            unclear |= slot > 0 && best < prev && !Key::barred(best) &&
+                       (best | Key::kMask) == (prev | Key::kMask);
+          if (l == 0 && slot < k) picks[g * k + slot] = best;
+          prev = best;
+        }
+        if (__any_sync(kFull, unclear)) pick_exact<T, V, NV, L>(row, l, E, k, picks + g * k);
+        __syncwarp();
+        // weights and indices, the warp's R k slots side by side
+        for (int it0 = 0; it0 < items; it0 += kWarp) {
+          const int it = it0 + lane;
+          const int r = min((it * a.k_magic) >> 16, R - 1);
+          const float ref_r = __shfl_sync(kFull, ref, r * L);
+          const float inv_r = __shfl_sync(kFull, inv, r * L);
+          if (it < items) {
+            unsigned pick = picks[it];
+            float p = 0.0f;
+            if (base + r >= hi || Key::barred(pick)) pick = 0u;
+            if (pick != 0u) {
+              p = exp_from(Key::logit(pick, logits + (base + r) * E), ref_r) * inv_r;
+              atomicAdd(s_count + Key::column(pick), 1u);
+            }
+            picks[it] = pick;
+            values[it] = p;
+          }
+        }
+        __syncwarp();
+        for (int it = lane; it < items; it += kWarp) {
+          const int r = (it * a.k_magic) >> 16;
+          if (base + r < hi) {
+            float w = values[it];
+            const unsigned pick = picks[it];
+            if (a.renormalize && pick != 0u) {
+              float sum = 0.0f;
+              for (int j = 0; j < k; ++j) sum += values[r * k + j];
+              w /= sum;
+            }
+            a.weights[base * k + it] = w;
+            a.chosen[base * k + it] = pick == 0u ? int64_t{-1} : Key::column(pick);
+          }
+        }
+        __syncwarp();
       }
-      if (l == 0 && base + g < hi) {
-        a.denom[base + g] = total;
-        if (valid) {
+      if (l == 0 && t < hi) {
+        a.denom[t] = total;
+        if (total != 0.0f) {  // a NaN counts
           const float lse = ref + logf(total);
           square += static_cast<double>(lse) * lse;
           ++valid_rows;
         }
       }
-      __syncwarp();
     }
 
     // flush the piece into its frame's totals
@@ -458,24 +653,46 @@ __global__ void __launch_bounds__(kBlock) route_losses_kernel(RouteArgs a) {
   route_losses(a, blockIdx.x, gridDim.x);
 }
 
-// Shared memory, per CTA: the cotangents share[s, e] grad_balance [E]; per warp
-// the slots' products [32 / L][k] and the rows on their way out [32 / L][E].
+// Shared memory, per CTA: the rows on their way out [warps][32 / L][E] and the
+// cotangents share[s, e] grad_balance [E].
 template <typename T, int V, int NV, int L>
-__global__ void __launch_bounds__(kBlock) route_backward_kernel(RouteArgs a) {
+__global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
+    route_backward_kernel(RouteArgs a) {
   constexpr int M = V * NV, R = kWarp / L;
   using RowT = Row<T, V, NV, L>;
   extern __shared__ __align__(16) unsigned char smem[];
-  const int E = a.experts, k = a.k, items = R * k;
+  const int E = a.experts, k = a.k;
   const int lane = lane_id(), warp = threadIdx.x / kWarp, l = lane % L, g = lane / L;
-  T* stage = reinterpret_cast<T*>(smem) + warp * R * E;
-  float* s_cot = reinterpret_cast<float*>(smem + a.stage_bytes);
-  float* values = s_cot + E + warp * items;
+  float* s_cot = reinterpret_cast<float*>(smem + a.stage_bytes);  // 16-byte aligned
+  T* stage = reinterpret_cast<T*>(smem) + (warp * R + g) * E;
   const T* logits = static_cast<const T*>(a.logits);
   T* out = static_cast<T*>(a.grad_logits);
+  const bool gated = a.grad_weights != nullptr;
   const float gb = a.grad_balance ? __ldg(a.grad_balance) : 0.0f;
   const float gz = a.grad_z ? __ldg(a.grad_z) * __ldg(a.z_scale) : 0.0f;
   const int64_t t0 = a.tokens_per_cta * blockIdx.x;
   const int64_t t1 = min(t0 + a.tokens_per_cta, a.tokens);
+
+  // What a token needs, requested one step ahead; slots l, l + L, ... of its k
+  // belong to lane l, the first of them here.
+  struct Fetch {
+    RowT row;
+    float total, w, gw;
+    int slot, first;  // expert of slot l; of slot 0
+  };
+  auto fetch = [&](int64_t t, int64_t hi) {
+    Fetch f;
+    const bool in = t < hi;
+    f.row.load(logits + t * E, l, E, in);
+    f.total = in ? __ldg(a.denom + t) : 1.0f;
+    f.first = in ? static_cast<int>(__ldg(a.chosen + t * k)) : -1;
+    const bool mine = gated && in && l < k;
+    f.slot = mine ? static_cast<int>(__ldg(a.chosen + t * k + l)) : -1;
+    f.w = mine ? __ldg(a.weights + t * k + l) : 0.0f;
+    f.gw = mine ? __ldg(a.grad_weights + t * k + l) : 0.0f;
+    return f;
+  };
+
   int64_t s = t0 < t1 ? frame_of(a, t0) : 0;
   for (int64_t lo = t0; lo < t1; ++s) {
     const int64_t hi = min(frame_end(a, s), t1);
@@ -486,90 +703,65 @@ __global__ void __launch_bounds__(kBlock) route_backward_kernel(RouteArgs a) {
     __syncthreads();
     for (int c = threadIdx.x; c < E; c += kBlock) s_cot[c] = gb * __ldg(a.share + s * E + c);
     __syncthreads();
-    float cot[M];
-#pragma unroll
-    for (int i = 0; i < M; ++i) {
-      const int c = RowT::column(i, l);
-      cot[i] = c < E ? s_cot[c] : 0.0f;
-    }
+    Fetch next = fetch(lo + warp * R + g, hi);
     for (int64_t base = lo + warp * R; base < hi; base += kWarpsPerBlock * R) {
       const int64_t t = base + g;
-      const bool in = t < hi;
-      RowT row;
-      row.load(logits + t * E, l, E, in);
-      const bool valid = in && __ldg(a.chosen + t * k) >= 0;
-      const float total = in ? __ldg(a.denom + t) : 1.0f;
-      const float inv = 1.0f / total;
-      float top = row.get(0);
-#pragma unroll
-      for (int i = 1; i < M; ++i) top = fmaxf(top, row.get(i));
-      top = row_max<L>(top);
+      const Fetch f = next;
+      if (base + kWarpsPerBlock * R < hi) next = fetch(t + kWarpsPerBlock * R, hi);
+      const bool valid = f.first >= 0;
+      const float inv = 1.0f / f.total;
+      const float top = row_max<L>(f.row.top());
       const float ref = top > -INFINITY ? top : 0.0f;
-      float along_w = 0.0f;
-      if (a.grad_weights != nullptr) {
-        for (int it0 = 0; it0 < items; it0 += kWarp) {
-          const int it = it0 + lane;
-          if (it < items && base + ((it * a.k_magic) >> 16) < hi)
-            values[it] = __ldg(a.weights + base * k + it) * __ldg(a.grad_weights + base * k + it);
-          else if (it < items)
-            values[it] = 0.0f;
-        }
-        __syncwarp();
-        for (int j = 0; j < k; ++j) along_w += values[g * k + j];
-      }
-      // p_e a_e and its sum; a weight that is p itself adds gw p at its expert
-      float p[M], pc[M], along = 0.0f;
+      float along_w = f.w * f.gw;
+      if (gated && k > L && t < hi)
+        for (int j = l + L; j < k; j += L)
+          along_w += __ldg(a.weights + t * k + j) * __ldg(a.grad_weights + t * k + j);
+      along_w = row_sum<L>(along_w);
+      // p_e and the sum of p_e a_e; a weight that is p itself adds gw p at its expert
+      float p[M], along = 0.0f;
 #pragma unroll
-      for (int i = 0; i < M; ++i) {
-        p[i] = __expf(row.get(i) - ref) * inv;
-        pc[i] = p[i] * cot[i];
-        along += pc[i];
+      for (int n = 0; n < NV; ++n) {
+        float cot[V];
+        load_cot<V>(s_cot, (n * L + l) * V, E, cot);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          p[n * V + i] = exp_from(f.row.get(n * V + i), ref) * inv;
+          along = fmaf(p[n * V + i], cot[i], along);
+        }
       }
       along = row_sum<L>(along);
       if (!a.renormalize) along += along_w;
-      const float pull = gz * (ref + logf(total)) - along;
+      const float pull = gz * (ref + logf(f.total)) - along;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         const int c = (n * L + l) * V;
         float v[V];
+        load_cot<V>(s_cot, c, E, v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          v[i] = fmaf(p[n * V + i], pull, pc[n * V + i]);
-          if (!valid) v[i] = 0.0f;
-        }
-        if (c < E) store_vec<V>(stage + g * E + c, v);
+        for (int i = 0; i < V; ++i) v[i] = valid ? p[n * V + i] * (v[i] + pull) : 0.0f;
+        if (c < E) store_vec<V>(stage + c, v);
       }
-      if (a.grad_weights != nullptr) {
+      if (gated) {  // the chosen experts once more, with the weights' part
         __syncwarp();
-        // the chosen experts once more, with the weights' part
-        for (int it0 = 0; it0 < items; it0 += kWarp) {
-          const int it = it0 + lane;
-          const int r = min((it * a.k_magic) >> 16, R - 1);
-          const float ref_r = __shfl_sync(kFull, ref, r * L);
-          const float inv_r = __shfl_sync(kFull, inv, r * L);
-          const float pull_r = __shfl_sync(kFull, pull, r * L);
-          const float along_r = __shfl_sync(kFull, along_w, r * L);
-          if (it < items && base + r < hi) {
-            const int64_t c = __ldg(a.chosen + base * k + it);
-            if (c >= 0) {
-              const float gw = __ldg(a.grad_weights + base * k + it);
-              const float pe = __expf(load_f32(logits + (base + r) * E + c) - ref_r) * inv_r;
-              const float value =
-                  a.renormalize
-                      ? fmaf(pe, s_cot[c] + pull_r,
-                             __ldg(a.weights + base * k + it) * (gw - along_r))
-                      : pe * (s_cot[c] + gw + pull_r);
-              store_value(stage + r * E + c, value);
-            }
+        for (int j = l; j < k; j += L) {
+          const bool head = j < L;
+          const int c = head ? f.slot : t < hi ? static_cast<int>(__ldg(a.chosen + t * k + j)) : -1;
+          if (c >= 0) {
+            const float gw = head ? f.gw : __ldg(a.grad_weights + t * k + j);
+            const float w = head ? f.w : __ldg(a.weights + t * k + j);
+            const float pe =
+                a.renormalize ? exp_from(load_f32(logits + t * E + c), ref) * inv : w;
+            store_value(stage + c, a.renormalize ? fmaf(pe, s_cot[c] + pull, w * (gw - along_w))
+                                                 : pe * (s_cot[c] + gw + pull));
           }
         }
       }
       __syncwarp();
-      if (in) {
+      if (t < hi) {
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
           const int c = (n * L + l) * V;
-          if (c < E) copy_vec<V>(out + t * E + c, stage + g * E + c);
+          if (c < E) copy_vec<V>(out + t * E + c, stage + c);
         }
       }
       __syncwarp();
@@ -579,55 +771,68 @@ __global__ void __launch_bounds__(kBlock) route_backward_kernel(RouteArgs a) {
 }
 
 // Launch shapes by the number of experts: L lanes a token and M logits a lane.
-// Few lanes a token mean few shuffles a slot; M = 16 keeps keys, exponentials
-// and masses in registers.  Rows whose length is not a multiple of the vector
-// width, or that are not aligned to 16 bytes, are read one logit at a time.
+// Few lanes a token mean few shuffles; the forward networks take M = 32 (128
+// experts and k = 8, bfloat16: see the figures at the kernel), the other
+// kernels M = 16, which leaves registers for more warps.  Rows whose length is
+// not a multiple of the vector width, or that are not aligned to 16 bytes, are
+// read one logit at a time.
 using RouteKernel = void (*)(RouteArgs);
 struct RouteShape {
   RouteKernel kernel;
   int lanes;
 };
 
-template <typename T, int V, int NV, int L, bool BACKWARD>
+enum RoutePass { kForwardSlots, kForwardNetwork, kBackward };
+
+template <typename T, int V, int NV, int L, RoutePass P>
 RouteShape route_shape() {
-  if constexpr (BACKWARD) return {route_backward_kernel<T, V, NV, L>, L};
-  else return {route_forward_kernel<T, V, NV, L>, L};
+  if constexpr (P == kBackward) return {route_backward_kernel<T, V, NV, L>, L};
+  else return {route_forward_kernel<T, V, NV, L, P == kForwardNetwork ? 8 : 0>, L};
 }
 
-template <typename T, bool BACKWARD>
+template <typename T, RoutePass P>
 RouteShape route_pick(int experts, bool vectors) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
+  constexpr int W = P == kForwardNetwork ? 2 : 1;  // 16 W logits a lane
   if (vectors) {
-    if (experts <= 16) return route_shape<T, V, 1, 16 / V, BACKWARD>();
-    if (experts <= 32) return route_shape<T, V, 8 / V, 4, BACKWARD>();
-    if (experts <= 64) return route_shape<T, V, 16 / V, 4, BACKWARD>();
-    if (experts <= 128) return route_shape<T, V, 16 / V, 8, BACKWARD>();
-    if (experts <= 256) return route_shape<T, V, 16 / V, 16, BACKWARD>();
-    if (experts <= 512) return route_shape<T, V, 16 / V, 32, BACKWARD>();
-    return route_shape<T, V, 32 / V, 32, BACKWARD>();
+    if (experts <= 16) return route_shape<T, V, 1, 16 / V, P>();
+    if (experts <= 32) return route_shape<T, V, 8 / V, 4, P>();
+    if (experts <= 64) return route_shape<T, V, 16 / V, 4, P>();
+    if (experts <= 128) return route_shape<T, V, 16 * W / V, 8 / W, P>();
+    if (experts <= 256) return route_shape<T, V, 16 * W / V, 16 / W, P>();
+    if (experts <= 512) return route_shape<T, V, 16 * W / V, 32 / W, P>();
+    return route_shape<T, V, 32 / V, 32, P>();
   }
-  if (experts <= 16) return route_shape<T, 1, 4, 4, BACKWARD>();
-  if (experts <= 64) return route_shape<T, 1, 8, 8, BACKWARD>();
-  if (experts <= 256) return route_shape<T, 1, 16, 16, BACKWARD>();
-  if (experts <= 512) return route_shape<T, 1, 16, 32, BACKWARD>();
-  return route_shape<T, 1, 32, 32, BACKWARD>();
+  if constexpr (P == kForwardNetwork) {
+    return route_pick<T, kForwardSlots>(experts, false);
+  } else {
+    if (experts <= 16) return route_shape<T, 1, 4, 4, P>();
+    if (experts <= 64) return route_shape<T, 1, 8, 8, P>();
+    if (experts <= 256) return route_shape<T, 1, 16, 16, P>();
+    if (experts <= 512) return route_shape<T, 1, 16, 32, P>();
+    return route_shape<T, 1, 32, 32, P>();
+  }
 }
 
-RouteShape route_pick_any(int dtype, int experts, const void* a, const void* b, bool backward) {
+template <typename T>
+RouteShape route_pick_pass(int experts, bool vectors, RoutePass pass) {
+  if (pass == kBackward) return route_pick<T, kBackward>(experts, vectors);
+  return pass == kForwardNetwork ? route_pick<T, kForwardNetwork>(experts, vectors)
+                                 : route_pick<T, kForwardSlots>(experts, vectors);
+}
+
+RouteShape route_pick_any(int dtype, int experts, const void* a, const void* b, RoutePass pass) {
   const int v = dtype == BYSJ_F32 ? 4 : 8;
   const bool vectors = experts % v == 0 && aligned16(a) && aligned16(b);
-  if (dtype == BYSJ_F32)
-    return backward ? route_pick<float, true>(experts, vectors)
-                    : route_pick<float, false>(experts, vectors);
-  return backward ? route_pick<__nv_bfloat16, true>(experts, vectors)
-                  : route_pick<__nv_bfloat16, false>(experts, vectors);
+  return dtype == BYSJ_F32 ? route_pick_pass<float>(experts, vectors, pass)
+                           : route_pick_pass<__nv_bfloat16>(experts, vectors, pass);
 }
 
 // A CTA's tokens: at least 64, so that its flush into the frames' totals is
-// small beside them, and at most four CTAs for each SM.
+// small beside them; one wave of the forward's two CTAs for each SM.
 int route_ctas(int64_t tokens) {
   int64_t ctas = (tokens + 63) / 64;
-  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 4;
+  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 2;
   if (ctas > cap) ctas = cap;
   return ctas < 1 ? 1 : static_cast<int>(ctas);
 }
@@ -659,7 +864,7 @@ size_t carve_workspace(RouteArgs& a, void* workspace) {
 
 void plan_tokens(RouteArgs& a) {
   a.ctas = route_ctas(a.tokens);
-  a.tokens_per_cta = (a.tokens + a.ctas - 1) / a.ctas;
+  a.tokens_per_cta = ((a.tokens + a.ctas - 1) / a.ctas + 63) / 64 * 64;
   a.k_magic = 65536 / a.k + 1;
 }
 
@@ -732,8 +937,6 @@ int bysj_route_forward(const void* logits, int dtype, int64_t tokens, int64_t n_
   a.share = share;
   a.shift = 40;
   while ((tokens >> (62 - a.shift)) != 0) --a.shift;
-  a.column_mask = 0xffffu;
-  if (dtype == BYSJ_F32) a.column_mask = static_cast<unsigned>(next_pow2(n_experts)) - 1;
   a.fused_losses = frames * n_experts <= kFusedLossCells;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.ctas > 1) {
@@ -741,7 +944,8 @@ int bysj_route_forward(const void* logits, int dtype, int64_t tokens, int64_t n_
                     "route: zero workspace");
     if (st) return st;
   }
-  const RouteShape shape = route_pick_any(dtype, a.experts, logits, logits, false);
+  const RouteShape shape = route_pick_any(dtype, a.experts, logits, logits,
+                                          k >= 3 && k <= 8 ? kForwardNetwork : kForwardSlots);
   const size_t smem = sizeof(unsigned) * (a.experts * (1 + kWarpsPerBlock) +
                                           kWarpsPerBlock * 2 * (kWarp / shape.lanes) * a.k);
   st = allow_dynamic_smem(reinterpret_cast<const void*>(shape.kernel), smem);
@@ -784,10 +988,15 @@ int bysj_route_backward(const void* logits, int dtype, int64_t tokens, int64_t n
   a.grad_z = grad_z;
   a.grad_logits = grad_logits;
   plan_tokens(a);
-  const RouteShape shape = route_pick_any(dtype, a.experts, logits, grad_logits, true);
+  // no flush here: smaller ranges, three CTAs for each SM and four waves
+  const int64_t per = (tokens + current_device_info().sm_count * 12 - 1) /
+                      (current_device_info().sm_count * 12);
+  a.tokens_per_cta = (per + 63) / 64 * 64;
+  a.ctas = static_cast<int>((tokens + a.tokens_per_cta - 1) / a.tokens_per_cta);
+  const RouteShape shape = route_pick_any(dtype, a.experts, logits, grad_logits, kBackward);
   const size_t rows = static_cast<size_t>(kWarpsPerBlock) * (kWarp / shape.lanes);
   a.stage_bytes = (rows * a.experts * (dtype == BYSJ_F32 ? 4 : 2) + 15) / 16 * 16;
-  const size_t smem = a.stage_bytes + sizeof(float) * (a.experts + rows * a.k);
+  const size_t smem = a.stage_bytes + sizeof(float) * a.experts;
   st = allow_dynamic_smem(reinterpret_cast<const void*>(shape.kernel), smem);
   if (st) return st;
   shape.kernel<<<a.ctas, kBlock, smem, static_cast<cudaStream_t>(stream)>>>(a);
