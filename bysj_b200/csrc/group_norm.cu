@@ -4,15 +4,31 @@
 //   dz = dy act'(z), d = dz w
 //   dx = rstd (d - mean(d) - xhat mean(d xhat)),  dw = sum dz xhat,  db = sum dz
 //
-// The rows of all frames are cut into chunks of equal length, whatever the
-// frames' lengths; the part of a frame inside a chunk is a piece.  Pieces are
-// numbered chunk + frame, which is unique because going from one piece to the
-// next advances at least one of the two.  A first kernel leaves two numbers
-// per piece and channel (mean and centred square sum; in the backward pass
-// sum dz and sum dz xhat, from which the group's sums and the gradients of
-// weight and bias both follow), a second joins the pieces of each frame in
-// their order, a third writes the result.  No atomics: results repeat bit
-// for bit.
+// By the mean size of a frame:
+//
+// Small frames: a CTA takes whole frames, reads each twice (the second time
+// from L1 or L2) and needs no other CTA.
+//
+// Larger frames: the rows of all frames are cut into one chunk for each
+// resident CTA, whatever the frames' lengths; the part of a frame inside a
+// chunk is a piece.  Pieces are numbered chunk + frame, which is unique because
+// going from one piece to the next advances at least one of the two.  A first
+// kernel leaves two numbers per piece and channel (mean and centred square
+// sum; in the backward pass sum dz and sum dz xhat, from which the group's sums
+// and the gradients of weight and bias both follow), a second joins the pieces
+// of each frame in their order, a third writes the result.  It walks each chunk
+// from its end, where the first kernel stopped, so that what L2 still holds is
+// read from there.
+//
+// Sums are float32 over the rows of one thread (64 terms at a time, about a
+// value of the piece, so a mean far from 0 takes no digits from the variance)
+// and float64 across threads and pieces.  No atomics: results repeat bit for
+// bit.
+//
+// z is one multiply-add, x A + B with A = rstd w and B = b - mean A: B's
+// rounding is 2^-24 |mean| rstd w, as large as that of the stored mean.
+#include <type_traits>
+
 #include "launch.cuh"
 
 namespace bysj {
@@ -47,119 +63,484 @@ struct GroupArgs {
   const void* grad_out;
   void* out;
   Frames frames;
-  int64_t channels, groups, group_channels;
-  int64_t chunk_rows, chunks;
+  int channels, groups, group_channels;
   const float* weight;
   const float* bias;
-  float* mean;
+  float* mean;  // forward: outputs
   float* rstd;
   float eps;
   int activation;
-  float2* partial;  // [chunks + frames][channels]
-  float2* sums;     // [frames][groups]: mean(d), mean(d xhat)
   float* grad_weight;
   float* grad_bias;
+  float2* affine;  // backward, frame kernel: [CTAs][channels] sum dz, sum dz xhat
+  // chunks
+  int64_t chunk_rows, chunks;
+  float2* partial;      // [chunks + frames][channels]
+  float2* sums;         // backward: [frames][groups] mean(d), mean(d xhat)
 };
 
-__device__ __forceinline__ float load_f32(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float load_f32(const float* p) { return *p; }
 __device__ __forceinline__ float load_f32(const __nv_bfloat16* p) {
   return __bfloat162float(*p);
 }
-__device__ __forceinline__ void store_value(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_value(__nv_bfloat16* p, float v) {
-  *p = __float2bfloat16_rn(v);
+
+// VEC values at p (global or shared memory).
+template <int VEC>
+__device__ __forceinline__ void load_vec(const float* p, float (&v)[VEC]) {
+  if constexpr (VEC == 4) {
+    const float4 q = *reinterpret_cast<const float4*>(p);
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+  } else {
+    v[0] = *p;
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float (&v)[VEC]) {
+  if constexpr (VEC == 4) {
+    const uint2 q = *reinterpret_cast<const uint2*>(p);
+    v[0] = bf16_lo(q.x); v[1] = bf16_hi(q.x); v[2] = bf16_lo(q.y); v[3] = bf16_hi(q.y);
+  } else {
+    v[0] = __bfloat162float(*p);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store_vec(float* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 4) __stcs(reinterpret_cast<float4*>(p), make_float4(v[0], v[1], v[2], v[3]));
+  else __stcs(p, v[0]);
+}
+template <int VEC>
+__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 4) {
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+    __stcs(reinterpret_cast<uint2*>(p), *reinterpret_cast<uint2*>(h));
+  } else {
+    p[0] = __float2bfloat16_rn(v[0]);
+  }
 }
 
-__device__ __forceinline__ float activate(float z, int activation) {
-  if (activation == BYSJ_ACT_NONE) return z;
-  const float s = 1.0f / (1.0f + expf(-z));
-  return activation == BYSJ_ACT_SILU ? z * s : s;
-}
-
-__device__ __forceinline__ float activate_grad(float z, int activation) {
-  if (activation == BYSJ_ACT_NONE) return 1.0f;
-  const float s = 1.0f / (1.0f + expf(-z));
-  return activation == BYSJ_ACT_SILU ? s * (1.0f + z * (1.0f - s)) : s * (1.0f - s);
-}
-
-// Threads of a CTA: `tx` channels side by side, `ty` rows at a time.
-struct Tile {
-  int tx, ty, cx, ry;
-  __device__ explicit Tile(int64_t channels) {
-    tx = channels < kBlock ? static_cast<int>(channels) : kBlock;
-    ty = kBlock / tx;
-    cx = threadIdx.x % tx;
-    ry = threadIdx.x / tx;
+// VEC values as loaded.
+template <typename T, int VEC>
+struct Raw {
+  static constexpr int kBytes = VEC * sizeof(T);
+  using Word = std::conditional_t<
+      kBytes == 16, uint4,
+      std::conditional_t<kBytes == 8, uint2,
+                         std::conditional_t<kBytes == 4, uint32_t, uint16_t>>>;
+  Word word;
+  __device__ __forceinline__ void load(const T* p) { word = *reinterpret_cast<const Word*>(p); }
+  __device__ __forceinline__ void get(float (&v)[VEC]) const {
+    load_vec<VEC>(reinterpret_cast<const T*>(&word), v);
   }
 };
 
-// Sum over the CTA's rows of one channel column; the total is returned to the
-// threads of row 0.
-__device__ __forceinline__ double column_sum(double v, const Tile& t, double* scratch) {
-  __syncthreads();
-  if (t.ry < t.ty) scratch[t.ry * t.tx + t.cx] = v;
-  __syncthreads();
-  double total = 0.0;
-  if (t.ry == 0)
-    for (int i = 0; i < t.ty; ++i) total += scratch[i * t.tx + t.cx];
-  return total;
+// 1 / (1 + exp(-z)) by the approximate exponential and reciprocal (2 units
+// and 1 unit in the last place; the product adds |z| 2^-24).
+__device__ __forceinline__ float sigmoid(float z) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2_ftz(z * -1.4426950408889634f)));
+  return r;
+}
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (ACT == BYSJ_ACT_NONE) return z;
+  const float s = sigmoid(z);
+  return ACT == BYSJ_ACT_SILU ? z * s : s;
+}
+template <int ACT>
+__device__ __forceinline__ float activate_grad(float z) {
+  if constexpr (ACT == BYSJ_ACT_NONE) return 1.0f;
+  const float s = sigmoid(z), t = 1.0f - s;
+  return ACT == BYSJ_ACT_SILU ? fmaf(s * t, z, s) : s * t;
 }
 
-// Per piece and channel: forward, the mean and the sum of squares about it;
-// backward, sum dz and sum dz xhat.
+// Threads over a tile of channels: cv vectors side by side, ty rows at a time.
+template <int VEC, int THREADS>
+struct Tile {
+  int c0, width, ty, ry, c;  // c: first channel of this thread
+  bool on;
+  __device__ Tile(int begin, int channels) {
+    c0 = begin;
+    width = min(channels - begin, THREADS * VEC);
+    const int cv = width / VEC;
+    ty = THREADS / cv;
+    ry = threadIdx.x / cv;
+    c = begin + (threadIdx.x % cv) * VEC;
+    on = ry < ty;
+  }
+};
+
+// Per channel of a thread: xhat = x r + o, z = xhat w + b (forward: z = x r + o
+// with weight and bias in r and o), and dx = dz k - xhat s - t.
+template <int VEC>
+struct Columns {
+  float r[VEC], o[VEC], w[VEC], b[VEC], k[VEC], s[VEC], t[VEC];
+  template <bool BACKWARD>
+  __device__ __forceinline__ void set(const GroupArgs& a, int c, int i, float mean, float rstd,
+                                      float2 sums) {
+    w[i] = a.weight ? __ldg(a.weight + c) : 1.0f;
+    b[i] = a.bias ? __ldg(a.bias + c) : 0.0f;
+    if constexpr (BACKWARD) {
+      r[i] = rstd;
+      o[i] = -mean * rstd;
+      k[i] = rstd * w[i];
+      s[i] = rstd * sums.y;
+      t[i] = rstd * sums.x;
+    } else {
+      r[i] = rstd * w[i];
+      o[i] = fmaf(-mean, r[i], b[i]);
+    }
+  }
+};
+
+// A channel's pair from its sums over `rows` rows; forward sums are about x[c].
 template <typename T, bool BACKWARD>
-__global__ void __launch_bounds__(kBlock) group_partial_kernel(GroupArgs a) {
-  __shared__ double scratch[kBlock];
-  const Tile t(a.channels);
-  const int64_t chunk = blockIdx.x;
-  const int64_t r0 = chunk * a.chunk_rows;
-  const int64_t r1 = min(r0 + a.chunk_rows, a.frames.rows);
+__device__ __forceinline__ float2 channel_value(double s1, double s2, int64_t rows, const T* x,
+                                                int c) {
+  if constexpr (BACKWARD) return make_float2(static_cast<float>(s1), static_cast<float>(s2));
+  const double n = static_cast<double>(rows);
+  return make_float2(static_cast<float>(load_f32(x + c) + s1 / n),
+                     static_cast<float>(s2 - s1 * s1 / n));
+}
+
+// Channel sums over a slab's rows into chan[] (forward: mean and the sum of
+// squares about it; backward: sum dz, sum dz xhat).  Ends synchronised.
+template <typename T, int VEC, int THREADS, bool BACKWARD, int ACT>
+__device__ __forceinline__ void column_stats(const Tile<VEC, THREADS>& t, const T* x, const T* dy,
+                                             int64_t rows, int channels, const Columns<VEC>& q,
+                                             float* scratch, double2* level, float2* chan) {
+  float s1[VEC], s2[VEC], pivot[VEC], o1[VEC], o2[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = o1[i] = o2[i] = pivot[i] = 0.0f;
+  if (t.on) {
+    if constexpr (!BACKWARD) load_vec<VEC>(x + t.c, pivot);
+    auto add = [&](const float (&v)[VEC], const float (&g)[VEC]) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if constexpr (BACKWARD) {
+          const float xhat = fmaf(v[i], q.r[i], q.o[i]);
+          const float dz = g[i] * activate_grad<ACT>(fmaf(xhat, q.w[i], q.b[i]));
+          s1[i] += dz;
+          s2[i] = fmaf(dz, xhat, s2[i]);
+        } else {
+          const float d = v[i] - pivot[i];
+          s1[i] += d;
+          s2[i] = fmaf(d, d, s2[i]);
+        }
+      }
+    };
+    // kAhead rows are requested before the first is used
+    constexpr int kAhead = BACKWARD ? 4 : 8;
+    const int64_t step = static_cast<int64_t>(t.ty) * channels;
+    const T* px = x + t.ry * static_cast<int64_t>(channels) + t.c;
+    const T* pg = dy + t.ry * static_cast<int64_t>(channels) + t.c;
+    int64_t n = rows > t.ry ? (rows - t.ry + t.ty - 1) / t.ty : 0;  // rows of this thread
+    int left = 64;  // terms of the inner sums before they join the outer ones
+    for (; n >= kAhead; n -= kAhead) {
+      Raw<T, VEC> v[kAhead], g[BACKWARD ? kAhead : 1];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        v[j].load(px);
+        px += step;
+        if constexpr (BACKWARD) {
+          g[j].load(pg);
+          pg += step;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        float fv[VEC], fg[VEC];
+        v[j].get(fv);
+        g[BACKWARD ? j : 0].get(fg);
+        add(fv, fg);
+      }
+      left -= kAhead;
+      if (left == 0) {
+        left = 64;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          o1[i] += s1[i];
+          o2[i] += s2[i];
+          s1[i] = s2[i] = 0.0f;
+        }
+      }
+    }
+    for (; n > 0; --n) {
+      float fv[VEC], fg[VEC];
+      load_vec<VEC>(px, fv);
+      if constexpr (BACKWARD) load_vec<VEC>(pg, fg);
+      px += step;
+      pg += step;
+      add(fv, fg);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      s1[i] += o1[i];
+      s2[i] += o2[i];
+    }
+    float* place = scratch + t.ry * t.width + t.c - t.c0;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      place[i] = s1[i];
+      place[THREADS * VEC + i] = s2[i];
+    }
+  }
+  __syncthreads();
+  // THREADS / width parts of the rows side by side, then the parts in order
+  const int parts = t.width < THREADS ? THREADS / t.width : 1;
+  const int share = (t.ty + parts - 1) / parts;
+  for (int i = threadIdx.x; i < parts * t.width; i += THREADS) {
+    const int part = i / t.width, c = i % t.width;
+    double a1 = 0.0, a2 = 0.0;
+    for (int r = part * share; r < min((part + 1) * share, t.ty); ++r) {
+      a1 += scratch[r * t.width + c];
+      a2 += scratch[THREADS * VEC + r * t.width + c];
+    }
+    if (parts > 1) {
+      level[i] = make_double2(a1, a2);
+    } else {
+      chan[t.c0 + c] = channel_value<T, BACKWARD>(a1, a2, rows, x, t.c0 + c);
+    }
+  }
+  __syncthreads();
+  if (parts > 1) {
+    for (int c = threadIdx.x; c < t.width; c += THREADS) {
+      double a1 = 0.0, a2 = 0.0;
+      for (int part = 0; part < parts; ++part) {
+        a1 += level[part * t.width + c].x;
+        a2 += level[part * t.width + c].y;
+      }
+      chan[t.c0 + c] = channel_value<T, BACKWARD>(a1, a2, rows, x, t.c0 + c);
+    }
+    __syncthreads();
+  }
+}
+
+// One warp: the channels of group g joined.  Forward: mean and sum of squares
+// about it of `rows` rows; backward: sum d and sum d xhat, d = dz w.
+template <bool BACKWARD>
+__device__ __forceinline__ float2 join_channels(const GroupArgs& a, const float2* chan, int g,
+                                                int64_t rows) {
+  const int lane = lane_id(), c0 = g * a.group_channels;
+  double s1 = 0.0, s2 = 0.0;
+  for (int c = c0 + lane; c < c0 + a.group_channels; c += kWarp) {
+    const double w = BACKWARD && a.weight ? __ldg(a.weight + c) : 1.0;
+    s1 += w * chan[c].x;
+    s2 += w * chan[c].y;
+  }
+  s1 = xor_sum(s1, 1);
+  if constexpr (!BACKWARD) {
+    s1 /= a.group_channels;
+    for (int c = c0 + lane; c < c0 + a.group_channels; c += kWarp) {
+      const double d = chan[c].x - s1;
+      s2 += static_cast<double>(rows) * d * d;
+    }
+  }
+  s2 = xor_sum(s2, 1);
+  return make_float2(static_cast<float>(s1), static_cast<float>(s2));
+}
+
+// y or dx of `rows` rows, the last first.  The result is written past L1 with
+// the first place in line to leave L2: nothing here reads it again.
+template <typename T, int VEC, int THREADS, bool BACKWARD, int ACT>
+__device__ __forceinline__ void apply_rows(const Tile<VEC, THREADS>& t, const T* x, const T* dy,
+                                           T* out, int64_t rows, int channels,
+                                           const Columns<VEC>& q) {
+  if (!t.on) return;
+  constexpr int kAhead = 4;
+  const int64_t step = static_cast<int64_t>(t.ty) * channels;
+  int64_t n = rows > t.ry ? (rows - t.ry + t.ty - 1) / t.ty : 0;
+  const int64_t at = (t.ry + (n - 1) * t.ty) * static_cast<int64_t>(channels) + t.c;
+  const T* px = x + at;
+  const T* pg = dy + at;
+  T* py = out + at;
+  auto put = [&](const Raw<T, VEC>& v, const Raw<T, VEC>& g) {
+    float fv[VEC], fg[VEC];
+    v.get(fv);
+    g.get(fg);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      if constexpr (BACKWARD) {
+        const float xhat = fmaf(fv[i], q.r[i], q.o[i]);
+        const float dz = fg[i] * activate_grad<ACT>(fmaf(xhat, q.w[i], q.b[i]));
+        fv[i] = fmaf(dz, q.k[i], -fmaf(xhat, q.s[i], q.t[i]));
+      } else {
+        fv[i] = activate<ACT>(fmaf(fv[i], q.r[i], q.o[i]));
+      }
+    }
+    store_vec<VEC>(py, fv);
+    py -= step;
+  };
+  for (; n >= kAhead; n -= kAhead) {
+    Raw<T, VEC> v[kAhead], g[BACKWARD ? kAhead : 1];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      v[j].load(px);
+      px -= step;
+      if constexpr (BACKWARD) {
+        g[j].load(pg);
+        pg -= step;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) put(v[j], g[BACKWARD ? j : 0]);
+  }
+  for (; n > 0; --n) {
+    Raw<T, VEC> v, g;
+    v.load(px);
+    px -= step;
+    g = v;
+    if constexpr (BACKWARD) {
+      g.load(pg);
+      pg -= step;
+    }
+    put(v, g);
+  }
+}
+
+// Shared memory of both kernels: float scratch [2][THREADS * VEC], double2 level [THREADS], chan [channels], stats
+// [groups] and, backward, the affine sums [channels].
+template <int VEC, int THREADS>
+__host__ __device__ constexpr size_t fixed_smem(int channels, int groups, bool backward) {
+  return sizeof(float) * 2 * THREADS * VEC + sizeof(double2) * THREADS +
+         sizeof(float2) * (static_cast<size_t>(channels) * (backward ? 2 : 1) + groups);
+}
+
+template <int VEC, int THREADS>
+struct Smem {
+  double2* level;
+  float* scratch;
+  float2 *chan, *stats, *affine;
+  __device__ Smem(unsigned char* base, int channels, int groups) {
+    level = reinterpret_cast<double2*>(base);
+    scratch = reinterpret_cast<float*>(level + THREADS);
+    chan = reinterpret_cast<float2*>(scratch + 2 * THREADS * VEC);
+    stats = chan + channels;
+    affine = stats + groups;
+  }
+};
+
+__device__ __forceinline__ float2 moments(const GroupArgs& a, double mean, double square,
+                                          double n) {
+  return make_float2(static_cast<float>(mean), static_cast<float>(1.0 / sqrt(square / n + a.eps)));
+}
+
+// Statistics of one tile's thread: mean and rstd of frame b, and its sums.
+template <int VEC, int THREADS, bool BACKWARD>
+__device__ __forceinline__ void set_columns(const GroupArgs& a, const Tile<VEC, THREADS>& t,
+                                            int64_t b, const float2* sums, Columns<VEC>& q) {
+  if (!t.on) return;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const int64_t at = b * a.groups + (t.c + i) / a.group_channels;
+    q.template set<BACKWARD>(a, t.c + i, i, a.mean[at], a.rstd[at],
+                             sums ? sums[at] : make_float2(0.0f, 0.0f));
+  }
+}
+
+// Whole frames, one CTA each, in steps of the grid.
+template <typename T, int VEC, int THREADS, bool BACKWARD, int ACT>
+__global__ void __launch_bounds__(THREADS) group_frame_kernel(GroupArgs a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  const Smem<VEC, THREADS> m(smem, a.channels, a.groups);
+  const int warp = threadIdx.x / kWarp;
+  if constexpr (BACKWARD)
+    for (int c = threadIdx.x; c < a.channels; c += THREADS) m.affine[c] = make_float2(0.f, 0.f);
+  for (int64_t b = blockIdx.x; b < a.frames.count; b += gridDim.x) {
+    const int64_t begin = a.frames.begin(b), rows = a.frames.begin(b + 1) - begin;
+    const T* x = static_cast<const T*>(a.x) + begin * a.channels;
+    const T* dy = static_cast<const T*>(BACKWARD ? a.grad_out : a.x) + begin * a.channels;
+    T* out = static_cast<T*>(a.out) + begin * a.channels;
+    if (rows <= 0) {
+      if constexpr (!BACKWARD)
+        for (int g = threadIdx.x; g < a.groups; g += THREADS)
+          a.mean[b * a.groups + g] = a.rstd[b * a.groups + g] = 0.0f;
+      continue;
+    }
+    __syncthreads();
+    Columns<VEC> q;
+    for (int c0 = 0; c0 < a.channels; c0 += THREADS * VEC) {
+      const Tile<VEC, THREADS> t(c0, a.channels);
+      if constexpr (BACKWARD) set_columns<VEC, THREADS, true>(a, t, b, nullptr, q);
+      column_stats<T, VEC, THREADS, BACKWARD, ACT>(t, x, dy, rows, a.channels, q, m.scratch,
+                                                   m.level, m.chan);
+    }
+    for (int g = warp; g < a.groups; g += THREADS / kWarp) {
+      const float2 v = join_channels<BACKWARD>(a, m.chan, g, rows);
+      const double n = static_cast<double>(rows) * a.group_channels;
+      if (lane_id() == 0) {
+        if constexpr (BACKWARD) {
+          m.stats[g] = make_float2(static_cast<float>(v.x / n), static_cast<float>(v.y / n));
+        } else {
+          m.stats[g] = moments(a, v.x, v.y, n);
+          a.mean[b * a.groups + g] = m.stats[g].x;
+          a.rstd[b * a.groups + g] = m.stats[g].y;
+        }
+      }
+    }
+    if constexpr (BACKWARD)
+      for (int c = threadIdx.x; c < a.channels; c += THREADS) {
+        m.affine[c].x += m.chan[c].x;
+        m.affine[c].y += m.chan[c].y;
+      }
+    __syncthreads();
+    for (int c0 = 0; c0 < a.channels; c0 += THREADS * VEC) {
+      const Tile<VEC, THREADS> t(c0, a.channels);
+      if (t.on) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const int g = (t.c + i) / a.group_channels;
+          const float2 v = m.stats[g];
+          if constexpr (BACKWARD)
+            q.template set<true>(a, t.c + i, i, a.mean[b * a.groups + g],
+                                 a.rstd[b * a.groups + g], v);
+          else q.template set<false>(a, t.c + i, i, v.x, v.y, v);
+        }
+      }
+      apply_rows<T, VEC, THREADS, BACKWARD, ACT>(t, x, dy, out, rows, a.channels, q);
+    }
+  }
+  if constexpr (BACKWARD) {
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.channels; c += THREADS)
+      a.affine[static_cast<int64_t>(blockIdx.x) * a.channels + c] = m.affine[c];
+  }
+}
+
+// ---- chunks of all frames ---------------------------------------------------
+
+constexpr int kChunkThreads = 256;
+
+// APPLY: y or dx; otherwise the pieces' numbers.  One chunk a CTA.
+template <typename T, int VEC, bool BACKWARD, int ACT, bool APPLY>
+__global__ void __launch_bounds__(kChunkThreads, BACKWARD ? 3 : 4)
+    group_chunk_kernel(GroupArgs a) {
+  constexpr int kThreads = kChunkThreads;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const Smem<VEC, kThreads> m(smem, a.channels, a.groups);
+  const int C = a.channels;
   const T* x = static_cast<const T*>(a.x);
-  const T* dy = static_cast<const T*>(a.grad_out);
+  const T* dy = static_cast<const T*>(BACKWARD ? a.grad_out : a.x);
+  const int64_t chunk = blockIdx.x;
+  const int64_t r0 = chunk * a.chunk_rows, r1 = min(r0 + a.chunk_rows, a.frames.rows);
   int64_t lo = r0;
   for (int64_t b = a.frames.of_row(r0); b < a.frames.count && lo < r1; ++b) {
     const int64_t hi = min(a.frames.begin(b + 1), r1);
     if (hi <= lo) continue;
-    for (int64_t c0 = 0; c0 < a.channels; c0 += t.tx) {
-      const int64_t c = c0 + t.cx;
-      const bool on = t.ry < t.ty && c < a.channels;
-      double s1 = 0.0, s2 = 0.0;
-      float pivot = 0.0f;
-      if (on) {
-        if constexpr (BACKWARD) {
-          const int64_t g = c / a.group_channels;
-          const float mean = a.mean[b * a.groups + g], rstd = a.rstd[b * a.groups + g];
-          const float w = a.weight ? a.weight[c] : 1.0f, bias = a.bias ? a.bias[c] : 0.0f;
-          for (int64_t r = lo + t.ry; r < hi; r += t.ty) {
-            const float xhat = (load_f32(x + r * a.channels + c) - mean) * rstd;
-            const float dz = load_f32(dy + r * a.channels + c) *
-                             activate_grad(xhat * w + bias, a.activation);
-            s1 += dz;
-            s2 += static_cast<double>(dz * xhat);
-          }
-        } else {
-          // squares about a value of the piece, not about 0: a mean far from
-          // 0 takes no digits from the variance
-          pivot = load_f32(x + lo * a.channels + c);
-          for (int64_t r = lo + t.ry; r < hi; r += t.ty) {
-            const float d = load_f32(x + r * a.channels + c) - pivot;
-            s1 += d;
-            s2 += static_cast<double>(d * d);
-          }
-        }
-      }
-      s1 = column_sum(s1, t, scratch);
-      s2 = column_sum(s2, t, scratch);
-      if (on && t.ry == 0) {
-        float2 v;
-        if constexpr (BACKWARD) {
-          v = make_float2(static_cast<float>(s1), static_cast<float>(s2));
-        } else {
-          const double n = static_cast<double>(hi - lo);
-          v = make_float2(static_cast<float>(pivot + s1 / n),
-                          static_cast<float>(s2 - s1 * s1 / n));
-        }
-        a.partial[(chunk + b) * a.channels + c] = v;
+    for (int c0 = 0; c0 < C; c0 += kThreads * VEC) {
+      const Tile<VEC, kThreads> t(c0, C);
+      Columns<VEC> q;
+      if constexpr (APPLY) {
+        set_columns<VEC, kThreads, BACKWARD>(a, t, b, BACKWARD ? a.sums : nullptr, q);
+        apply_rows<T, VEC, kThreads, BACKWARD, ACT>(t, x + lo * C, dy + lo * C,
+                                                    static_cast<T*>(a.out) + lo * C, hi - lo, C,
+                                                    q);
+      } else {
+        if constexpr (BACKWARD) set_columns<VEC, kThreads, true>(a, t, b, nullptr, q);
+        column_stats<T, VEC, kThreads, BACKWARD, ACT>(t, x + lo * C, dy + lo * C, hi - lo, C, q,
+                                                      m.scratch, m.level, m.chan);
+        for (int c = threadIdx.x; c < t.width; c += kThreads)
+          a.partial[(chunk + b) * C + c0 + c] = m.chan[c0 + c];
+        __syncthreads();
       }
     }
     lo = hi;
@@ -176,156 +557,241 @@ __device__ __forceinline__ double block_sum(double v, double* scratch) {
   return total;
 }
 
-// Joins the pieces of frame blockIdx.x for group blockIdx.y.
-template <bool BACKWARD>
-__global__ void __launch_bounds__(kBlock) group_join_kernel(GroupArgs a) {
-  __shared__ double scratch[kWarpsPerBlock];
-  const int64_t b = blockIdx.x;
-  const int64_t r0 = a.frames.begin(b), r1 = a.frames.begin(b + 1);
-  const double n = static_cast<double>(r1 - r0) * static_cast<double>(a.group_channels);
-  for (int64_t g = blockIdx.y; g < a.groups; g += gridDim.y) {
-    if (r1 <= r0) {
-      if (threadIdx.x == 0) {
-        if constexpr (BACKWARD) {
-          a.sums[b * a.groups + g] = make_float2(0.0f, 0.0f);
-        } else {
-          a.mean[b * a.groups + g] = 0.0f;
-          a.rstd[b * a.groups + g] = 0.0f;
-        }
-      }
-      continue;
-    }
-    const int64_t first = r0 / a.chunk_rows, last = (r1 - 1) / a.chunk_rows;
-    const int64_t items = (last - first + 1) * a.group_channels;
-    double s1 = 0.0, s2 = 0.0;
-    for (int64_t i = threadIdx.x; i < items; i += kBlock) {
-      const int64_t chunk = first + i / a.group_channels;
-      const int64_t c = g * a.group_channels + i % a.group_channels;
-      const float2 v = a.partial[(chunk + b) * a.channels + c];
-      if constexpr (BACKWARD) {
-        const double w = a.weight ? a.weight[c] : 1.0;
-        s1 += w * v.x;
-        s2 += w * v.y;
-      } else {
-        const int64_t begin = max(chunk * a.chunk_rows, r0);
-        const int64_t end = min((chunk + 1) * a.chunk_rows, r1);
-        s1 += static_cast<double>(end - begin) * v.x;
-      }
-    }
-    const double mean = block_sum(s1, scratch) / n;
-    if constexpr (BACKWARD) {
-      s2 = block_sum(s2, scratch) / n;
-      if (threadIdx.x == 0)
-        a.sums[b * a.groups + g] =
-            make_float2(static_cast<float>(mean), static_cast<float>(s2));
-    } else {
-      for (int64_t i = threadIdx.x; i < items; i += kBlock) {
-        const int64_t chunk = first + i / a.group_channels;
-        const int64_t c = g * a.group_channels + i % a.group_channels;
-        const float2 v = a.partial[(chunk + b) * a.channels + c];
-        const int64_t begin = max(chunk * a.chunk_rows, r0);
-        const int64_t end = min((chunk + 1) * a.chunk_rows, r1);
-        const double d = v.x - mean;
-        s2 += v.y + static_cast<double>(end - begin) * d * d;
-      }
-      s2 = block_sum(s2, scratch) / n;
-      if (threadIdx.x == 0) {
-        a.mean[b * a.groups + g] = static_cast<float>(mean);
-        a.rstd[b * a.groups + g] = static_cast<float>(1.0 / sqrt(s2 + a.eps));
-      }
-    }
-  }
-}
-
-template <typename T, bool BACKWARD>
-__global__ void __launch_bounds__(kBlock) group_apply_kernel(GroupArgs a) {
-  const Tile t(a.channels);
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.chunk_rows;
-  const int64_t r1 = min(r0 + a.chunk_rows, a.frames.rows);
-  const T* x = static_cast<const T*>(a.x);
-  const T* dy = static_cast<const T*>(a.grad_out);
-  T* out = static_cast<T*>(a.out);
-  int64_t lo = r0;
-  for (int64_t b = a.frames.of_row(r0); b < a.frames.count && lo < r1; ++b) {
-    const int64_t hi = min(a.frames.begin(b + 1), r1);
-    if (hi <= lo) continue;
-    for (int64_t c = t.cx; c < a.channels && t.ry < t.ty; c += t.tx) {
-      const int64_t g = c / a.group_channels;
-      const float mean = a.mean[b * a.groups + g], rstd = a.rstd[b * a.groups + g];
-      const float w = a.weight ? a.weight[c] : 1.0f, bias = a.bias ? a.bias[c] : 0.0f;
-      float2 sums = make_float2(0.0f, 0.0f);
-      if constexpr (BACKWARD) sums = a.sums[b * a.groups + g];
-      for (int64_t r = lo + t.ry; r < hi; r += t.ty) {
-        const int64_t i = r * a.channels + c;
-        const float xhat = (load_f32(x + i) - mean) * rstd;
-        const float z = xhat * w + bias;
-        if constexpr (BACKWARD) {
-          const float d = load_f32(dy + i) * activate_grad(z, a.activation) * w;
-          store_value(out + i, rstd * (d - sums.x - xhat * sums.y));
-        } else {
-          store_value(out + i, activate(z, a.activation));
-        }
-      }
-    }
-    lo = hi;
-  }
-}
-
-// grad_weight and grad_bias: the pieces of all frames, channel by channel.
-__global__ void __launch_bounds__(kBlock) group_affine_grad_kernel(GroupArgs a) {
-  __shared__ double scratch[kWarpsPerBlock];
-  const int64_t c = blockIdx.x;
+// Sums rows of channel pairs in a fixed order into the gradients of weight
+// and bias, 32 channels a CTA.
+__device__ __forceinline__ void affine_grad(const GroupArgs& a, int tile, const float2* rows,
+                                            int64_t count) {
+  __shared__ double2 part[kWarpsPerBlock][kWarp];
+  const int warp = threadIdx.x / kWarp, c = tile * kWarp + lane_id();
   double s1 = 0.0, s2 = 0.0;
-  for (int64_t chunk = threadIdx.x; chunk < a.chunks; chunk += kBlock) {
-    const int64_t r0 = chunk * a.chunk_rows;
-    const int64_t r1 = min(r0 + a.chunk_rows, a.frames.rows);
-    int64_t lo = r0;
-    for (int64_t b = a.frames.of_row(r0); b < a.frames.count && lo < r1; ++b) {
-      const int64_t hi = min(a.frames.begin(b + 1), r1);
-      if (hi <= lo) continue;
-      const float2 v = a.partial[(chunk + b) * a.channels + c];
+  if (c < a.channels) {
+#pragma unroll 8
+    for (int64_t i = warp; i < count; i += kWarpsPerBlock) {
+      const float2 v = rows[i * a.channels + c];
       s1 += v.x;
       s2 += v.y;
-      lo = hi;
     }
   }
-  s1 = block_sum(s1, scratch);
-  s2 = block_sum(s2, scratch);
-  if (threadIdx.x == 0) {
+  part[warp][lane_id()] = make_double2(s1, s2);
+  __syncthreads();
+  if (warp == 0 && c < a.channels) {
+    s1 = s2 = 0.0;
+    for (int i = 0; i < kWarpsPerBlock; ++i) {
+      s1 += part[i][lane_id()].x;
+      s2 += part[i][lane_id()].y;
+    }
     if (a.grad_bias) a.grad_bias[c] = static_cast<float>(s1);
     if (a.grad_weight) a.grad_weight[c] = static_cast<float>(s2);
   }
 }
 
-// Rows of a chunk: about four chunks for each SM, 16 to 512 rows.
-int64_t chunk_rows_of(int64_t rows) {
-  const int64_t want = rows / (static_cast<int64_t>(current_device_info().sm_count) * 4);
-  return want < 16 ? 16 : want > 512 ? 512 : want;
+__global__ void __launch_bounds__(kBlock) group_affine_kernel(GroupArgs a, int ctas) {
+  affine_grad(a, blockIdx.x, a.affine, ctas);
 }
 
-size_t carve_workspace(GroupArgs& a, void* workspace, bool backward) {
+// Joins the pieces of one frame and group a CTA (in steps of the grid); the
+// first `tiles` CTAs take the gradients of weight and bias, from all pieces
+// (rows that no piece has are zero).
+template <bool BACKWARD>
+__global__ void __launch_bounds__(kBlock) group_join_kernel(GroupArgs a, int tiles) {
+  __shared__ double scratch[kWarpsPerBlock];
+  if constexpr (BACKWARD) {
+    if (static_cast<int>(blockIdx.x) < tiles) {
+      affine_grad(a, blockIdx.x, a.partial, a.chunks + a.frames.count);
+      return;
+    }
+  }
+  const int64_t units = a.frames.count * a.groups;
+  for (int64_t unit = blockIdx.x - tiles; unit < units; unit += gridDim.x - tiles) {
+    const int64_t b = unit / a.groups;
+    const int g = static_cast<int>(unit % a.groups), c0 = g * a.group_channels;
+    const int64_t r0 = a.frames.begin(b), r1 = a.frames.begin(b + 1);
+    if (r1 <= r0) {
+      if constexpr (!BACKWARD)
+        if (threadIdx.x == 0) a.mean[unit] = a.rstd[unit] = 0.0f;
+      continue;
+    }
+    const int64_t first = r0 / a.chunk_rows, pieces = (r1 - 1) / a.chunk_rows - first + 1;
+    const double n = static_cast<double>(r1 - r0) * a.group_channels;
+    const float2* partial = a.partial + (first + b) * a.channels + c0;
+    // threads side by side over the group's channels, then over pieces; the
+    // sum and the sum of squares about the first piece's mean
+    const int width = a.group_channels < kBlock ? a.group_channels : kBlock;
+    const int lanes = kBlock / width, rank = threadIdx.x / width;
+    const double centre = BACKWARD ? 0.0 : partial->x;
+    double s1 = 0.0, s2 = 0.0;
+    if (rank < lanes) {
+      for (int c = threadIdx.x % width; c < a.group_channels; c += width) {
+        const double w = BACKWARD && a.weight ? __ldg(a.weight + c0 + c) : 1.0;
+#pragma unroll 8
+        for (int64_t p = rank; p < pieces; p += lanes) {
+          const float2 v = partial[p * a.channels + c];
+          if constexpr (BACKWARD) {
+            s1 += w * v.x;
+            s2 += w * v.y;
+          } else {
+            const double m = static_cast<double>(min((first + p + 1) * a.chunk_rows, r1) -
+                                                 max((first + p) * a.chunk_rows, r0));
+            const double d = v.x - centre;
+            s1 += m * d;
+            s2 += v.y + m * d * d;
+          }
+        }
+      }
+    }
+    s1 = block_sum(s1, scratch);
+    s2 = block_sum(s2, scratch);
+    if (threadIdx.x == 0) {
+      if constexpr (BACKWARD) {
+        a.sums[unit] = make_float2(static_cast<float>(s1 / n), static_cast<float>(s2 / n));
+      } else {
+        const float2 v = moments(a, centre + s1 / n, fmax(s2 - s1 * s1 / n, 0.0), n);
+        a.mean[unit] = v.x;
+        a.rstd[unit] = v.y;
+      }
+    }
+  }
+}
+
+// ---- host -------------------------------------------------------------------
+
+// A frame of at most this many bytes is one CTA's work: two passes over it
+// through L1 cost less than a meeting of CTAs.
+constexpr int64_t kSmallFrame = 64 * 1024;
+
+struct Plan {
+  bool chunked = false;
+  int ctas = 1;
+  int threads = 256;  // frame kernel
+  int64_t chunk_rows = 1, chunks = 0;
+};
+
+// Depends on sizes only, so that the workspace size follows from them; `item`
+// is the element size.
+Plan make_plan(int64_t rows, int64_t channels, int64_t frames, int item, bool backward) {
+  Plan p;
+  const int64_t sms = current_device_info().sm_count;
+  const int64_t row_bytes = channels * item;
+  p.chunked = rows * row_bytes / (frames > 0 ? frames : 1) > kSmallFrame;
+  // few frames: more threads for each
+  p.threads = frames <= sms ? 512 : 256;
+  p.ctas = static_cast<int>(frames < sms * 4 ? frames : sms * 4);
+  if (!p.chunked) return p;
+  // one chunk for each resident CTA, of 16 KB at least
+  const int64_t least = (16384 + row_bytes - 1) / row_bytes;
+  p.chunk_rows = (rows + sms * (backward ? 3 : 4) - 1) / (sms * (backward ? 3 : 4));
+  if (p.chunk_rows < least) p.chunk_rows = least;
+  p.chunks = (rows + p.chunk_rows - 1) / p.chunk_rows;
+  return p;
+}
+
+size_t carve_workspace(GroupArgs& a, const Plan& p, void* workspace, bool backward) {
   Carver carve(workspace);
-  a.partial = carve.take<float2>(static_cast<size_t>(a.chunks + a.frames.count) * a.channels);
-  if (backward) a.sums = carve.take<float2>(static_cast<size_t>(a.frames.count) * a.groups);
+  if (p.chunked) {
+    a.partial =
+        carve.take<float2>(static_cast<size_t>(p.chunks + a.frames.count) * a.channels);
+    if (backward) a.sums = carve.take<float2>(static_cast<size_t>(a.frames.count) * a.groups);
+  } else if (backward) {
+    a.affine = carve.take<float2>(static_cast<size_t>(p.ctas) * a.channels);
+  }
   return carve.need;
 }
 
-void plan(GroupArgs& a, int64_t rows, int64_t channels, int64_t groups, int64_t frames) {
-  a.frames.rows = rows;
+void set_sizes(GroupArgs& a, int64_t rows, int64_t channels, int64_t groups,
+               const int64_t* offsets, int64_t frames, int64_t inner) {
+  a.frames.offsets = offsets;
   a.frames.count = frames;
-  a.channels = channels;
-  a.groups = groups;
-  a.group_channels = channels / groups;
-  a.chunk_rows = chunk_rows_of(rows);
-  a.chunks = (rows + a.chunk_rows - 1) / a.chunk_rows;
+  a.frames.inner = inner;
+  a.frames.rows = rows;
+  a.channels = static_cast<int>(channels);
+  a.groups = static_cast<int>(groups);
+  a.group_channels = static_cast<int>(channels / groups);
 }
 
+// The larger of what the plans of either element size need.
 size_t workspace_size(int64_t rows, int64_t channels, int64_t groups, int64_t frames,
                       bool backward) {
   if (rows <= 0 || channels <= 0 || groups <= 0 || frames <= 0) return 0;
-  GroupArgs a{};
-  plan(a, rows, channels, groups, frames);
-  return carve_workspace(a, nullptr, backward);
+  size_t most = 0;
+  for (int item : {2, 4}) {
+    GroupArgs a{};
+    set_sizes(a, rows, channels, groups, nullptr, frames, 1);
+    const size_t need = carve_workspace(a, make_plan(rows, channels, frames, item, backward),
+                                        nullptr, backward);
+    if (need > most) most = need;
+  }
+  return most;
+}
+
+using GroupKernel = void (*)(GroupArgs);
+
+int launch_one(GroupKernel kernel, const char* name, unsigned ctas, int threads, size_t smem,
+               const GroupArgs& a, cudaStream_t s) {
+  const int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (st) return st;
+  kernel<<<ctas, threads, smem, s>>>(a);
+  return launch_check(name);
+}
+
+template <typename T, int VEC, bool BACKWARD, int ACT>
+int launch_act(const GroupArgs& a, const Plan& p, cudaStream_t s) {
+  const bool affine = BACKWARD && (a.grad_weight != nullptr || a.grad_bias != nullptr);
+  const int tiles = affine ? (a.channels + kWarp - 1) / kWarp : 0;
+  if (!p.chunked) {
+    const int st =
+        p.threads == 512
+            ? launch_one(group_frame_kernel<T, VEC, 512, BACKWARD, ACT>, "group_frame_kernel",
+                         p.ctas, 512, fixed_smem<VEC, 512>(a.channels, a.groups, BACKWARD), a, s)
+            : launch_one(group_frame_kernel<T, VEC, 256, BACKWARD, ACT>, "group_frame_kernel",
+                         p.ctas, 256, fixed_smem<VEC, 256>(a.channels, a.groups, BACKWARD), a, s);
+    if (st || !affine) return st;
+    group_affine_kernel<<<tiles, kBlock, 0, s>>>(a, p.ctas);
+    return launch_check("group_affine_kernel");
+  }
+  int st = BYSJ_OK;
+  if (affine)
+    st = cuda_check(cudaMemsetAsync(a.partial, 0,
+                                    sizeof(float2) * (a.chunks + a.frames.count) * a.channels, s),
+                    "group norm: zero the pieces");
+  if (st) return st;
+  const unsigned chunks = static_cast<unsigned>(p.chunks);
+  const size_t smem = fixed_smem<VEC, kChunkThreads>(a.channels, a.groups, BACKWARD);
+  st = launch_one(group_chunk_kernel<T, VEC, BACKWARD, ACT, false>, "group_chunk_kernel", chunks,
+                  kChunkThreads, smem, a, s);
+  if (st) return st;
+  const int64_t units = a.frames.count * a.groups;
+  group_join_kernel<BACKWARD>
+      <<<static_cast<unsigned>((units < 65536 ? units : 65536) + tiles), kBlock, 0, s>>>(a, tiles);
+  st = launch_check("group_join_kernel");
+  if (st) return st;
+  return launch_one(group_chunk_kernel<T, VEC, BACKWARD, ACT, true>, "group_chunk_kernel", chunks,
+                    kChunkThreads, 0, a, s);
+}
+
+template <typename T, int VEC, bool BACKWARD>
+int launch_vec(const GroupArgs& a, const Plan& p, cudaStream_t s) {
+  switch (a.activation) {
+    case BYSJ_ACT_SILU: return launch_act<T, VEC, BACKWARD, BYSJ_ACT_SILU>(a, p, s);
+    case BYSJ_ACT_SIGMOID: return launch_act<T, VEC, BACKWARD, BYSJ_ACT_SIGMOID>(a, p, s);
+    default: return launch_act<T, VEC, BACKWARD, BYSJ_ACT_NONE>(a, p, s);
+  }
+}
+
+template <typename T, bool BACKWARD>
+int launch(GroupArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
+  // four channels a thread: 16 or 8 bytes
+  constexpr uintptr_t kAlign = 4 * sizeof(T) - 1;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.out) |
+                        (BACKWARD ? reinterpret_cast<uintptr_t>(a.grad_out) : 0);
+  const bool vectors = a.channels % 4 == 0 && (all & kAlign) == 0;
+  const Plan p = make_plan(a.frames.rows, a.channels, a.frames.count, sizeof(T), BACKWARD);
+  const size_t need = carve_workspace(a, p, workspace, BACKWARD);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(BYSJ_ERR_WORKSPACE, "group norm: workspace of %zu bytes needed, %zu given", need,
+                workspace_bytes);
+  a.chunk_rows = p.chunk_rows;
+  a.chunks = p.chunks;
+  return vectors ? launch_vec<T, 4, BACKWARD>(a, p, s) : launch_vec<T, 1, BACKWARD>(a, p, s);
 }
 
 int check_shape(const char* name, int dtype, int64_t rows, int64_t channels, int64_t groups,
@@ -343,24 +809,10 @@ int check_shape(const char* name, int dtype, int64_t rows, int64_t channels, int
   if (activation != BYSJ_ACT_NONE && activation != BYSJ_ACT_SILU &&
       activation != BYSJ_ACT_SIGMOID)
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", name, activation);
-  if (frames > 0x7fffffff)
-    return fail(BYSJ_ERR_TOO_LARGE, "%s: more than 2^31 - 1 frames", name);
+  if (channels > BYSJ_GROUP_NORM_MAX_CHANNELS)
+    return fail(BYSJ_ERR_UNSUPPORTED, "%s: at most %d channels", name,
+                BYSJ_GROUP_NORM_MAX_CHANNELS);
   return BYSJ_OK;
-}
-
-template <typename T, bool BACKWARD>
-int launch(const GroupArgs& a, cudaStream_t s) {
-  const unsigned chunks = static_cast<unsigned>(a.chunks);
-  const dim3 joins(static_cast<unsigned>(a.frames.count),
-                   static_cast<unsigned>(a.groups < 65535 ? a.groups : 65535));
-  group_partial_kernel<T, BACKWARD><<<chunks, kBlock, 0, s>>>(a);
-  int st = launch_check("group_partial_kernel");
-  if (st) return st;
-  group_join_kernel<BACKWARD><<<joins, kBlock, 0, s>>>(a);
-  st = launch_check("group_join_kernel");
-  if (st) return st;
-  group_apply_kernel<T, BACKWARD><<<chunks, kBlock, 0, s>>>(a);
-  return launch_check("group_apply_kernel");
 }
 
 }  // namespace
@@ -402,13 +854,7 @@ int bysj_group_norm_forward(const void* x, int dtype, int64_t rows, int64_t chan
   if (x == nullptr || y == nullptr)
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "group norm: NULL pointer");
   GroupArgs a{};
-  plan(a, rows, channels, groups, frames);
-  const size_t need = carve_workspace(a, workspace, false);
-  if (workspace == nullptr || workspace_bytes < need)
-    return fail(BYSJ_ERR_WORKSPACE, "group norm: workspace of %zu bytes needed, %zu given", need,
-                workspace_bytes);
-  a.frames.offsets = offsets;
-  a.frames.inner = inner;
+  set_sizes(a, rows, channels, groups, offsets, frames, inner);
   a.x = x;
   a.out = y;
   a.weight = weight;
@@ -417,7 +863,8 @@ int bysj_group_norm_forward(const void* x, int dtype, int64_t rows, int64_t chan
   a.rstd = rstd;
   a.eps = eps;
   a.activation = activation;
-  return dtype == BYSJ_F32 ? launch<float, false>(a, s) : launch<__nv_bfloat16, false>(a, s);
+  return dtype == BYSJ_F32 ? launch<float, false>(a, workspace, workspace_bytes, s)
+                           : launch<__nv_bfloat16, false>(a, workspace, workspace_bytes, s);
 }
 
 int bysj_group_norm_backward(const void* grad_out, const void* x, int dtype, int64_t rows,
@@ -442,14 +889,7 @@ int bysj_group_norm_backward(const void* grad_out, const void* x, int dtype, int
       rstd == nullptr)
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "group norm backward: NULL pointer");
   GroupArgs a{};
-  plan(a, rows, channels, groups, frames);
-  const size_t need = carve_workspace(a, workspace, true);
-  if (workspace == nullptr || workspace_bytes < need)
-    return fail(BYSJ_ERR_WORKSPACE,
-                "group norm backward: workspace of %zu bytes needed, %zu given", need,
-                workspace_bytes);
-  a.frames.offsets = offsets;
-  a.frames.inner = inner;
+  set_sizes(a, rows, channels, groups, offsets, frames, inner);
   a.x = x;
   a.grad_out = grad_out;
   a.out = grad_x;
@@ -460,10 +900,8 @@ int bysj_group_norm_backward(const void* grad_out, const void* x, int dtype, int
   a.activation = activation;
   a.grad_weight = grad_weight;
   a.grad_bias = grad_bias;
-  st = dtype == BYSJ_F32 ? launch<float, true>(a, s) : launch<__nv_bfloat16, true>(a, s);
-  if (st || (grad_weight == nullptr && grad_bias == nullptr)) return st;
-  group_affine_grad_kernel<<<static_cast<unsigned>(channels), kBlock, 0, s>>>(a);
-  return launch_check("group_affine_grad_kernel");
+  return dtype == BYSJ_F32 ? launch<float, true>(a, workspace, workspace_bytes, s)
+                           : launch<__nv_bfloat16, true>(a, workspace, workspace_bytes, s);
 }
 
 }  // extern "C"

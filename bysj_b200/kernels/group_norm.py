@@ -16,6 +16,7 @@ from torch.autograd.function import once_differentiable
 from . import segment as _segment
 from .native import _extension, require_dcu
 
+MAX_CHANNELS = 8192
 _ACTIVATIONS = {None: 0, "none": 0, "silu": 1, "sigmoid": 2}
 
 
@@ -31,6 +32,8 @@ def _validate(x, groups, weight, bias, eps, activation, offsets):
         raise TypeError("group norm groups must be an int")
     if channels <= 0 or groups <= 0 or channels % groups:
         raise ValueError("group norm groups must divide the (positive) channel count")
+    if channels > MAX_CHANNELS:
+        raise ValueError(f"group norm takes at most {MAX_CHANNELS} channels")
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
@@ -101,4 +104,4 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     return _GroupNormFunction.apply(x, groups, weight, bias, eps, _ACTIVATIONS[activation], offsets)
 
 
-__all__ = ["group_norm"]
+__all__ = ["MAX_CHANNELS", "group_norm"]

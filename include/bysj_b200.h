@@ -509,7 +509,8 @@ BYSJ_API int bysj_rotary_axes(const bysj_rotary_side* q, const bysj_rotary_side*
  *   z = (x - mean) rstd w[c] + b[c],  rstd = 1 / sqrt(var + eps),  y = act(z)
  * weight / bias float32 [channels] or NULL; mean / rstd float32
  * [frames, groups] are outputs for the backward pass; an empty frame has
- * mean 0 and rstd 0. */
+ * mean 0 and rstd 0.  At most BYSJ_GROUP_NORM_MAX_CHANNELS channels. */
+#define BYSJ_GROUP_NORM_MAX_CHANNELS 8192
 BYSJ_API size_t bysj_group_norm_forward_workspace_size(int64_t rows, int64_t channels,
                                                        int64_t groups, int64_t frames);
 BYSJ_API int bysj_group_norm_forward(const void* x, int dtype, int64_t rows, int64_t channels,

@@ -162,6 +162,14 @@ NORM = [
     ([500, 300], (), 48, 4, F32, None, True, True, 1000.0),
     ([0, 0, 20000, 0], (), 40, 8, F32, "silu", True, True, 0.0),
     ([3000, 10], (), 8, 1, BF16, "sigmoid", False, True, 0.0),
+    # frames cut into slabs, joined across CTAs; vector and single loads
+    ([6000, 0, 9000, 1, 4000], (), 64, 8, F32, "silu", True, True, 0.5),
+    ([6000, 0, 9000, 1, 4000], (), 65, 5, BF16, "silu", True, True, 0.5),
+    ([700] * 9, (16,), 64, 4, F32, "silu", True, False, 0.3),
+    ([30000], (), 50, 25, F32, "sigmoid", True, False, 0.0),
+    # more slabs than are held at once: the frame is read again
+    ([140000], (), 128, 8, F32, "silu", True, False, 0.3),
+    ([5, 260000, 0, 9000], (), 72, 3, BF16, "silu", True, True, 0.3),
 ]
 
 
