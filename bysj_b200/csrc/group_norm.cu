@@ -133,6 +133,66 @@ struct Raw {
   }
 };
 
+// A thread's rows of one or two arrays, kRows at a time.
+template <typename T, int VEC, bool TWO>
+struct Rows {
+  static constexpr int kRows = 32 / (VEC * sizeof(T) * (TWO ? 2 : 1)) * (VEC == 1 ? 1 : 2);
+  Raw<T, VEC> a[kRows], b[TWO ? kRows : 1];
+  __device__ __forceinline__ void load(const T*& pa, const T*& pb, int64_t step) {
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      a[j].load(pa);
+      pa += step;
+      if constexpr (TWO) {
+        b[j].load(pb);
+        pb += step;
+      }
+    }
+  }
+  // The last 1 .. kRows - 1 rows.
+  __device__ __forceinline__ void load(const T* pa, const T* pb, int64_t step, int count) {
+#pragma unroll
+    for (int j = 0; j < kRows - 1; ++j) {
+      if (j >= count) continue;
+      a[j].load(pa);
+      pa += step;
+      if constexpr (TWO) {
+        b[j].load(pb);
+        pb += step;
+      }
+    }
+  }
+};
+
+// use(a, b) for n rows of a thread in order, the next kRows requested before
+// the last ones are used.
+template <typename T, int VEC, bool TWO, typename Use>
+__device__ __forceinline__ void each_row(const T* pa, const T* pb, int64_t step, int64_t n,
+                                         Use use) {
+  using RowsT = Rows<T, VEC, TWO>;
+  constexpr int kRows = RowsT::kRows;
+  const int rest = static_cast<int>(n % kRows);
+  auto apply = [&](const RowsT& rows, int j) {
+    float a[VEC], b[VEC];
+    rows.a[j].get(a);
+    rows.b[TWO ? j : 0].get(b);
+    use(a, b);
+  };
+  RowsT next;
+  if (n >= kRows) next.load(pa, pb, step);
+  else next.load(pa, pb, step, rest);
+  for (; n >= kRows; n -= kRows) {
+    const RowsT now = next;
+    if (n >= 2 * kRows) next.load(pa, pb, step);
+    else next.load(pa, pb, step, rest);
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) apply(now, j);
+  }
+#pragma unroll
+  for (int j = 0; j < kRows - 1; ++j)
+    if (j < rest) apply(next, j);
+}
+
 // 1 / (1 + exp(-z)) by the approximate exponential and reciprocal (2 units
 // and 1 unit in the last place; the product adds |z| 2^-24).
 __device__ __forceinline__ float sigmoid(float z) {
@@ -228,50 +288,22 @@ __device__ __forceinline__ void column_stats(const Tile<VEC, THREADS>& t, const 
         }
       }
     };
-    // kAhead rows are requested before the first is used
-    constexpr int kAhead = BACKWARD ? 4 : 8;
     const int64_t step = static_cast<int64_t>(t.ty) * channels;
     const T* px = x + t.ry * static_cast<int64_t>(channels) + t.c;
     const T* pg = dy + t.ry * static_cast<int64_t>(channels) + t.c;
-    int64_t n = rows > t.ry ? (rows - t.ry + t.ty - 1) / t.ty : 0;  // rows of this thread
+    const int64_t n = rows > t.ry ? (rows - t.ry + t.ty - 1) / t.ty : 0;  // of this thread
     int left = 64;  // terms of the inner sums before they join the outer ones
-    for (; n >= kAhead; n -= kAhead) {
-      Raw<T, VEC> v[kAhead], g[BACKWARD ? kAhead : 1];
+    each_row<T, VEC, BACKWARD>(px, pg, step, n, [&](const float(&v)[VEC], const float(&g)[VEC]) {
+      add(v, g);
+      if (--left > 0) return;
+      left = 64;
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        v[j].load(px);
-        px += step;
-        if constexpr (BACKWARD) {
-          g[j].load(pg);
-          pg += step;
-        }
+      for (int i = 0; i < VEC; ++i) {
+        o1[i] += s1[i];
+        o2[i] += s2[i];
+        s1[i] = s2[i] = 0.0f;
       }
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        float fv[VEC], fg[VEC];
-        v[j].get(fv);
-        g[BACKWARD ? j : 0].get(fg);
-        add(fv, fg);
-      }
-      left -= kAhead;
-      if (left == 0) {
-        left = 64;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          o1[i] += s1[i];
-          o2[i] += s2[i];
-          s1[i] = s2[i] = 0.0f;
-        }
-      }
-    }
-    for (; n > 0; --n) {
-      float fv[VEC], fg[VEC];
-      load_vec<VEC>(px, fv);
-      if constexpr (BACKWARD) load_vec<VEC>(pg, fg);
-      px += step;
-      pg += step;
-      add(fv, fg);
-    }
+    });
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       s1[i] += o1[i];
@@ -346,55 +378,28 @@ __device__ __forceinline__ void apply_rows(const Tile<VEC, THREADS>& t, const T*
                                            T* out, int64_t rows, int channels,
                                            const Columns<VEC>& q) {
   if (!t.on) return;
-  constexpr int kAhead = 4;
   const int64_t step = static_cast<int64_t>(t.ty) * channels;
-  int64_t n = rows > t.ry ? (rows - t.ry + t.ty - 1) / t.ty : 0;
+  const int64_t n = rows > t.ry ? (rows - t.ry + t.ty - 1) / t.ty : 0;
+  if (n == 0) return;
   const int64_t at = (t.ry + (n - 1) * t.ty) * static_cast<int64_t>(channels) + t.c;
   const T* px = x + at;
   const T* pg = dy + at;
   T* py = out + at;
-  auto put = [&](const Raw<T, VEC>& v, const Raw<T, VEC>& g) {
-    float fv[VEC], fg[VEC];
-    v.get(fv);
-    g.get(fg);
+  each_row<T, VEC, BACKWARD>(px, pg, -step, n, [&](const float(&v)[VEC], const float(&g)[VEC]) {
+    float y[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       if constexpr (BACKWARD) {
-        const float xhat = fmaf(fv[i], q.r[i], q.o[i]);
-        const float dz = fg[i] * activate_grad<ACT>(fmaf(xhat, q.w[i], q.b[i]));
-        fv[i] = fmaf(dz, q.k[i], -fmaf(xhat, q.s[i], q.t[i]));
+        const float xhat = fmaf(v[i], q.r[i], q.o[i]);
+        const float dz = g[i] * activate_grad<ACT>(fmaf(xhat, q.w[i], q.b[i]));
+        y[i] = fmaf(dz, q.k[i], -fmaf(xhat, q.s[i], q.t[i]));
       } else {
-        fv[i] = activate<ACT>(fmaf(fv[i], q.r[i], q.o[i]));
+        y[i] = activate<ACT>(fmaf(v[i], q.r[i], q.o[i]));
       }
     }
-    store_vec<VEC>(py, fv);
+    store_vec<VEC>(py, y);
     py -= step;
-  };
-  for (; n >= kAhead; n -= kAhead) {
-    Raw<T, VEC> v[kAhead], g[BACKWARD ? kAhead : 1];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      v[j].load(px);
-      px -= step;
-      if constexpr (BACKWARD) {
-        g[j].load(pg);
-        pg -= step;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) put(v[j], g[BACKWARD ? j : 0]);
-  }
-  for (; n > 0; --n) {
-    Raw<T, VEC> v, g;
-    v.load(px);
-    px -= step;
-    g = v;
-    if constexpr (BACKWARD) {
-      g.load(pg);
-      pg -= step;
-    }
-    put(v, g);
-  }
+  });
 }
 
 // Shared memory of both kernels: float scratch [2][THREADS * VEC], double2 level [THREADS], chan [channels], stats
