@@ -7,6 +7,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -806,6 +807,43 @@ std::tuple<Tensor, Tensor, Tensor> gie_zonal_scatter_backward(Tensor grad_output
   return {gz, gr, gi};
 }
 
+// ---- autograd of the training-step operators -----------------------------------
+//
+// Their gradients are autograd nodes in C++: a node called through Python costs
+// about 60 us more for a forward and backward call, several times what the
+// kernels of a small frame take.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+
+bool wants_grad(std::initializer_list<const Tensor*> tensors,
+                std::initializer_list<const OptTensor*> optional) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t->requires_grad()) return true;
+  for (const OptTensor* t : optional)
+    if (t->has_value() && (*t)->requires_grad()) return true;
+  return false;
+}
+
+// Gradients that cannot be differentiated again: with create_graph, an attempt
+// to go through them raises.
+variable_list once(variable_list grads, const char* op) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list live;
+  for (Tensor& g : grads)
+    if (g.defined()) live.push_back(g.detach().requires_grad_());
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string(op) + " is differentiable once", static_cast<int64_t>(live.size()));
+  const variable_list out = (*error)(variable_list(live));
+  size_t i = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = out[i++];
+  return grads;
+}
+
 // ---- rotary positions ----------------------------------------------------------
 
 // [tokens, heads, dim] with channel stride 1 and any other strides.
@@ -834,12 +872,13 @@ bysj_rotary_side rotary_side(const Tensor& x, const Tensor& y, const OptTensor& 
 }
 
 // Turns q and k; with saved_q / saved_k (the forward inputs) also returns the
-// gradient of float positions.
-std::tuple<Tensor, Tensor, OptTensor> rotary_axes(Tensor q, Tensor k, Tensor positions,
-                                                  Tensor inv_freq,
-                                                  std::vector<int64_t> sections,
-                                                  bool interleaved, bool inverse,
-                                                  OptTensor saved_q, OptTensor saved_k) {
+// gradient of float positions (else undefined).
+std::tuple<Tensor, Tensor, Tensor> rotary_turn(const Tensor& q, const Tensor& k,
+                                               const Tensor& positions, const Tensor& inv_freq,
+                                               const std::vector<int64_t>& sections,
+                                               bool interleaved, bool inverse,
+                                               const OptTensor& saved_q,
+                                               const OptTensor& saved_k) {
   const int dt = heads_dtype(q, "rotary q");
   TORCH_CHECK(heads_dtype(k, "rotary k") == dt, "rotary q and k must have one dtype");
   TORCH_CHECK(k.size(0) == q.size(0) && k.size(2) == q.size(2),
@@ -867,15 +906,57 @@ std::tuple<Tensor, Tensor, OptTensor> rotary_axes(Tensor q, Tensor k, Tensor pos
   }
   c10::cuda::CUDAGuard guard(q.device());
   Tensor yq = torch::empty(q.sizes(), q.options()), yk = torch::empty(k.sizes(), k.options());
-  OptTensor gp;
+  Tensor gp;
   if (saved_q) gp = torch::empty(positions.sizes(), positions.options());
   const bysj_rotary_side qs = rotary_side(q, yq, saved_q), ks = rotary_side(k, yk, saved_k);
   check(bysj_rotary_axes(&qs, &ks, dt, positions.data_ptr(), integers,
                          pairs ? inv_freq.data_ptr<float>() : nullptr, sections.data(),
                          static_cast<int>(axes), q.size(0), q.size(2), interleaved, inverse,
-                         gp ? gp->data_ptr<float>() : nullptr, stream_of(q)),
+                         saved_q ? gp.data_ptr<float>() : nullptr, stream_of(q)),
         "rotary_axes");
   return {yq, yk, gp};
+}
+
+Tensor channels_contiguous(const Tensor& t) {
+  return t.size(2) <= 1 || t.stride(2) == 1 ? t : t.contiguous();
+}
+
+class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                               const Tensor& positions, const Tensor& inv_freq,
+                               const std::vector<int64_t>& sections, bool interleaved) {
+    auto [yq, yk, none] = rotary_turn(q, k, positions, inv_freq, sections, interleaved, false,
+                                      std::nullopt, std::nullopt);
+    if (positions.requires_grad()) ctx->save_for_backward({positions, inv_freq, q, k});
+    else ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["interleaved"] = interleaved;
+    return {yq, yk};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool positions = saved.size() == 4;
+    auto [gq, gk, gp] = rotary_turn(
+        channels_contiguous(grads[0]), channels_contiguous(grads[1]), saved[0], saved[1],
+        ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), true,
+        positions ? OptTensor(saved[2]) : std::nullopt,
+        positions ? OptTensor(saved[3]) : std::nullopt);
+    return once({gq, gk, gp, Tensor(), Tensor(), Tensor()}, "rotary_axes");
+  }
+};
+
+std::tuple<Tensor, Tensor> rotary_axes(const Tensor& q, const Tensor& k, const Tensor& positions,
+                                       const Tensor& inv_freq,
+                                       const std::vector<int64_t>& sections, bool interleaved) {
+  if (!wants_grad({&q, &k, &positions}, {})) {
+    auto [yq, yk, none] = rotary_turn(q, k, positions, inv_freq, sections, interleaved, false,
+                                      std::nullopt, std::nullopt);
+    return {yq, yk};
+  }
+  const variable_list out =
+      RotaryFunction::apply(q, k, positions, inv_freq, sections, interleaved);
+  return {out[0], out[1]};
 }
 
 // ---- group norm -----------------------------------------------------------------
@@ -911,62 +992,102 @@ NormShape group_norm_shape(const Tensor& x, const OptTensor& offsets, const OptT
   return s;
 }
 
-std::tuple<Tensor, Tensor, Tensor> group_norm_forward(Tensor x, int64_t groups, OptTensor weight,
-                                                      OptTensor bias, double eps,
-                                                      int64_t activation, OptTensor offsets) {
+// Returns y and the statistics [2, frames, groups] (mean, rstd).
+std::tuple<Tensor, Tensor> group_norm_forward(const Tensor& x, int64_t groups,
+                                              const OptTensor& weight, const OptTensor& bias,
+                                              double eps, int64_t activation,
+                                              const OptTensor& offsets) {
   const int dt = value_dtype(x, "group norm input");
   const NormShape s = group_norm_shape(x, offsets, weight, bias);
   c10::cuda::CUDAGuard guard(x.device());
   Tensor y = torch::empty_like(x);
   Tensor stats = torch::empty({2, s.frames, groups}, x.options().dtype(torch::kFloat32));
-  Tensor mean = stats.select(0, 0), rstd = stats.select(0, 1);
-  Tensor ws = workspace(
-      x, bysj_group_norm_forward_workspace_size(s.rows, s.channels, groups, s.frames));
+  float* mean = stats.data_ptr<float>();
+  const size_t bytes =
+      bysj_group_norm_forward_workspace_size(s.rows, s.channels, groups, s.frames);
+  Tensor ws;
+  if (bytes) ws = workspace(x, bytes);
   check(bysj_group_norm_forward(x.data_ptr(), dt, s.rows, s.channels, groups,
                                 opt_ptr<int64_t>(offsets), s.frames, s.inner,
                                 opt_ptr<float>(weight), opt_ptr<float>(bias),
                                 static_cast<float>(eps), static_cast<int>(activation),
-                                y.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(),
-                                ws.data_ptr(), static_cast<size_t>(ws.numel()), stream_of(x)),
+                                y.data_ptr(), mean, mean + s.frames * groups,
+                                bytes ? ws.data_ptr() : nullptr, bytes, stream_of(x)),
         "group_norm_forward");
-  return {y, mean, rstd};
+  return {y, stats};
 }
 
-std::tuple<Tensor, OptTensor, OptTensor> group_norm_backward(
-    Tensor grad_out, Tensor x, int64_t groups, OptTensor weight, OptTensor bias, Tensor mean,
-    Tensor rstd, int64_t activation, OptTensor offsets, bool want_weight, bool want_bias) {
+std::tuple<Tensor, Tensor, Tensor> group_norm_backward(
+    const Tensor& grad_out, const Tensor& x, int64_t groups, const OptTensor& weight,
+    const OptTensor& bias, const Tensor& stats, int64_t activation, const OptTensor& offsets,
+    bool want_weight, bool want_bias) {
   const int dt = value_dtype(x, "group norm input");
   TORCH_CHECK(value_dtype(grad_out, "group norm grad_out") == dt && grad_out.sizes() == x.sizes(),
               "group norm grad_out must match the input");
   const NormShape s = group_norm_shape(x, offsets, weight, bias);
-  f32(mean, "group norm mean");
-  f32(rstd, "group norm rstd");
-  TORCH_CHECK(mean.numel() == s.frames * groups && rstd.numel() == mean.numel(),
+  f32(stats, "group norm statistics");
+  TORCH_CHECK(stats.numel() == 2 * s.frames * groups,
               "group norm saved statistics have an invalid shape");
   c10::cuda::CUDAGuard guard(x.device());
-  Tensor gx = torch::empty_like(x);
-  OptTensor gw, gb;
-  if (want_weight) gw = torch::empty({s.channels}, mean.options());
-  if (want_bias) gb = torch::empty({s.channels}, mean.options());
-  Tensor ws = workspace(
-      x, bysj_group_norm_backward_workspace_size(s.rows, s.channels, groups, s.frames));
+  Tensor gx = torch::empty_like(x), gw, gb;
+  if (want_weight) gw = torch::empty({s.channels}, stats.options());
+  if (want_bias) gb = torch::empty({s.channels}, stats.options());
+  const float* mean = stats.data_ptr<float>();
+  const size_t bytes =
+      bysj_group_norm_backward_workspace_size(s.rows, s.channels, groups, s.frames);
+  Tensor ws;
+  if (bytes) ws = workspace(x, bytes);
   check(bysj_group_norm_backward(
             grad_out.data_ptr(), x.data_ptr(), dt, s.rows, s.channels, groups,
             opt_ptr<int64_t>(offsets), s.frames, s.inner, opt_ptr<float>(weight),
-            opt_ptr<float>(bias), mean.data_ptr<float>(), rstd.data_ptr<float>(),
-            static_cast<int>(activation), gx.data_ptr(), gw ? gw->data_ptr<float>() : nullptr,
-            gb ? gb->data_ptr<float>() : nullptr, ws.data_ptr(),
-            static_cast<size_t>(ws.numel()), stream_of(x)),
+            opt_ptr<float>(bias), mean, mean + s.frames * groups, static_cast<int>(activation),
+            gx.data_ptr(), want_weight ? gw.data_ptr<float>() : nullptr,
+            want_bias ? gb.data_ptr<float>() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
+            stream_of(x)),
         "group_norm_backward");
   return {gx, gw, gb};
 }
 
+class GroupNormFunction : public torch::autograd::Function<GroupNormFunction> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& weight,
+                        const OptTensor& bias, const OptTensor& offsets, int64_t groups,
+                        double eps, int64_t activation) {
+    auto [y, stats] = group_norm_forward(x, groups, weight, bias, eps, activation, offsets);
+    ctx->save_for_backward({x, weight.value_or(Tensor()), bias.value_or(Tensor()),
+                            offsets.value_or(Tensor()), stats});
+    ctx->saved_data["options"] = std::vector<int64_t>{
+        groups, activation, weight && weight->requires_grad(), bias && bias->requires_grad()};
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto o = ctx->saved_data["options"].toIntVector();
+    auto [gx, gw, gb] =
+        group_norm_backward(grads[0].contiguous(), saved[0], o[0], given(saved[1]),
+                            given(saved[2]), saved[4], o[1], given(saved[3]), o[2], o[3]);
+    return once({gx, gw, gb, Tensor(), Tensor(), Tensor(), Tensor()}, "group_norm");
+  }
+};
+
+Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight,
+                  const OptTensor& bias, double eps, int64_t activation,
+                  const OptTensor& offsets) {
+  if (!wants_grad({&x}, {&weight, &bias}))
+    return std::get<0>(group_norm_forward(x, groups, weight, bias, eps, activation, offsets));
+  return GroupNormFunction::apply(x, weight, bias, offsets, groups, eps, activation);
+}
+
 // ---- expert router ----------------------------------------------------------------
 
-// Returns weights, experts, counts, balance, z, and for the backward pass
-// z_scale, denom and share.
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> route_forward(
-    Tensor logits, int64_t k, OptTensor mask, OptTensor offsets, bool renormalize) {
+// weights, experts, counts, balance, z, and for the backward pass one buffer
+// of z_scale, denom [tokens] and share [frames, experts].
+struct Routed {
+  Tensor weights, experts, counts, balance, z, saved;
+};
+
+Routed route_forward(const Tensor& logits, int64_t k, const OptTensor& mask,
+                     const OptTensor& offsets, bool renormalize) {
   const int dt = value_dtype(logits, "router logits");
   TORCH_CHECK(logits.dim() == 2, "router logits must have shape (tokens, experts)");
   const int64_t tokens = logits.size(0), experts = logits.size(1);
@@ -988,57 +1109,87 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> route
   c10::cuda::CUDAGuard guard(logits.device());
   const auto f32o = logits.options().dtype(torch::kFloat32);
   const auto i64o = logits.options().dtype(torch::kInt64);
-  Tensor weights = torch::empty({tokens, k}, f32o), chosen = torch::empty({tokens, k}, i64o);
-  Tensor counts = offsets ? torch::empty({frames, experts}, i64o)
-                          : torch::empty({experts}, i64o);
-  Tensor balance = torch::empty({}, f32o), z = torch::empty({}, f32o);
-  Tensor z_scale = torch::empty({}, f32o), denom = torch::empty({tokens}, f32o);
-  Tensor share = torch::empty({frames, experts}, f32o);
+  Routed r;
+  r.weights = torch::empty({tokens, k}, f32o);
+  r.experts = torch::empty({tokens, k}, i64o);
+  r.counts = offsets ? torch::empty({frames, experts}, i64o) : torch::empty({experts}, i64o);
+  r.balance = torch::empty({}, f32o);
+  r.z = torch::empty({}, f32o);
+  r.saved = torch::empty({1 + tokens + frames * experts}, f32o);
   Tensor ws = workspace(logits, bysj_route_forward_workspace_size(tokens, experts, frames));
+  float* saved = r.saved.data_ptr<float>();
   check(bysj_route_forward(logits.data_ptr(), dt, tokens, experts, k,
                            mask ? reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>())
                                 : nullptr,
                            opt_ptr<int64_t>(offsets), frames, renormalize,
-                           weights.data_ptr<float>(), chosen.data_ptr<int64_t>(),
-                           counts.data_ptr<int64_t>(), balance.data_ptr<float>(),
-                           z.data_ptr<float>(), z_scale.data_ptr<float>(),
-                           denom.data_ptr<float>(), share.data_ptr<float>(), ws.data_ptr(),
-                           static_cast<size_t>(ws.numel()), stream_of(logits)),
+                           r.weights.data_ptr<float>(), r.experts.data_ptr<int64_t>(),
+                           r.counts.data_ptr<int64_t>(), r.balance.data_ptr<float>(),
+                           r.z.data_ptr<float>(), saved, saved + 1, saved + 1 + tokens,
+                           ws.data_ptr(), static_cast<size_t>(ws.numel()), stream_of(logits)),
         "route_forward");
-  return {weights, chosen, counts, balance, z, z_scale, denom, share};
+  return r;
 }
 
-Tensor route_backward(Tensor logits, int64_t k, OptTensor offsets, bool renormalize,
-                      Tensor weights, Tensor experts, Tensor denom, Tensor share, Tensor z_scale,
-                      OptTensor grad_weights, OptTensor grad_balance, OptTensor grad_z) {
+Tensor route_backward(const Tensor& logits, int64_t k, const OptTensor& offsets,
+                      bool renormalize, const Tensor& weights, const Tensor& experts,
+                      const Tensor& saved, const Tensor& grad_weights,
+                      const Tensor& grad_balance, const Tensor& grad_z) {
   const int dt = value_dtype(logits, "router logits");
   const int64_t tokens = logits.size(0), n_experts = logits.size(1);
-  f32(weights, "router weights");
-  i64(experts, "router experts");
-  f32(denom, "router denom");
-  f32(share, "router share");
-  f32(z_scale, "router z_scale");
-  TORCH_CHECK(weights.numel() == tokens * k && experts.numel() == tokens * k &&
-                  denom.numel() == tokens && z_scale.numel() == 1 &&
-                  share.numel() == (offsets ? offsets->numel() - 1 : 1) * n_experts,
+  const int64_t frames = offsets ? offsets->numel() - 1 : 1;
+  for (const Tensor* t : {&grad_weights, &grad_balance, &grad_z})
+    if (t->defined()) f32(*t, "router gradients");
+  TORCH_CHECK(saved.numel() == 1 + tokens + frames * n_experts &&
+                  (!grad_weights.defined() || grad_weights.numel() == tokens * k),
               "router saved tensors have an invalid shape");
-  if (grad_weights) {
-    f32(*grad_weights, "router grad_weights");
-    TORCH_CHECK(grad_weights->numel() == tokens * k, "router grad_weights must match the weights");
-  }
-  if (grad_balance) f32(*grad_balance, "router grad_balance");
-  if (grad_z) f32(*grad_z, "router grad_z");
   c10::cuda::CUDAGuard guard(logits.device());
   Tensor grad = torch::empty_like(logits);
+  const float* s = saved.data_ptr<float>();
+  const auto pointer = [](const Tensor& t) {
+    return t.defined() ? t.data_ptr<float>() : nullptr;
+  };
   check(bysj_route_backward(logits.data_ptr(), dt, tokens, n_experts, k,
-                            opt_ptr<int64_t>(offsets), share.numel() / n_experts, renormalize,
-                            weights.data_ptr<float>(), experts.data_ptr<int64_t>(),
-                            denom.data_ptr<float>(), share.data_ptr<float>(),
-                            z_scale.data_ptr<float>(), opt_ptr<float>(grad_weights),
-                            opt_ptr<float>(grad_balance), opt_ptr<float>(grad_z),
-                            grad.data_ptr(), stream_of(logits)),
+                            opt_ptr<int64_t>(offsets), frames, renormalize,
+                            weights.data_ptr<float>(), experts.data_ptr<int64_t>(), s + 1,
+                            s + 1 + tokens, s, pointer(grad_weights), pointer(grad_balance),
+                            pointer(grad_z), grad.data_ptr(), stream_of(logits)),
         "route_backward");
   return grad;
+}
+
+class RouteFunction : public torch::autograd::Function<RouteFunction> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& mask,
+                               const OptTensor& offsets, int64_t k, bool renormalize) {
+    const Routed r = route_forward(logits, k, mask, offsets, renormalize);
+    ctx->mark_non_differentiable({r.experts, r.counts});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward(
+        {logits, offsets.value_or(Tensor()), r.weights, r.experts, r.saved});
+    ctx->saved_data["k"] = k;
+    ctx->saved_data["renormalize"] = renormalize;
+    return {r.weights, r.experts, r.counts, r.balance, r.z};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor grad = route_backward(
+        s[0], ctx->saved_data["k"].toInt(), given(s[1]), ctx->saved_data["renormalize"].toBool(),
+        s[2], s[3], s[4], grads[0].defined() ? grads[0].contiguous() : Tensor(), grads[3],
+        grads[4]);
+    return once({grad, Tensor(), Tensor(), Tensor(), Tensor()}, "route_experts");
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_experts(const Tensor& logits, int64_t k,
+                                                                 const OptTensor& mask,
+                                                                 const OptTensor& offsets,
+                                                                 bool renormalize) {
+  if (!wants_grad({&logits}, {})) {
+    const Routed r = route_forward(logits, k, mask, offsets, renormalize);
+    return {r.weights, r.experts, r.counts, r.balance, r.z};
+  }
+  const variable_list v = RouteFunction::apply(logits, mask, offsets, k, renormalize);
+  return {v[0], v[1], v[2], v[3], v[4]};
 }
 
 // ---- AdamW ---------------------------------------------------------------------------
@@ -1186,21 +1337,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("dst_offsets"), py::arg("summed_partial"));
   m.def("group_by_key", &group_by_key, py::arg("keys"), py::arg("n_keys"));
   m.def("rotary_axes", &rotary_axes, py::arg("q"), py::arg("k"), py::arg("positions"),
-        py::arg("inv_freq"), py::arg("sections"), py::arg("interleaved") = false,
-        py::arg("inverse") = false, py::arg("saved_q") = py::none(),
-        py::arg("saved_k") = py::none());
-  m.def("group_norm_forward", &group_norm_forward, py::arg("x"), py::arg("groups"),
-        py::arg("weight"), py::arg("bias"), py::arg("eps"), py::arg("activation"),
-        py::arg("offsets"));
-  m.def("group_norm_backward", &group_norm_backward, py::arg("grad_out"), py::arg("x"),
-        py::arg("groups"), py::arg("weight"), py::arg("bias"), py::arg("mean"), py::arg("rstd"),
-        py::arg("activation"), py::arg("offsets"), py::arg("want_weight"), py::arg("want_bias"));
-  m.def("route_forward", &route_forward, py::arg("logits"), py::arg("k"), py::arg("mask"),
+        py::arg("inv_freq"), py::arg("sections"), py::arg("interleaved"));
+  m.def("group_norm", &group_norm, py::arg("x"), py::arg("groups"), py::arg("weight"),
+        py::arg("bias"), py::arg("eps"), py::arg("activation"), py::arg("offsets"));
+  m.def("route_experts", &route_experts, py::arg("logits"), py::arg("k"), py::arg("mask"),
         py::arg("offsets"), py::arg("renormalize"));
-  m.def("route_backward", &route_backward, py::arg("logits"), py::arg("k"), py::arg("offsets"),
-        py::arg("renormalize"), py::arg("weights"), py::arg("experts"), py::arg("denom"),
-        py::arg("share"), py::arg("z_scale"), py::arg("grad_weights"), py::arg("grad_balance"),
-        py::arg("grad_z"));
   m.def("adamw_step", &adamw_step);
   m.def("adamw_state_values", &adamw_state_values);
   m.def("library_version", []() { return bysj_version(); });

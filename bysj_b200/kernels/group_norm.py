@@ -11,7 +11,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import segment as _segment
 from .native import _extension, require_dcu
@@ -62,26 +61,6 @@ def _validate(x, groups, weight, bias, eps, activation, offsets):
     return eps
 
 
-class _GroupNormFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, groups, weight, bias, eps, activation, offsets):
-        y, mean, rstd = _extension("group_norm_forward").group_norm_forward(
-            x, groups, weight, bias, eps, activation, offsets)
-        ctx.save_for_backward(x, weight, bias, offsets, mean, rstd)
-        ctx.options = groups, activation
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output):
-        x, weight, bias, offsets, mean, rstd = ctx.saved_tensors
-        groups, activation = ctx.options
-        gx, gw, gb = _extension("group_norm_backward").group_norm_backward(
-            grad_output.contiguous(), x, groups, weight, bias, mean, rstd, activation, offsets,
-            ctx.needs_input_grad[2], ctx.needs_input_grad[3])
-        return (gx if ctx.needs_input_grad[0] else None, None, gw, gb, None, None, None)
-
-
 def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
                bias: torch.Tensor | None = None, eps: float = 1.0e-5, *,
                activation: str | None = None, offsets: torch.Tensor | None = None):
@@ -101,7 +80,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     require_dcu(x, weight, bias, offsets)
     if offsets is not None and _segment._should_check(None):
         _segment.check_indices(offsets, x.shape[0], name="group norm")
-    return _GroupNormFunction.apply(x, groups, weight, bias, eps, _ACTIVATIONS[activation], offsets)
+    return _extension("group_norm").group_norm(x, groups, weight, bias, eps,
+                                               _ACTIVATIONS[activation], offsets)
 
 
 __all__ = ["MAX_CHANNELS", "group_norm"]

@@ -12,7 +12,6 @@ from __future__ import annotations
 from typing import Sequence
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .native import _extension, require_dcu
 
@@ -66,32 +65,6 @@ def _validate(q, k, positions, inv_freq, sections) -> list[int]:
     return sections
 
 
-def _channels_last(grad: torch.Tensor) -> torch.Tensor:
-    return grad if grad.shape[2] <= 1 or grad.stride(2) == 1 else grad.contiguous()
-
-
-class _RotaryFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, sections, interleaved):
-        yq, yk, _ = _extension("rotary_axes").rotary_axes(q, k, positions, inv_freq, sections,
-                                                          interleaved)
-        ctx.position_grad = ctx.needs_input_grad[2]
-        kept = (q, k) if ctx.position_grad else ()
-        ctx.save_for_backward(positions, inv_freq, *kept)
-        ctx.options = sections, interleaved
-        return yq, yk
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_q, grad_k):
-        positions, inv_freq, *kept = ctx.saved_tensors
-        sections, interleaved = ctx.options
-        gq, gk, gp = _extension("rotary_axes").rotary_axes(
-            _channels_last(grad_q), _channels_last(grad_k), positions, inv_freq, sections,
-            interleaved, True, *kept)
-        return gq, gk, gp, None, None, None
-
-
 def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
                 inv_freq: torch.Tensor, sections: Sequence[int], *, interleaved: bool = False):
     """Turned ``(q, k)``, new contiguous tensors of the inputs' dtype.
@@ -109,7 +82,8 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     sections = _validate(q, k, positions, inv_freq, sections)
     require_dcu(q, k, positions, inv_freq)
     other = q.new_empty((q.shape[0], 0, q.shape[2])) if k is None else k
-    yq, yk = _RotaryFunction.apply(q, other, positions, inv_freq, sections, bool(interleaved))
+    yq, yk = _extension("rotary_axes").rotary_axes(q, other, positions, inv_freq, sections,
+                                                   bool(interleaved))
     return yq, (None if k is None else yk)
 
 

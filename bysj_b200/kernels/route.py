@@ -11,7 +11,6 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import segment as _segment
 from .native import _extension, require_dcu
@@ -61,30 +60,6 @@ def _validate(logits, k, mask, offsets):
         raise ValueError("all router inputs must share a device")
 
 
-class _RouteFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, k, mask, offsets, renormalize):
-        weights, experts, counts, balance, z, z_scale, denom, share = _extension(
-            "route_forward").route_forward(logits, k, mask, offsets, renormalize)
-        ctx.mark_non_differentiable(experts, counts)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, offsets, weights, experts, denom, share, z_scale)
-        ctx.options = k, renormalize
-        return weights, experts, counts, balance, z
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_weights, _experts, _counts, grad_balance, grad_z):
-        logits, offsets, weights, experts, denom, share, z_scale = ctx.saved_tensors
-        k, renormalize = ctx.options
-        if grad_weights is not None:
-            grad_weights = grad_weights.contiguous()
-        grad = _extension("route_backward").route_backward(
-            logits, k, offsets, renormalize, weights, experts, denom, share, z_scale,
-            grad_weights, grad_balance, grad_z)
-        return grad, None, None, None, None
-
-
 def route_experts(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = None,
                   offsets: torch.Tensor | None = None, renormalize: bool = False) -> Routing:
     """Route each token to its ``k`` largest logits; a :class:`Routing` tuple.
@@ -107,7 +82,8 @@ def route_experts(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = N
     require_dcu(logits, mask, offsets)
     if offsets is not None and _segment._should_check(None):
         _segment.check_indices(offsets, logits.shape[0], name="router")
-    return Routing(*_RouteFunction.apply(logits, k, mask, offsets, bool(renormalize)))
+    return Routing(*_extension("route_experts").route_experts(logits, k, mask, offsets,
+                                                              bool(renormalize)))
 
 
 __all__ = ["MAX_EXPERTS", "MAX_K", "Routing", "route_experts"]

@@ -526,6 +526,46 @@ def test_adamw_uses_parameter_gradients(cuda):
     assert p.grad is None
 
 
+# ---- autograd ---------------------------------------------------------------------------
+
+def test_gradients_are_differentiable_once(cuda):
+    gen = generator(23)
+    x = normal(gen, 40, 8).requires_grad_()
+    q = normal(gen, 5, 2, 8).requires_grad_()
+    pos, freq = torch.rand(5, 2, device="cuda"), torch.rand(4, device="cuda")
+    for out, leaf in ((K.group_norm(x, 2), x), (K.route_experts(x, 2).weights, x),
+                      (K.rotary_axes(q, q, pos, freq, (2, 2))[0], q)):
+        grad, = torch.autograd.grad((out * out).sum(), [leaf], create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            grad.sum().backward()
+
+
+def test_gradients_of_a_part_of_the_outputs(cuda):
+    gen = generator(29)
+    x = normal(gen, 40, 8).requires_grad_()
+    offsets = np.array([0, 40])
+    zero = np.zeros((40, 2))
+    for pick, grads in ((lambda r: r.balance, (zero, 1.0, 0.0)), (lambda r: r.z, (zero, 0.0, 1.0)),
+                        (lambda r: r.weights[:, 0].sum(), (zero + np.array([1.0, 0.0]), 0.0, 0.0))):
+        got, = torch.autograd.grad(pick(K.route_experts(x, 2)), [x])
+        want = O.route(f64(x), 2, None, offsets, False, grads)[5]
+        close(got, want, 4 * 17 * U * 15.0)
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    y = K.group_norm(x.detach()[None], 2, w)
+    got, = torch.autograd.grad(y.sum(), [w])
+    want = O.group_norm(f64(x), offsets, 2, f64(w), None, 1e-5, None, np.ones((40, 8)))[1][1]
+    close(got, want, 4 * np.sqrt(40) * 16 * U * 2 * 6.0 + 2 * U * np.abs(want))
+    q = normal(gen, 5, 2, 8)
+    pos = torch.rand(5, 2, device="cuda").requires_grad_()
+    freq = torch.rand(4, device="cuda")
+    yq, _ = K.rotary_axes(q, None, pos, freq, (2, 2))
+    got, = torch.autograd.grad(yq[..., ::2].sum(), [pos])
+    g = np.zeros((5, 2, 8))
+    g[..., ::2] = 1.0
+    want = O.rotary_position_grad([f64(q)], [g], f64(pos), f64(freq), (2, 2))
+    close(got, want, 16 * 16 * U * 16.0)
+
+
 # ---- streams and graphs ------------------------------------------------------------------
 
 def test_operators_run_on_the_current_stream(cuda):
