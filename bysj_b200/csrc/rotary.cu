@@ -8,8 +8,12 @@
 // forward input and gx the gradient just computed: neither y nor the angles
 // are kept between the passes.
 //
-// One warp per token; a lane takes pairs p = lane, lane + 32, ..., evaluates
-// sin and cos of its angle once and turns that pair of every head of q and k.
+// A CTA takes a few tokens at a time.  It evaluates sine and cosine of each
+// (token, pair) once into shared memory; then a thread holds the 8 (bfloat16)
+// or 4 (float32) pairs of one 16-byte vector in registers and turns them in
+// every HS-th head of q and k, two heads requested at a time.  Consecutive
+// threads take consecutive vectors, then consecutive heads, so a warp reads and
+// writes whole lines.  Bound by HBM: each value is read and written once.
 #include "launch.cuh"
 
 namespace bysj {
@@ -27,16 +31,9 @@ struct RotaryArgs {
   int interleaved;
   float sign;
   float* grad_positions;
+  // a CTA's tile: tokens and pairs, and threads side by side
+  int tile_tokens, tile_pairs, heads_abreast, vectors_abreast;
 };
-
-__device__ __forceinline__ float load_f32(const float* p) { return __ldg(p); }
-__device__ __forceinline__ float load_f32(const __nv_bfloat16* p) {
-  return __bfloat162float(*p);
-}
-__device__ __forceinline__ void store_value(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_value(__nv_bfloat16* p, float v) {
-  *p = __float2bfloat16_rn(v);
-}
 
 __device__ __forceinline__ int axis_of(const RotaryArgs& a, int p) {
   int axis = 0;
@@ -53,61 +50,243 @@ __device__ __forceinline__ float position_of(const RotaryArgs& a, int64_t t, int
   return __ldg(static_cast<const float*>(a.positions) + i);
 }
 
-template <typename T, bool POS_GRAD>
-__global__ void __launch_bounds__(kBlock) rotary_kernel(RotaryArgs a) {
-  const int lane = lane_id();
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
-  for (int64_t t = global_warp(); t < a.tokens; t += warps) {
-    float grad[BYSJ_ROTARY_MAX_AXES] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = lane; p < a.pairs; p += kWarp) {
-      const int axis = axis_of(a, p);
-      const float freq = __ldg(a.inv_freq + p);
-      float sine, cosine;
-      sincosf(position_of(a, t, axis) * freq, &sine, &cosine);
-      sine *= a.sign;
-      const int64_t c1 = a.interleaved ? 2 * p : p;
-      const int64_t c2 = a.interleaved ? 2 * p + 1 : p + a.pairs;
-      float dtheta = 0.0f;
-      for (int s = 0; s < 2; ++s) {
-        const bysj_rotary_side& side = a.side[s];
-        for (int64_t h = 0; h < side.heads; ++h) {
-          const T* x = static_cast<const T*>(side.x) + t * side.x_token_stride +
-                       h * side.x_head_stride;
-          T* y = static_cast<T*>(side.y) + (t * side.heads + h) * a.dim;
-          const float x1 = load_f32(x + c1), x2 = load_f32(x + c2);
-          const float y1 = x1 * cosine - x2 * sine, y2 = x2 * cosine + x1 * sine;
-          store_value(y + c1, y1);
-          store_value(y + c2, y2);
-          if constexpr (POS_GRAD) {
-            const T* v = static_cast<const T*>(side.saved) + t * side.saved_token_stride +
-                         h * side.saved_head_stride;
-            dtheta += y2 * load_f32(v + c1) - y1 * load_f32(v + c2);
+// The pairs that a thread turns in one head: VP pairs as loaded.
+template <typename T, int VP, bool INTERLEAVED>
+struct Pairs {
+  RowVec<T, VP> a, b;  // channels p .. and pairs + p .., or 2 p .. and on
+  __device__ __forceinline__ void load(const T* head, int p, int pairs) {
+    if constexpr (INTERLEAVED) {
+      a.load(head + 2 * p, 0);
+      b.load(head + 2 * p + VP, 0);
+    } else {
+      a.load(head + p, 0);
+      b.load(head + pairs + p, 0);
+    }
+  }
+  __device__ __forceinline__ float first(int i) const {
+    if constexpr (INTERLEAVED && VP > 1) return i < VP / 2 ? a.get(2 * i) : b.get(2 * i - VP);
+    else return a.get(i);
+  }
+  __device__ __forceinline__ float second(int i) const {
+    if constexpr (INTERLEAVED && VP > 1)
+      return i < VP / 2 ? a.get(2 * i + 1) : b.get(2 * i + 1 - VP);
+    else return b.get(i);
+  }
+};
+
+template <int VP>
+__device__ __forceinline__ void store_vec(float* p, const float (&v)[VP]) {
+  if constexpr (VP == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  else p[0] = v[0];
+}
+template <int VP>
+__device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&v)[VP]) {
+  if constexpr (VP == 8) {
+    __nv_bfloat162 h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+  } else {
+    p[0] = __float2bfloat16_rn(v[0]);
+  }
+}
+
+template <typename T, int VP, bool INTERLEAVED>
+__device__ __forceinline__ void store_pairs(T* head, int p, int pairs, const float (&y1)[VP],
+                                            const float (&y2)[VP]) {
+  if constexpr (!INTERLEAVED) {
+    store_vec<VP>(head + p, y1);
+    store_vec<VP>(head + pairs + p, y2);
+  } else if constexpr (VP == 1) {
+    store_vec<1>(head + 2 * p, y1);
+    store_vec<1>(head + 2 * p + 1, y2);
+  } else {
+    float v[VP];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int i = 0; i < VP / 2; ++i) {
+        v[2 * i] = y1[half * VP / 2 + i];
+        v[2 * i + 1] = y2[half * VP / 2 + i];
+      }
+      store_vec<VP>(head + 2 * p + half * VP, v);
+    }
+  }
+}
+
+// Shared memory: sine and cosine [2][tokens][tile pairs] (two tiles, so one
+// barrier each), and with a position gradient the threads' angle gradients
+// [tokens][heads side by side][tile pairs] and the axes' sums [tokens][4].
+template <typename T, int VP, bool INTERLEAVED, bool POS_GRAD>
+__global__ void __launch_bounds__(kBlock, POS_GRAD ? 3 : 4) rotary_kernel(RotaryArgs a) {
+  extern __shared__ __align__(16) float2 s_turn[];
+  const int tile_pairs = a.tile_pairs, tt = a.tile_tokens, hs = a.heads_abreast;
+  float* s_dtheta = reinterpret_cast<float*>(s_turn + 2 * tt * tile_pairs);
+  float* s_axis = s_dtheta + tt * hs * tile_pairs;
+  const int heads_q = static_cast<int>(a.side[0].heads);
+  const int heads = heads_q + static_cast<int>(a.side[1].heads);
+  // thread -> (token, first head, vector of pairs)
+  const int vectors = a.vectors_abreast;
+  const int vector = threadIdx.x % vectors, rest = threadIdx.x / vectors;
+  const int h0 = rest % hs, tok = rest / hs;
+  const int64_t token_tiles = (a.tokens + tt - 1) / tt;
+  int buffer = 0;
+  for (int64_t tile = blockIdx.x; tile < token_tiles; tile += gridDim.x) {
+    const int64_t t0 = tile * tt;
+    const int count = static_cast<int>(min(static_cast<int64_t>(tt), a.tokens - t0));
+    if constexpr (POS_GRAD) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < tt * BYSJ_ROTARY_MAX_AXES; i += kBlock) s_axis[i] = 0.0f;
+    }
+    for (int p0 = 0; p0 < a.pairs; p0 += tile_pairs) {
+      const int np = min(tile_pairs, a.pairs - p0);
+      float2* turn = s_turn + buffer * tt * tile_pairs;
+      buffer ^= 1;
+      for (int i = threadIdx.x; i < count * np; i += kBlock) {
+        const int t = i / np, p = i - t * np;
+        const float theta =
+            position_of(a, t0 + t, axis_of(a, p0 + p)) * __ldg(a.inv_freq + p0 + p);
+        float sine, cosine;
+        sincosf(theta, &sine, &cosine);
+        turn[t * tile_pairs + p] = make_float2(cosine, sine * a.sign);
+      }
+      __syncthreads();
+      if (tok < count) {
+        const int64_t t = t0 + tok;
+        for (int v = vector; v * VP < np; v += vectors) {
+          const int pl = v * VP, p = p0 + pl;
+          float cosine[VP], sine[VP], dtheta[VP];
+#pragma unroll
+          for (int i = 0; i < VP; ++i) {
+            const float2 q = turn[tok * tile_pairs + pl + i];
+            cosine[i] = q.x;
+            sine[i] = q.y;
+            dtheta[i] = 0.0f;
           }
+          auto head_of = [&](int h, const T*& x, T*& y, const T*& saved) {
+            const bool k = h >= heads_q;
+            const bysj_rotary_side& side = a.side[k ? 1 : 0];
+            const int64_t at = k ? h - heads_q : h;
+            x = static_cast<const T*>(side.x) + t * side.x_token_stride + at * side.x_head_stride;
+            y = static_cast<T*>(side.y) + (t * side.heads + at) * a.dim;
+            if constexpr (POS_GRAD)
+              saved = static_cast<const T*>(side.saved) + t * side.saved_token_stride +
+                      at * side.saved_head_stride;
+          };
+          using PairsT = Pairs<T, VP, INTERLEAVED>;
+          auto finish = [&](const PairsT& x, const PairsT& saved, T* y) {
+            float y1[VP], y2[VP];
+#pragma unroll
+            for (int i = 0; i < VP; ++i) {
+              const float x1 = x.first(i), x2 = x.second(i);
+              y1[i] = x1 * cosine[i] - x2 * sine[i];
+              y2[i] = x2 * cosine[i] + x1 * sine[i];
+              if constexpr (POS_GRAD)
+                dtheta[i] += y2[i] * saved.first(i) - y1[i] * saved.second(i);
+            }
+            store_pairs<T, VP, INTERLEAVED>(y, p, a.pairs, y1, y2);
+          };
+          for (int h = h0; h < heads; h += 2 * hs) {
+            const T *x0, *x1 = nullptr, *s0 = nullptr, *s1 = nullptr;
+            T *y0, *y1 = nullptr;
+            PairsT a0, a1, b0, b1;
+            const bool two = h + hs < heads;
+            head_of(h, x0, y0, s0);
+            a0.load(x0, p, a.pairs);
+            if constexpr (POS_GRAD) b0.load(s0, p, a.pairs);
+            if (two) {
+              head_of(h + hs, x1, y1, s1);
+              a1.load(x1, p, a.pairs);
+              if constexpr (POS_GRAD) b1.load(s1, p, a.pairs);
+            }
+            finish(a0, b0, y0);
+            if (two) finish(a1, b1, y1);
+          }
+          if constexpr (POS_GRAD)
+#pragma unroll
+            for (int i = 0; i < VP; ++i)
+              s_dtheta[(tok * hs + h0) * tile_pairs + pl + i] = dtheta[i];
         }
       }
       if constexpr (POS_GRAD) {
+        __syncthreads();
+        // a warp joins a token's heads and pairs, in their order
+        for (int t = threadIdx.x / kWarp; t < count; t += kWarpsPerBlock) {
+          float sums[BYSJ_ROTARY_MAX_AXES] = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int p = lane_id(); p < np; p += kWarp) {
+            float d = 0.0f;
+            for (int h = 0; h < hs; ++h) d += s_dtheta[(t * hs + h) * tile_pairs + p];
+            d *= __ldg(a.inv_freq + p0 + p);
+            const int axis = axis_of(a, p0 + p);
 #pragma unroll
-        for (int i = 0; i < BYSJ_ROTARY_MAX_AXES; ++i)
-          if (i == axis) grad[i] += freq * dtheta;
-      }
-    }
-    for (int s = 0; s < 2; ++s) {
-      const bysj_rotary_side& side = a.side[s];
-      for (int64_t h = 0; h < side.heads; ++h) {
-        const T* x = static_cast<const T*>(side.x) + t * side.x_token_stride +
-                     h * side.x_head_stride;
-        T* y = static_cast<T*>(side.y) + (t * side.heads + h) * a.dim;
-        for (int64_t c = 2 * a.pairs + lane; c < a.dim; c += kWarp) y[c] = x[c];
+            for (int i = 0; i < BYSJ_ROTARY_MAX_AXES; ++i)
+              if (i == axis) sums[i] += d;
+          }
+#pragma unroll
+          for (int i = 0; i < BYSJ_ROTARY_MAX_AXES; ++i) {
+            const float total = xor_sum(sums[i], 1);
+            if (lane_id() == 0) s_axis[t * BYSJ_ROTARY_MAX_AXES + i] += total;
+          }
+        }
+        __syncthreads();
       }
     }
     if constexpr (POS_GRAD) {
-#pragma unroll
-      for (int i = 0; i < BYSJ_ROTARY_MAX_AXES; ++i) {
-        const float total = xor_sum(grad[i], 1);
-        if (lane == 0 && i < a.axes) a.grad_positions[t * a.axes + i] = total;
+      __syncthreads();
+      for (int i = threadIdx.x; i < count * a.axes; i += kBlock) {
+        const int t = i / a.axes, axis = i - t * a.axes;
+        a.grad_positions[(t0 + t) * a.axes + axis] = s_axis[t * BYSJ_ROTARY_MAX_AXES + axis];
       }
     }
+    // channels without an angle
+    const int tail = static_cast<int>(a.dim) - 2 * a.pairs;
+    if (tail > 0)
+      for (int64_t i = threadIdx.x; i < static_cast<int64_t>(count) * heads * tail; i += kBlock) {
+        const int c = 2 * a.pairs + static_cast<int>(i % tail);
+        const int h = static_cast<int>(i / tail % heads);
+        const int64_t t = t0 + i / tail / heads;
+        const bysj_rotary_side& side = a.side[h >= heads_q ? 1 : 0];
+        const int64_t at = h >= heads_q ? h - heads_q : h;
+        static_cast<T*>(side.y)[(t * side.heads + at) * a.dim + c] =
+            static_cast<const T*>(side.x)[t * side.x_token_stride + at * side.x_head_stride + c];
+      }
   }
+}
+
+using RotaryKernel = void (*)(RotaryArgs);
+
+template <typename T, int VP>
+RotaryKernel rotary_pick(bool interleaved, bool pos_grad) {
+  if (interleaved)
+    return pos_grad ? rotary_kernel<T, VP, true, true> : rotary_kernel<T, VP, true, false>;
+  return pos_grad ? rotary_kernel<T, VP, false, true> : rotary_kernel<T, VP, false, false>;
+}
+
+// Whole 16-byte vectors of every head are aligned.
+bool side_aligned(const bysj_rotary_side& side, int64_t dim, int64_t vec, bool saved) {
+  if (side.heads == 0) return true;
+  bool ok = aligned16(side.x) && aligned16(side.y) && dim % vec == 0 &&
+            side.x_token_stride % vec == 0 && side.x_head_stride % vec == 0;
+  if (saved)
+    ok = ok && aligned16(side.saved) && side.saved_token_stride % vec == 0 &&
+         side.saved_head_stride % vec == 0;
+  return ok;
+}
+
+// Tiles: up to 256 pairs; threads over the vectors of a tile, then over as many
+// heads as make 64 threads or so (lines of several heads in one request), then
+// over tokens.
+size_t plan_tiles(RotaryArgs& a, int vp, bool pos_grad) {
+  const int heads = static_cast<int>(a.side[0].heads + a.side[1].heads);
+  a.tile_pairs = a.pairs < 1 ? 1 : a.pairs < 256 ? a.pairs : 256;
+  a.vectors_abreast = (a.tile_pairs + vp - 1) / vp;
+  const int want = 64 / a.vectors_abreast < 1 ? 1 : 64 / a.vectors_abreast;
+  a.heads_abreast = heads < want ? heads : want;
+  a.tile_tokens = kBlock / (a.vectors_abreast * a.heads_abreast);
+  const size_t turn = sizeof(float2) * 2 * a.tile_tokens * a.tile_pairs;
+  if (!pos_grad) return turn;
+  return turn + sizeof(float) * a.tile_tokens *
+                    (a.heads_abreast * a.tile_pairs + BYSJ_ROTARY_MAX_AXES);
 }
 
 }  // namespace
@@ -123,8 +302,8 @@ extern "C" int bysj_rotary_axes(const bysj_rotary_side* q, const bysj_rotary_sid
   clear_error();
   if (dtype != BYSJ_F32 && dtype != BYSJ_BF16)
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "rotary: unknown dtype %d", dtype);
-  if (tokens < 0 || dim <= 0 || dim > (int64_t{1} << 30) || q == nullptr || k == nullptr ||
-      q->heads < 0 || k->heads < 0)
+  if (tokens < 0 || dim <= 0 || dim > (int64_t{1} << 20) || q == nullptr || k == nullptr ||
+      q->heads < 0 || k->heads < 0 || q->heads + k->heads > (int64_t{1} << 20))
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "rotary: invalid sizes");
   if (axes < 1 || axes > BYSJ_ROTARY_MAX_AXES || sections == nullptr)
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "rotary: 1 to %d axes", BYSJ_ROTARY_MAX_AXES);
@@ -169,14 +348,22 @@ extern "C" int bysj_rotary_axes(const bysj_rotary_side* q, const bysj_rotary_sid
   a.sign = inverse ? -1.0f : 1.0f;
   a.grad_positions = grad_positions;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int64_t blocks = (tokens + kWarpsPerBlock - 1) / kWarpsPerBlock;
-  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 16;
+  const int64_t vec = dtype == BYSJ_F32 ? 4 : 8;
+  const bool pos_grad = grad_positions != nullptr;
+  const bool vectors = pairs > 0 && pairs % vec == 0 && side_aligned(*q, dim, vec, pos_grad) &&
+                       side_aligned(*k, dim, vec, pos_grad);
+  const size_t smem = plan_tiles(a, vectors ? static_cast<int>(vec) : 1, pos_grad);
+  const RotaryKernel kernel =
+      dtype == BYSJ_F32 ? (vectors ? rotary_pick<float, 4>(interleaved, pos_grad)
+                                   : rotary_pick<float, 1>(interleaved, pos_grad))
+                        : (vectors ? rotary_pick<__nv_bfloat16, 8>(interleaved, pos_grad)
+                                   : rotary_pick<__nv_bfloat16, 1>(interleaved, pos_grad));
+  const int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (st) return st;
+  int64_t blocks = (tokens + a.tile_tokens - 1) / a.tile_tokens;
+  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) *
+                      resident_blocks(reinterpret_cast<const void*>(kernel), smem);
   if (blocks > cap) blocks = cap;
-  const auto kernel = dtype == BYSJ_F32
-                          ? (grad_positions ? rotary_kernel<float, true>
-                                            : rotary_kernel<float, false>)
-                          : (grad_positions ? rotary_kernel<__nv_bfloat16, true>
-                                            : rotary_kernel<__nv_bfloat16, false>);
-  kernel<<<static_cast<unsigned>(blocks), kBlock, 0, s>>>(a);
+  kernel<<<static_cast<unsigned>(blocks), kBlock, smem, s>>>(a);
   return launch_check("rotary_kernel");
 }
