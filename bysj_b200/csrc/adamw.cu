@@ -6,9 +6,12 @@
 // Work is counted in blocks of 256 elements, the unit that shares one scale
 // of an 8-bit state.  The tensor table travels in the kernel's parameters
 // (no copy to the device); a warp finds the tensor of its block by a binary
-// search and takes 8 elements per lane.  Every tensor's states begin at a
-// block boundary of the shared state buffers, so the table holds no state
-// pointers and their loads are always aligned.
+// search and takes 8 elements per lane, four side by side twice, so that each
+// array is read and written in whole lines (16 bytes a lane of float32, 8 of
+// bfloat16, 4 of codes).  Every tensor's states begin at a block boundary of
+// the shared state buffers, so the table holds no state pointers and their
+// loads are always aligned; a parameter or gradient that is not, and a tensor's
+// last block, goes element by element.
 //
 // Each product and sum is rounded to fp32 on its own (no fused
 // multiply-add), so a step gives the same bits as the formula evaluated one
@@ -59,7 +62,7 @@ struct AdamArgs {
 constexpr int kSmallTable = 96;
 constexpr int kLargeTable = 800;
 
-__device__ __forceinline__ float load_f32(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float load_f32(const float* p) { return *p; }
 __device__ __forceinline__ float load_f32(const __nv_bfloat16* p) {
   return __bfloat162float(*p);
 }
@@ -68,10 +71,39 @@ __device__ __forceinline__ void store_value(__nv_bfloat16* p, float v) {
   *p = __float2bfloat16_rn(v);
 }
 
+// The i-th of a lane's elements in its block.
+__device__ __forceinline__ int element(int lane, int i) {
+  return lane * 4 + i / 4 * 4 * kWarp + i % 4;
+}
+__device__ __forceinline__ void load4(const float* p, float* v) {
+  const float4 q = *reinterpret_cast<const float4*>(p);
+  v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, float* v) {
+  const uint2 q = *reinterpret_cast<const uint2*>(p);
+  v[0] = bf16_lo(q.x); v[1] = bf16_hi(q.x); v[2] = bf16_lo(q.y); v[3] = bf16_hi(q.y);
+}
+__device__ __forceinline__ void store4(float* p, const float* v) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* v) {
+  __nv_bfloat162 h[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+  *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(h);
+}
+
 template <int TOP, int MANT>
 __device__ __forceinline__ float code_value(int code) {
   const float v = __int_as_float((code - TOP + (127 << MANT)) << (23 - MANT));
   return code > 0 ? v : 0.0f;
+}
+
+__device__ __forceinline__ float value_m(int code, float scale) {
+  const float size = __fmul_rn(code_value<kTopM, kMantM>(code & 127), scale);
+  return code & 128 ? -size : size;
+}
+__device__ __forceinline__ float value_v(int code, float scale) {
+  const float root = __fmul_rn(code_value<kTopV, kMantV>(code), scale);
+  return __fmul_rn(root, root);
 }
 
 // Code of ratio in [0, 1]: the bits of the float rounded to MANT mantissa
@@ -113,7 +145,7 @@ __device__ __forceinline__ int encode_v(float root, float inv) {
 }
 
 template <typename T, int BITS, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kBlock)
+__global__ void __launch_bounds__(kBlock, 4)
     adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
   const int lane = lane_id();
   const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
@@ -134,23 +166,45 @@ __global__ void __launch_bounds__(kBlock)
     const T* grad = static_cast<const T*>(a.entry[lo].grad) + begin;
     const int64_t state = block * kStateBlock;
     float p[kPerLane], g[kPerLane], m[kPerLane], v[kPerLane];
+    const bool whole = left >= kStateBlock &&
+                       ((reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) &
+                        (4 * sizeof(T) - 1)) == 0;
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int j = lane + i * kWarp;
-      const bool in = j < left;
-      g[i] = in ? load_f32(grad + j) : 0.0f;
-      if constexpr (MASTER) p[i] = a.master[state + j];
-      else p[i] = in ? load_f32(param + j) : 0.0f;
+      for (int i = 0; i < kPerLane; i += 4) {
+        load4(grad + element(lane, i), g + i);
+        if constexpr (!MASTER) load4(param + element(lane, i), p + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        const int j = element(lane, i);
+        g[i] = j < left ? load_f32(grad + j) : 0.0f;
+        if constexpr (!MASTER) p[i] = j < left ? load_f32(param + j) : 0.0f;
+      }
+    }
+    float scale_m = 0.0f, scale_v = 0.0f;
+    if constexpr (BITS == 8) {
+      scale_m = a.exp_avg_scale[block];
+      scale_v = a.exp_avg_sq_scale[block];
+    }
+#pragma unroll
+    for (int i = 0; i < kPerLane; i += 4) {
+      const int64_t at = state + element(lane, i);
+      if constexpr (MASTER) load4(a.master + at, p + i);
       if constexpr (BITS == 32) {
-        m[i] = static_cast<const float*>(a.exp_avg)[state + j];
-        v[i] = static_cast<const float*>(a.exp_avg_sq)[state + j];
+        load4(static_cast<const float*>(a.exp_avg) + at, m + i);
+        load4(static_cast<const float*>(a.exp_avg_sq) + at, v + i);
       } else {
-        const int cm = static_cast<const uint8_t*>(a.exp_avg)[state + j];
-        const int cv = static_cast<const uint8_t*>(a.exp_avg_sq)[state + j];
-        const float size = __fmul_rn(code_value<kTopM, kMantM>(cm & 127), a.exp_avg_scale[block]);
-        const float root = __fmul_rn(code_value<kTopV, kMantV>(cv), a.exp_avg_sq_scale[block]);
-        m[i] = cm & 128 ? -size : size;
-        v[i] = __fmul_rn(root, root);
+        const uchar4 cm = *reinterpret_cast<const uchar4*>(static_cast<uint8_t*>(a.exp_avg) + at);
+        const uchar4 cv =
+            *reinterpret_cast<const uchar4*>(static_cast<uint8_t*>(a.exp_avg_sq) + at);
+        const int codes_m[4] = {cm.x, cm.y, cm.z, cm.w}, codes_v[4] = {cv.x, cv.y, cv.z, cv.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          m[i + j] = value_m(codes_m[j], scale_m);
+          v[i + j] = value_v(codes_v[j], scale_v);
+        }
       }
     }
     float root[kPerLane];
@@ -164,30 +218,42 @@ __global__ void __launch_bounds__(kBlock)
       const float den = __fadd_rn(__fmul_rn(root[i], a.h.correct), a.h.eps);
       p[i] = __fsub_rn(__fmul_rn(p[i], a.h.decay), __fmul_rn(__fdiv_rn(m[i], den), a.h.size));
     }
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int j = lane + i * kWarp;
-      if (j < left) {
-        store_value(param + j, p[i]);
-        if constexpr (MASTER) a.master[state + j] = p[i];
+      for (int i = 0; i < kPerLane; i += 4) {
+        store4(param + element(lane, i), p + i);
+        if constexpr (MASTER) store4(a.master + state + element(lane, i), p + i);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        const int j = element(lane, i);
+        if (j < left) {
+          store_value(param + j, p[i]);
+          if constexpr (MASTER) a.master[state + j] = p[i];
+        }
       }
     }
     if constexpr (BITS == 32) {
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        const int j = lane + i * kWarp;
-        static_cast<float*>(a.exp_avg)[state + j] = m[i];
-        static_cast<float*>(a.exp_avg_sq)[state + j] = v[i];
+      for (int i = 0; i < kPerLane; i += 4) {
+        store4(static_cast<float*>(a.exp_avg) + state + element(lane, i), m + i);
+        store4(static_cast<float*>(a.exp_avg_sq) + state + element(lane, i), v + i);
       }
     } else {
       const float sm = block_max(m), sv = block_max(root);
       const float im = inverse_scale(sm), iv = inverse_scale(sv);
 #pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        const int j = lane + i * kWarp;
-        static_cast<uint8_t*>(a.exp_avg)[state + j] = static_cast<uint8_t>(encode_m(m[i], im));
-        static_cast<uint8_t*>(a.exp_avg_sq)[state + j] =
-            static_cast<uint8_t>(encode_v(root[i], iv));
+      for (int i = 0; i < kPerLane; i += 4) {
+        unsigned codes_m = 0, codes_v = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          codes_m |= static_cast<unsigned>(encode_m(m[i + j], im)) << (8 * j);
+          codes_v |= static_cast<unsigned>(encode_v(root[i + j], iv)) << (8 * j);
+        }
+        const int64_t at = state + element(lane, i);
+        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.exp_avg) + at) = codes_m;
+        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.exp_avg_sq) + at) = codes_v;
       }
       if (lane == 0) {
         a.exp_avg_scale[block] = sm;
@@ -197,17 +263,38 @@ __global__ void __launch_bounds__(kBlock)
   }
 }
 
+// Four elements a lane, four times in steps of the grid.
 __global__ void __launch_bounds__(kBlock)
     adamw_values_kernel(const uint8_t* exp_avg, const uint8_t* exp_avg_sq, const float* scale_m,
-                        const float* scale_v, int64_t count, float* out_m, float* out_v) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < count;
-       i += step) {
-    const int cm = exp_avg[i], cv = exp_avg_sq[i];
-    const float size = __fmul_rn(code_value<kTopM, kMantM>(cm & 127), scale_m[i / kStateBlock]);
-    const float root = __fmul_rn(code_value<kTopV, kMantV>(cv), scale_v[i / kStateBlock]);
-    out_m[i] = cm & 128 ? -size : size;
-    out_v[i] = __fmul_rn(root, root);
+                        const float* scale_v, int64_t quads, float* out_m, float* out_v) {
+  constexpr int kQuadsBlock = kStateBlock / 4, kUnroll = 4;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kBlock;
+  for (int64_t q0 = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; q0 < quads;
+       q0 += step * kUnroll) {
+    unsigned cm[kUnroll], cv[kUnroll];
+    float sm[kUnroll], sv[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t q = q0 + u * step;
+      if (q >= quads) continue;
+      cm[u] = reinterpret_cast<const unsigned*>(exp_avg)[q];
+      cv[u] = reinterpret_cast<const unsigned*>(exp_avg_sq)[q];
+      sm[u] = __ldg(scale_m + q / kQuadsBlock);
+      sv[u] = __ldg(scale_v + q / kQuadsBlock);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t q = q0 + u * step;
+      if (q >= quads) continue;
+      float m[4], v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m[j] = value_m((cm[u] >> (8 * j)) & 255, sm[u]);
+        v[j] = value_v((cv[u] >> (8 * j)) & 255, sv[u]);
+      }
+      store4(out_m + 4 * q, m);
+      store4(out_v + 4 * q, v);
+    }
   }
 }
 
@@ -325,13 +412,13 @@ int bysj_adamw_state_values(const uint8_t* exp_avg, const uint8_t* exp_avg_sq,
   if (exp_avg == nullptr || exp_avg_sq == nullptr || exp_avg_scale == nullptr ||
       exp_avg_sq_scale == nullptr || exp_avg_values == nullptr || exp_avg_sq_values == nullptr)
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw values: NULL pointer");
-  const int64_t count = blocks * kStateBlock;
-  int64_t grid = (count + kBlock - 1) / kBlock;
-  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 16;
+  const int64_t quads = blocks * (kStateBlock / 4);
+  int64_t grid = (quads + kBlock - 1) / kBlock;
+  const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 8;
   if (grid > cap) grid = cap;
   adamw_values_kernel<<<static_cast<unsigned>(grid), kBlock, 0,
                         static_cast<cudaStream_t>(stream)>>>(
-      exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, count, exp_avg_values,
+      exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, quads, exp_avg_values,
       exp_avg_sq_values);
   return launch_check("adamw_values_kernel");
 }

@@ -11,7 +11,7 @@
 // A CTA takes a few tokens at a time.  It evaluates sine and cosine of each
 // (token, pair) once into shared memory; then a thread holds the 8 (bfloat16)
 // or 4 (float32) pairs of one 16-byte vector in registers and turns them in
-// every HS-th head of q and k, two heads requested at a time.  Consecutive
+// every HS-th head of q and k, four heads requested at a time.  Consecutive
 // threads take consecutive vectors, then consecutive heads, so a warp reads and
 // writes whole lines.  Bound by HBM: each value is read and written once.
 #include "launch.cuh"
@@ -118,7 +118,7 @@ __device__ __forceinline__ void store_pairs(T* head, int p, int pairs, const flo
 // barrier each), and with a position gradient the threads' angle gradients
 // [tokens][heads side by side][tile pairs] and the axes' sums [tokens][4].
 template <typename T, int VP, bool INTERLEAVED, bool POS_GRAD>
-__global__ void __launch_bounds__(kBlock, POS_GRAD ? 3 : 4) rotary_kernel(RotaryArgs a) {
+__global__ void __launch_bounds__(kBlock, 3) rotary_kernel(RotaryArgs a) {
   extern __shared__ __align__(16) float2 s_turn[];
   const int tile_pairs = a.tile_pairs, tt = a.tile_tokens, hs = a.heads_abreast;
   float* s_dtheta = reinterpret_cast<float*>(s_turn + 2 * tt * tile_pairs);
@@ -153,6 +153,16 @@ __global__ void __launch_bounds__(kBlock, POS_GRAD ? 3 : 4) rotary_kernel(Rotary
       __syncthreads();
       if (tok < count) {
         const int64_t t = t0 + tok;
+        const int64_t stride_q = a.side[0].x_head_stride, stride_k = a.side[1].x_head_stride;
+        const T* xq = static_cast<const T*>(a.side[0].x) + t * a.side[0].x_token_stride;
+        const T* xk = static_cast<const T*>(a.side[1].x) + t * a.side[1].x_token_stride;
+        T* yq = static_cast<T*>(a.side[0].y) + t * heads_q * a.dim;
+        T* yk = static_cast<T*>(a.side[1].y) + t * (heads - heads_q) * a.dim;
+        const T *sq = nullptr, *sk = nullptr;
+        if constexpr (POS_GRAD) {
+          sq = static_cast<const T*>(a.side[0].saved) + t * a.side[0].saved_token_stride;
+          sk = static_cast<const T*>(a.side[1].saved) + t * a.side[1].saved_token_stride;
+        }
         for (int v = vector; v * VP < np; v += vectors) {
           const int pl = v * VP, p = p0 + pl;
           float cosine[VP], sine[VP], dtheta[VP];
@@ -163,16 +173,6 @@ __global__ void __launch_bounds__(kBlock, POS_GRAD ? 3 : 4) rotary_kernel(Rotary
             sine[i] = q.y;
             dtheta[i] = 0.0f;
           }
-          auto head_of = [&](int h, const T*& x, T*& y, const T*& saved) {
-            const bool k = h >= heads_q;
-            const bysj_rotary_side& side = a.side[k ? 1 : 0];
-            const int64_t at = k ? h - heads_q : h;
-            x = static_cast<const T*>(side.x) + t * side.x_token_stride + at * side.x_head_stride;
-            y = static_cast<T*>(side.y) + (t * side.heads + at) * a.dim;
-            if constexpr (POS_GRAD)
-              saved = static_cast<const T*>(side.saved) + t * side.saved_token_stride +
-                      at * side.saved_head_stride;
-          };
           using PairsT = Pairs<T, VP, INTERLEAVED>;
           auto finish = [&](const PairsT& x, const PairsT& saved, T* y) {
             float y1[VP], y2[VP];
@@ -186,21 +186,27 @@ __global__ void __launch_bounds__(kBlock, POS_GRAD ? 3 : 4) rotary_kernel(Rotary
             }
             store_pairs<T, VP, INTERLEAVED>(y, p, a.pairs, y1, y2);
           };
-          for (int h = h0; h < heads; h += 2 * hs) {
-            const T *x0, *x1 = nullptr, *s0 = nullptr, *s1 = nullptr;
-            T *y0, *y1 = nullptr;
-            PairsT a0, a1, b0, b1;
-            const bool two = h + hs < heads;
-            head_of(h, x0, y0, s0);
-            a0.load(x0, p, a.pairs);
-            if constexpr (POS_GRAD) b0.load(s0, p, a.pairs);
-            if (two) {
-              head_of(h + hs, x1, y1, s1);
-              a1.load(x1, p, a.pairs);
-              if constexpr (POS_GRAD) b1.load(s1, p, a.pairs);
+          // kAhead heads are requested before the first is turned
+          constexpr int kAhead = POS_GRAD ? 2 : 4;
+          for (int h = h0; h < heads; h += kAhead * hs) {
+            PairsT x[kAhead], saved[POS_GRAD ? kAhead : 1];
+            T* y[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+              const int head = h + j * hs;
+              if (head >= heads) continue;
+              const bool k = head >= heads_q;
+              const int at = k ? head - heads_q : head;
+              x[j].load((k ? xk : xq) + at * (k ? stride_k : stride_q), p, a.pairs);
+              y[j] = (k ? yk : yq) + at * a.dim;
+              if constexpr (POS_GRAD)
+                saved[j].load((k ? sk : sq) + at * (k ? a.side[1].saved_head_stride
+                                                      : a.side[0].saved_head_stride),
+                              p, a.pairs);
             }
-            finish(a0, b0, y0);
-            if (two) finish(a1, b1, y1);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+              if (h + j * hs < heads) finish(x[j], saved[POS_GRAD ? j : 0], y[j]);
           }
           if constexpr (POS_GRAD)
 #pragma unroll
@@ -273,16 +279,25 @@ bool side_aligned(const bysj_rotary_side& side, int64_t dim, int64_t vec, bool s
   return ok;
 }
 
-// Tiles: up to 256 pairs; threads over the vectors of a tile, then over as many
-// heads as make 64 threads or so (lines of several heads in one request), then
-// over tokens.
+// Tiles: up to 256 pairs; threads over the vectors of a tile, then over heads
+// (up to 64 threads, so that a request covers lines of several heads), then over
+// tokens.  Of the numbers of heads side by side the one that leaves the fewest
+// threads without work.
 size_t plan_tiles(RotaryArgs& a, int vp, bool pos_grad) {
   const int heads = static_cast<int>(a.side[0].heads + a.side[1].heads);
   a.tile_pairs = a.pairs < 1 ? 1 : a.pairs < 256 ? a.pairs : 256;
   a.vectors_abreast = (a.tile_pairs + vp - 1) / vp;
   const int want = 64 / a.vectors_abreast < 1 ? 1 : 64 / a.vectors_abreast;
-  a.heads_abreast = heads < want ? heads : want;
-  a.tile_tokens = kBlock / (a.vectors_abreast * a.heads_abreast);
+  double best = 0.0;
+  for (int hs = heads < want ? heads : want; hs >= 1; --hs) {
+    const int tokens = kBlock / (a.vectors_abreast * hs), rounds = (heads + hs - 1) / hs;
+    const double busy = static_cast<double>(tokens) * a.vectors_abreast * heads / rounds;
+    if (busy > best * 1.01) {
+      best = busy;
+      a.heads_abreast = hs;
+      a.tile_tokens = tokens;
+    }
+  }
   const size_t turn = sizeof(float2) * 2 * a.tile_tokens * a.tile_pairs;
   if (!pos_grad) return turn;
   return turn + sizeof(float) * a.tile_tokens *
