@@ -91,29 +91,40 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float* v) {
   *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(h);
 }
 
+// Byte j of a word moved to the bits above 23 - MANT of a float, cut by `mask`.
+template <int MANT>
+__device__ __forceinline__ unsigned byte_bits(unsigned word, int j, unsigned mask) {
+  const int up = 23 - MANT - 8 * j;
+  return (up >= 0 ? word << up : word >> -up) & mask;
+}
 template <int TOP, int MANT>
-__device__ __forceinline__ float code_value(int code) {
-  const float v = __int_as_float((code - TOP + (127 << MANT)) << (23 - MANT));
-  return code > 0 ? v : 0.0f;
+__device__ __forceinline__ float code_value(unsigned bits) {
+  const float v = __uint_as_float(bits + (((127u << MANT) - TOP) << (23 - MANT)));
+  return bits != 0 ? v : 0.0f;
 }
 
-__device__ __forceinline__ float value_m(int code, float scale) {
-  const float size = __fmul_rn(code_value<kTopM, kMantM>(code & 127), scale);
-  return code & 128 ? -size : size;
+// What byte j of a word of codes stands for.
+__device__ __forceinline__ float value_m(unsigned word, int j, float scale) {
+  const float size = __fmul_rn(
+      code_value<kTopM, kMantM>(byte_bits<kMantM>(word, j, 127u << (23 - kMantM))), scale);
+  const unsigned sign = (word << (24 - 8 * j)) & 0x80000000u;
+  return __uint_as_float(__float_as_uint(size) | sign);
 }
-__device__ __forceinline__ float value_v(int code, float scale) {
-  const float root = __fmul_rn(code_value<kTopV, kMantV>(code), scale);
+__device__ __forceinline__ float value_v(unsigned word, int j, float scale) {
+  const float root = __fmul_rn(
+      code_value<kTopV, kMantV>(byte_bits<kMantV>(word, j, 255u << (23 - kMantV))), scale);
   return __fmul_rn(root, root);
 }
 
-// Code of ratio in [0, 1]: the bits of the float rounded to MANT mantissa
-// bits (to nearest, ties to even), counted down from TOP; may come out <= 0.
+// Code of a ratio from the smallest code's value on: the bits of the float
+// rounded to MANT mantissa bits (to nearest, ties to even), counted down from
+// TOP.
 template <int TOP, int MANT>
-__device__ __forceinline__ int ratio_code(float ratio) {
+__device__ __forceinline__ unsigned ratio_code(float ratio) {
   constexpr int kShift = 23 - MANT;
-  const int bits = __float_as_int(ratio);
-  const int code = (bits + ((1 << (kShift - 1)) - 1) + ((bits >> kShift) & 1)) >> kShift;
-  return min(code - (127 << MANT) + TOP, TOP);
+  const unsigned bits = __float_as_uint(ratio);
+  return ((bits + ((1u << (kShift - 1)) - 1u) + ((bits >> kShift) & 1u)) >> kShift) -
+         ((127u << MANT) - TOP);
 }
 
 // Largest magnitude over the warp's block; for non-negative floats the order
@@ -130,18 +141,24 @@ __device__ __forceinline__ float inverse_scale(float scale) {
   return scale > 0.0f ? __frcp_rn(scale) : 0.0f;
 }
 
-__device__ __forceinline__ int encode_m(float m, float inv) {
-  const float size = fabsf(m);
-  const float ratio = __fmul_rn(size, inv);
-  int code = ratio_code<kTopM, kMantM>(ratio);
-  // below the smallest code's value (1.25 2^-16): to it or to 0, the nearer
-  if (code < 1) code = ratio >= 0.5f * 1.25f / 65536.0f ? 1 : 0;
-  return m < 0.0f ? code + 128 : code;
-}
+// Ratios are at most 1 up to a rounding that the code drops, unless the scale
+// is so small that its inverse is infinite: then every value but 0 takes the
+// top code (and a NaN's block has a NaN scale, whatever its codes).
+constexpr float kLeastM = 1.25f / 65536.0f, kLeastV = 1.125f / 65536.0f;  // value(1)
 
-__device__ __forceinline__ int encode_v(float root, float inv) {
-  const int code = ratio_code<kTopV, kMantV>(__fmul_rn(root, inv));
-  return root > 0.0f ? max(code, 1) : 0;
+// Below the smallest code's value: to it or to 0, the nearer.
+__device__ __forceinline__ unsigned encode_m(float m, float inv) {
+  const float ratio = fminf(__fmul_rn(fabsf(m), inv), 1.0f);
+  const unsigned code = ratio_code<kTopM, kMantM>(fmaxf(ratio, kLeastM));
+  return (ratio >= 0.5f * kLeastM ? code : 0u) | (m < 0.0f ? 128u : 0u);
+}
+__device__ __forceinline__ unsigned encode_v(float root, float inv) {
+  const float ratio = fminf(__fmul_rn(root, inv), 1.0f);
+  const unsigned code = ratio_code<kTopV, kMantV>(fmaxf(ratio, kLeastV));
+  return root > 0.0f ? code : 0u;
+}
+__device__ __forceinline__ unsigned pack4(const unsigned (&c)[4]) {
+  return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
 template <typename T, int BITS, bool MASTER, int CAP>
@@ -151,12 +168,16 @@ __global__ void __launch_bounds__(kBlock, 4)
   const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
   const float scale = a.grad_scale != nullptr ? __ldg(a.grad_scale) : 1.0f;
   const bool scaled = a.grad_scale != nullptr;
+  int lo = 0;  // last entry whose work_block <= work
   for (int64_t work = global_warp(); work < a.work_blocks; work += warps) {
-    int lo = 0, hi = a.count - 1;  // last entry whose work_block <= work
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (a.entry[mid].work_block <= work) lo = mid;
-      else hi = mid - 1;
+    if (lo + 1 < a.count && a.entry[lo + 1].work_block <= work) {
+      ++lo;
+      int hi = a.count - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.entry[mid].work_block <= work) lo = mid;
+        else hi = mid - 1;
+      }
     }
     const int64_t local = work - a.entry[lo].work_block;
     const int64_t block = a.entry[lo].state_block + local;
@@ -196,14 +217,14 @@ __global__ void __launch_bounds__(kBlock, 4)
         load4(static_cast<const float*>(a.exp_avg) + at, m + i);
         load4(static_cast<const float*>(a.exp_avg_sq) + at, v + i);
       } else {
-        const uchar4 cm = *reinterpret_cast<const uchar4*>(static_cast<uint8_t*>(a.exp_avg) + at);
-        const uchar4 cv =
-            *reinterpret_cast<const uchar4*>(static_cast<uint8_t*>(a.exp_avg_sq) + at);
-        const int codes_m[4] = {cm.x, cm.y, cm.z, cm.w}, codes_v[4] = {cv.x, cv.y, cv.z, cv.w};
+        const unsigned cm =
+            *reinterpret_cast<const unsigned*>(static_cast<uint8_t*>(a.exp_avg) + at);
+        const unsigned cv =
+            *reinterpret_cast<const unsigned*>(static_cast<uint8_t*>(a.exp_avg_sq) + at);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          m[i + j] = value_m(codes_m[j], scale_m);
-          v[i + j] = value_v(codes_v[j], scale_v);
+          m[i + j] = value_m(cm, j, scale_m);
+          v[i + j] = value_v(cv, j, scale_v);
         }
       }
     }
@@ -245,15 +266,15 @@ __global__ void __launch_bounds__(kBlock, 4)
       const float im = inverse_scale(sm), iv = inverse_scale(sv);
 #pragma unroll
       for (int i = 0; i < kPerLane; i += 4) {
-        unsigned codes_m = 0, codes_v = 0;
+        unsigned codes_m[4], codes_v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          codes_m |= static_cast<unsigned>(encode_m(m[i + j], im)) << (8 * j);
-          codes_v |= static_cast<unsigned>(encode_v(root[i + j], iv)) << (8 * j);
+          codes_m[j] = encode_m(m[i + j], im);
+          codes_v[j] = encode_v(root[i + j], iv);
         }
         const int64_t at = state + element(lane, i);
-        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.exp_avg) + at) = codes_m;
-        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.exp_avg_sq) + at) = codes_v;
+        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.exp_avg) + at) = pack4(codes_m);
+        *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.exp_avg_sq) + at) = pack4(codes_v);
       }
       if (lane == 0) {
         a.exp_avg_scale[block] = sm;
@@ -289,8 +310,8 @@ __global__ void __launch_bounds__(kBlock)
       float m[4], v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        m[j] = value_m((cm[u] >> (8 * j)) & 255, sm[u]);
-        v[j] = value_v((cv[u] >> (8 * j)) & 255, sv[u]);
+        m[j] = value_m(cm[u], j, sm[u]);
+        v[j] = value_v(cv[u], j, sv[u]);
       }
       store4(out_m + 4 * q, m);
       store4(out_v + 4 * q, v);
