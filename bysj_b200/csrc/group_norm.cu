@@ -15,15 +15,16 @@
 // going from one piece to the next advances at least one of the two.  A first
 // kernel leaves two numbers per piece and channel (mean and centred square
 // sum; in the backward pass sum dz and sum dz xhat, from which the group's sums
-// and the gradients of weight and bias both follow), a second joins the pieces
-// of each frame in their order, a third writes the result.  It walks each chunk
-// from its end, where the first kernel stopped, so that what L2 still holds is
-// read from there.
+// and the gradients of weight and bias both follow); numbers that no piece has
+// are zero.  A second kernel joins the pieces of each frame and group, a third
+// writes the result.  It walks each chunk from its end, where the first stopped,
+// so that what L2 still holds is read from there.
 //
-// Sums are float32 over the rows of one thread (64 terms at a time, about a
-// value of the piece, so a mean far from 0 takes no digits from the variance)
-// and float64 across threads and pieces.  No atomics: results repeat bit for
-// bit.
+// Sums are float32, of a few tens of terms at a time (rows of a thread, threads
+// of a channel, pieces of a frame), so their rounding does not grow with the
+// rows; float64 arithmetic cost tens of microseconds a kernel here.  Squares are
+// taken about a value near the mean, which costs the variance no digits
+// wherever the mean lies.  No atomics: results repeat bit for bit.
 //
 // z is one multiply-add, x A + B with A = rstd w and B = b - mean A: B's
 // rounding is 2^-24 |mean| rstd w, as large as that of the stored mean.
@@ -45,14 +46,16 @@ struct Frames {
     r = r < 0 ? 0 : r;
     return r > rows ? rows : r;
   }
-  // Last frame that begins at or before row r.
+  // Last frame that begins at or before row r; a whole warp, 32 probes a step.
   __device__ __forceinline__ int64_t of_row(int64_t r) const {
     if (offsets == nullptr) return r / (rows / count);
-    int64_t lo = 0, hi = count - 1;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) >> 1;
-      if (begin(mid) <= r) lo = mid;
-      else hi = mid - 1;
+    int64_t lo = 0, hi = count;
+    while (hi - lo > 1) {
+      const int64_t step = (hi - lo + kWarp - 1) / kWarp, probe = lo + lane_id() * step;
+      const bool before = probe < hi && (probe == lo || begin(probe) <= r);
+      const int64_t next = lo + (__popc(__ballot_sync(kFull, before)) - 1) * step;
+      hi = min(hi, next + step);
+      lo = next;
     }
     return lo;
   }
@@ -78,11 +81,6 @@ struct GroupArgs {
   float2* partial;      // [chunks + frames][channels]
   float2* sums;         // backward: [frames][groups] mean(d), mean(d xhat)
 };
-
-__device__ __forceinline__ float load_f32(const float* p) { return *p; }
-__device__ __forceinline__ float load_f32(const __nv_bfloat16* p) {
-  return __bfloat162float(*p);
-}
 
 // VEC values at p (global or shared memory).
 template <int VEC>
@@ -252,14 +250,32 @@ struct Columns {
   }
 };
 
-// A channel's pair from its sums over `rows` rows; forward sums are about x[c].
-template <typename T, bool BACKWARD>
-__device__ __forceinline__ float2 channel_value(double s1, double s2, int64_t rows, const T* x,
-                                                int c) {
-  if constexpr (BACKWARD) return make_float2(static_cast<float>(s1), static_cast<float>(s2));
-  const double n = static_cast<double>(rows);
-  return make_float2(static_cast<float>(load_f32(x + c) + s1 / n),
-                     static_cast<float>(s2 - s1 * s1 / n));
+// A channel's pair from its sums over `rows` rows; forward sums are about the
+// pivot.
+template <bool BACKWARD>
+__device__ __forceinline__ float2 channel_value(float s1, float s2, int64_t rows, float pivot) {
+  if constexpr (BACKWARD) return make_float2(s1, s2);
+  const float mean = s1 / static_cast<float>(rows);
+  return make_float2(pivot + mean, fmaxf(fmaf(-s1, mean, s2), 0.0f));
+}
+
+// Adds n terms term(i) for i = first, first + step, ...: eight at a time, the
+// eights then to the sum, so that the rounding grows with n / 8 + 8 terms.
+template <typename Term>
+__device__ __forceinline__ void add_terms(int first, int n, int step, float& s1, float& s2,
+                                          Term term) {
+  for (int i = first; i < n;) {
+    float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u, i += step) {
+      if (i >= n) continue;
+      const float2 v = term(i);
+      t1 += v.x;
+      t2 += v.y;
+    }
+    s1 += t1;
+    s2 += t2;
+  }
 }
 
 // Channel sums over a slab's rows into chan[] (forward: mean and the sum of
@@ -267,12 +283,22 @@ __device__ __forceinline__ float2 channel_value(double s1, double s2, int64_t ro
 template <typename T, int VEC, int THREADS, bool BACKWARD, int ACT>
 __device__ __forceinline__ void column_stats(const Tile<VEC, THREADS>& t, const T* x, const T* dy,
                                              int64_t rows, int channels, const Columns<VEC>& q,
-                                             float* scratch, double2* level, float2* chan) {
+                                             float* scratch, float2* level, float2* chan) {
   float s1[VEC], s2[VEC], pivot[VEC], o1[VEC], o2[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = o1[i] = o2[i] = pivot[i] = 0.0f;
   if (t.on) {
-    if constexpr (!BACKWARD) load_vec<VEC>(x + t.c, pivot);
+    if constexpr (!BACKWARD) {  // about the mean of the first rows
+      const int count = rows < 4 ? static_cast<int>(rows) : 4;
+      for (int r = 0; r < count; ++r) {
+        float v[VEC];
+        load_vec<VEC>(x + r * static_cast<int64_t>(channels) + t.c, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) pivot[i] += v[i];
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) pivot[i] /= static_cast<float>(count);
+    }
     auto add = [&](const float (&v)[VEC], const float (&g)[VEC]) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -314,6 +340,7 @@ __device__ __forceinline__ void column_stats(const Tile<VEC, THREADS>& t, const 
     for (int i = 0; i < VEC; ++i) {
       place[i] = s1[i];
       place[THREADS * VEC + i] = s2[i];
+      if (t.ry == 0) chan[t.c + i].x = pivot[i];
     }
   }
   __syncthreads();
@@ -321,27 +348,27 @@ __device__ __forceinline__ void column_stats(const Tile<VEC, THREADS>& t, const 
   const int parts = t.width < THREADS ? THREADS / t.width : 1;
   const int share = (t.ty + parts - 1) / parts;
   for (int i = threadIdx.x; i < parts * t.width; i += THREADS) {
-    const int part = i / t.width, c = i % t.width;
-    double a1 = 0.0, a2 = 0.0;
+    const int part = i / t.width, c = i - part * t.width;
+    float a1 = 0.0f, a2 = 0.0f;
     for (int r = part * share; r < min((part + 1) * share, t.ty); ++r) {
       a1 += scratch[r * t.width + c];
       a2 += scratch[THREADS * VEC + r * t.width + c];
     }
     if (parts > 1) {
-      level[i] = make_double2(a1, a2);
+      level[i] = make_float2(a1, a2);
     } else {
-      chan[t.c0 + c] = channel_value<T, BACKWARD>(a1, a2, rows, x, t.c0 + c);
+      chan[t.c0 + c] = channel_value<BACKWARD>(a1, a2, rows, chan[t.c0 + c].x);
     }
   }
   __syncthreads();
   if (parts > 1) {
     for (int c = threadIdx.x; c < t.width; c += THREADS) {
-      double a1 = 0.0, a2 = 0.0;
+      float a1 = 0.0f, a2 = 0.0f;
       for (int part = 0; part < parts; ++part) {
         a1 += level[part * t.width + c].x;
         a2 += level[part * t.width + c].y;
       }
-      chan[t.c0 + c] = channel_value<T, BACKWARD>(a1, a2, rows, x, t.c0 + c);
+      chan[t.c0 + c] = channel_value<BACKWARD>(a1, a2, rows, chan[t.c0 + c].x);
     }
     __syncthreads();
   }
@@ -353,22 +380,22 @@ template <bool BACKWARD>
 __device__ __forceinline__ float2 join_channels(const GroupArgs& a, const float2* chan, int g,
                                                 int64_t rows) {
   const int lane = lane_id(), c0 = g * a.group_channels;
-  double s1 = 0.0, s2 = 0.0;
+  float s1 = 0.0f, s2 = 0.0f;
   for (int c = c0 + lane; c < c0 + a.group_channels; c += kWarp) {
-    const double w = BACKWARD && a.weight ? __ldg(a.weight + c) : 1.0;
+    const float w = BACKWARD && a.weight ? __ldg(a.weight + c) : 1.0f;
     s1 += w * chan[c].x;
     s2 += w * chan[c].y;
   }
   s1 = xor_sum(s1, 1);
   if constexpr (!BACKWARD) {
-    s1 /= a.group_channels;
+    s1 /= static_cast<float>(a.group_channels);
     for (int c = c0 + lane; c < c0 + a.group_channels; c += kWarp) {
-      const double d = chan[c].x - s1;
-      s2 += static_cast<double>(rows) * d * d;
+      const float d = chan[c].x - s1;
+      s2 += static_cast<float>(rows) * d * d;
     }
   }
   s2 = xor_sum(s2, 1);
-  return make_float2(static_cast<float>(s1), static_cast<float>(s2));
+  return make_float2(s1, s2);
 }
 
 // y or dx of `rows` rows, the last first.  The result is written past L1 with
@@ -402,21 +429,21 @@ __device__ __forceinline__ void apply_rows(const Tile<VEC, THREADS>& t, const T*
   });
 }
 
-// Shared memory of both kernels: float scratch [2][THREADS * VEC], double2 level [THREADS], chan [channels], stats
-// [groups] and, backward, the affine sums [channels].
+// Shared memory of both kernels: level [THREADS], scratch [2][THREADS * VEC],
+// chan [channels], stats [groups] and, backward, the affine sums [channels].
 template <int VEC, int THREADS>
 __host__ __device__ constexpr size_t fixed_smem(int channels, int groups, bool backward) {
-  return sizeof(float) * 2 * THREADS * VEC + sizeof(double2) * THREADS +
+  return sizeof(float) * 2 * THREADS * VEC + sizeof(float2) * THREADS +
          sizeof(float2) * (static_cast<size_t>(channels) * (backward ? 2 : 1) + groups);
 }
 
 template <int VEC, int THREADS>
 struct Smem {
-  double2* level;
+  float2* level;
   float* scratch;
   float2 *chan, *stats, *affine;
   __device__ Smem(unsigned char* base, int channels, int groups) {
-    level = reinterpret_cast<double2*>(base);
+    level = reinterpret_cast<float2*>(base);
     scratch = reinterpret_cast<float*>(level + THREADS);
     chan = reinterpret_cast<float2*>(scratch + 2 * THREADS * VEC);
     stats = chan + channels;
@@ -424,9 +451,8 @@ struct Smem {
   }
 };
 
-__device__ __forceinline__ float2 moments(const GroupArgs& a, double mean, double square,
-                                          double n) {
-  return make_float2(static_cast<float>(mean), static_cast<float>(1.0 / sqrt(square / n + a.eps)));
+__device__ __forceinline__ float2 moments(const GroupArgs& a, float mean, float variance) {
+  return make_float2(mean, 1.0f / sqrtf(fmaxf(variance, 0.0f) + a.eps));
 }
 
 // Statistics of one tile's thread: mean and rstd of frame b, and its sums.
@@ -471,12 +497,12 @@ __global__ void __launch_bounds__(THREADS) group_frame_kernel(GroupArgs a) {
     }
     for (int g = warp; g < a.groups; g += THREADS / kWarp) {
       const float2 v = join_channels<BACKWARD>(a, m.chan, g, rows);
-      const double n = static_cast<double>(rows) * a.group_channels;
+      const float n = static_cast<float>(rows) * static_cast<float>(a.group_channels);
       if (lane_id() == 0) {
         if constexpr (BACKWARD) {
-          m.stats[g] = make_float2(static_cast<float>(v.x / n), static_cast<float>(v.y / n));
+          m.stats[g] = make_float2(v.x / n, v.y / n);
         } else {
-          m.stats[g] = moments(a, v.x, v.y, n);
+          m.stats[g] = moments(a, v.x, v.y / n);
           a.mean[b * a.groups + g] = m.stats[g].x;
           a.rstd[b * a.groups + g] = m.stats[g].y;
         }
@@ -513,7 +539,86 @@ __global__ void __launch_bounds__(THREADS) group_frame_kernel(GroupArgs a) {
 
 // ---- chunks of all frames ---------------------------------------------------
 
+__device__ __forceinline__ float block_sum(float v, float* scratch) {
+  v = xor_sum(v, 1);
+  __syncthreads();
+  if (lane_id() == 0) scratch[threadIdx.x / kWarp] = v;
+  __syncthreads();
+  float total = 0.0f;
+  for (int i = 0; i < kWarpsPerBlock; ++i) total += scratch[i];
+  return total;
+}
+
+// Sums rows of channel pairs in a fixed order into the gradients of weight
+// and bias, 32 channels a CTA.
+__device__ __forceinline__ void affine_grad(const GroupArgs& a, int tile, const float2* rows,
+                                            int64_t count) {
+  __shared__ float2 part[kWarpsPerBlock][kWarp];
+  const int warp = threadIdx.x / kWarp, c = tile * kWarp + lane_id();
+  float s1 = 0.0f, s2 = 0.0f;
+  if (c < a.channels)
+    add_terms(warp, static_cast<int>(count), kWarpsPerBlock, s1, s2,
+              [&](int i) { return rows[static_cast<int64_t>(i) * a.channels + c]; });
+  part[warp][lane_id()] = make_float2(s1, s2);
+  __syncthreads();
+  if (warp == 0 && c < a.channels) {
+    s1 = s2 = 0.0f;
+    for (int i = 0; i < kWarpsPerBlock; ++i) {
+      s1 += part[i][lane_id()].x;
+      s2 += part[i][lane_id()].y;
+    }
+    if (a.grad_bias) a.grad_bias[c] = s1;
+    if (a.grad_weight) a.grad_weight[c] = s2;
+  }
+}
+
 constexpr int kChunkThreads = 256;
+static_assert(kChunkThreads == kBlock, "affine_grad and block_sum run in both kernels");
+
+// The pieces of a frame, for one channel: terms whose sums (and n, all values
+// of the group) give its group's numbers.  Backward: sum d, sum d xhat; forward:
+// the sum and the sum of squares about `centre`, the first piece's mean of the
+// group's first channel.
+template <bool BACKWARD>
+struct Pieces {
+  const GroupArgs& a;
+  int64_t r0, r1, first;
+  int count;
+  float n;
+  const float2* partial;  // the first piece's channels
+  __device__ Pieces(const GroupArgs& args, int64_t b) : a(args) {
+    r0 = a.frames.begin(b);
+    r1 = a.frames.begin(b + 1);
+    first = r0 / a.chunk_rows;
+    count = static_cast<int>((r1 - 1) / a.chunk_rows - first) + 1;
+    n = static_cast<float>(r1 - r0) * static_cast<float>(a.group_channels);
+    partial = a.partial + (first + b) * a.channels;
+  }
+  __device__ float centre(int g) const { return BACKWARD ? 0.0f : partial[g * a.group_channels].x; }
+  // Pieces from, from + step, ... of channel c into s1 and s2.
+  __device__ void add(int c, float middle, int from, int step, float& s1, float& s2) const {
+    const float w = BACKWARD && a.weight ? __ldg(a.weight + c) : 1.0f;
+    add_terms(from, count, step, s1, s2, [&](int p) {
+      float2 v = partial[static_cast<int64_t>(p) * a.channels + c];
+      if constexpr (BACKWARD) {
+        v.x *= w;
+        v.y *= w;
+      } else {
+        const int64_t chunk = first + p;
+        const float rows = static_cast<float>(
+            static_cast<int>(min((chunk + 1) * a.chunk_rows, r1) - max(chunk * a.chunk_rows, r0)));
+        const float d = v.x - middle;
+        v = make_float2(rows * d, fmaf(rows * d, d, v.y));
+      }
+      return v;
+    });
+  }
+  __device__ float2 numbers(int g, float s1, float s2) const {
+    s1 /= n;
+    if constexpr (BACKWARD) return make_float2(s1, s2 / n);
+    else return moments(a, centre(g) + s1, fmaf(-s1, s1, s2 / n));
+  }
+};
 
 // APPLY: y or dx; otherwise the pieces' numbers.  One chunk a CTA.
 template <typename T, int VEC, bool BACKWARD, int ACT, bool APPLY>
@@ -527,10 +632,20 @@ __global__ void __launch_bounds__(kChunkThreads, BACKWARD ? 3 : 4)
   const T* dy = static_cast<const T*>(BACKWARD ? a.grad_out : a.x);
   const int64_t chunk = blockIdx.x;
   const int64_t r0 = chunk * a.chunk_rows, r1 = min(r0 + a.chunk_rows, a.frames.rows);
-  int64_t lo = r0;
-  for (int64_t b = a.frames.of_row(r0); b < a.frames.count && lo < r1; ++b) {
+  const int64_t b0 = a.frames.of_row(r0);
+  auto no_piece = [&](int64_t from, int64_t to) {  // numbers [from, to)
+    if constexpr (!APPLY)
+      for (int64_t i = from * C + threadIdx.x; i < to * C; i += kThreads)
+        a.partial[i] = make_float2(0.0f, 0.0f);
+  };
+  no_piece(chunk == 0 ? 0 : chunk + b0, chunk + b0);
+  int64_t lo = r0, b = b0;
+  for (; b < a.frames.count && lo < r1; ++b) {
     const int64_t hi = min(a.frames.begin(b + 1), r1);
-    if (hi <= lo) continue;
+    if (hi <= lo) {
+      no_piece(chunk + b, chunk + b + 1);
+      continue;
+    }
     for (int c0 = 0; c0 < C; c0 += kThreads * VEC) {
       const Tile<VEC, kThreads> t(c0, C);
       Columns<VEC> q;
@@ -550,43 +665,10 @@ __global__ void __launch_bounds__(kChunkThreads, BACKWARD ? 3 : 4)
     }
     lo = hi;
   }
-}
-
-__device__ __forceinline__ double block_sum(double v, double* scratch) {
-  v = xor_sum(v, 1);
-  __syncthreads();
-  if (lane_id() == 0) scratch[threadIdx.x / kWarp] = v;
-  __syncthreads();
-  double total = 0.0;
-  for (int i = 0; i < kWarpsPerBlock; ++i) total += scratch[i];
-  return total;
-}
-
-// Sums rows of channel pairs in a fixed order into the gradients of weight
-// and bias, 32 channels a CTA.
-__device__ __forceinline__ void affine_grad(const GroupArgs& a, int tile, const float2* rows,
-                                            int64_t count) {
-  __shared__ double2 part[kWarpsPerBlock][kWarp];
-  const int warp = threadIdx.x / kWarp, c = tile * kWarp + lane_id();
-  double s1 = 0.0, s2 = 0.0;
-  if (c < a.channels) {
-#pragma unroll 8
-    for (int64_t i = warp; i < count; i += kWarpsPerBlock) {
-      const float2 v = rows[i * a.channels + c];
-      s1 += v.x;
-      s2 += v.y;
-    }
-  }
-  part[warp][lane_id()] = make_double2(s1, s2);
-  __syncthreads();
-  if (warp == 0 && c < a.channels) {
-    s1 = s2 = 0.0;
-    for (int i = 0; i < kWarpsPerBlock; ++i) {
-      s1 += part[i][lane_id()].x;
-      s2 += part[i][lane_id()].y;
-    }
-    if (a.grad_bias) a.grad_bias[c] = static_cast<float>(s1);
-    if (a.grad_weight) a.grad_weight[c] = static_cast<float>(s2);
+  if constexpr (!APPLY) {  // up to the next chunk's first number
+    const int64_t next =
+        r1 < a.frames.rows ? chunk + 1 + a.frames.of_row(r1) : a.chunks + a.frames.count;
+    no_piece(chunk + b, next);
   }
 }
 
@@ -594,12 +676,11 @@ __global__ void __launch_bounds__(kBlock) group_affine_kernel(GroupArgs a, int c
   affine_grad(a, blockIdx.x, a.affine, ctas);
 }
 
-// Joins the pieces of one frame and group a CTA (in steps of the grid); the
-// first `tiles` CTAs take the gradients of weight and bias, from all pieces
-// (rows that no piece has are zero).
+// Joins the pieces of one frame and group a CTA, in steps of the grid; the
+// first `tiles` CTAs take the gradients of weight and bias, from all pieces.
 template <bool BACKWARD>
 __global__ void __launch_bounds__(kBlock) group_join_kernel(GroupArgs a, int tiles) {
-  __shared__ double scratch[kWarpsPerBlock];
+  __shared__ float scratch[kWarpsPerBlock];
   if constexpr (BACKWARD) {
     if (static_cast<int>(blockIdx.x) < tiles) {
       affine_grad(a, blockIdx.x, a.partial, a.chunks + a.frames.count);
@@ -610,47 +691,25 @@ __global__ void __launch_bounds__(kBlock) group_join_kernel(GroupArgs a, int til
   for (int64_t unit = blockIdx.x - tiles; unit < units; unit += gridDim.x - tiles) {
     const int64_t b = unit / a.groups;
     const int g = static_cast<int>(unit % a.groups), c0 = g * a.group_channels;
-    const int64_t r0 = a.frames.begin(b), r1 = a.frames.begin(b + 1);
-    if (r1 <= r0) {
+    if (a.frames.begin(b + 1) <= a.frames.begin(b)) {
       if constexpr (!BACKWARD)
         if (threadIdx.x == 0) a.mean[unit] = a.rstd[unit] = 0.0f;
       continue;
     }
-    const int64_t first = r0 / a.chunk_rows, pieces = (r1 - 1) / a.chunk_rows - first + 1;
-    const double n = static_cast<double>(r1 - r0) * a.group_channels;
-    const float2* partial = a.partial + (first + b) * a.channels + c0;
-    // threads side by side over the group's channels, then over pieces; the
-    // sum and the sum of squares about the first piece's mean
+    const Pieces<BACKWARD> pieces(a, b);
     const int width = a.group_channels < kBlock ? a.group_channels : kBlock;
     const int lanes = kBlock / width, rank = threadIdx.x / width;
-    const double centre = BACKWARD ? 0.0 : partial->x;
-    double s1 = 0.0, s2 = 0.0;
-    if (rank < lanes) {
-      for (int c = threadIdx.x % width; c < a.group_channels; c += width) {
-        const double w = BACKWARD && a.weight ? __ldg(a.weight + c0 + c) : 1.0;
-#pragma unroll 8
-        for (int64_t p = rank; p < pieces; p += lanes) {
-          const float2 v = partial[p * a.channels + c];
-          if constexpr (BACKWARD) {
-            s1 += w * v.x;
-            s2 += w * v.y;
-          } else {
-            const double m = static_cast<double>(min((first + p + 1) * a.chunk_rows, r1) -
-                                                 max((first + p) * a.chunk_rows, r0));
-            const double d = v.x - centre;
-            s1 += m * d;
-            s2 += v.y + m * d * d;
-          }
-        }
-      }
-    }
+    float s1 = 0.0f, s2 = 0.0f;
+    if (rank < lanes)
+      for (int c = threadIdx.x % width; c < a.group_channels; c += width)
+        pieces.add(c0 + c, pieces.centre(g), rank, lanes, s1, s2);
     s1 = block_sum(s1, scratch);
     s2 = block_sum(s2, scratch);
     if (threadIdx.x == 0) {
+      const float2 v = pieces.numbers(g, s1, s2);
       if constexpr (BACKWARD) {
-        a.sums[unit] = make_float2(static_cast<float>(s1 / n), static_cast<float>(s2 / n));
+        a.sums[unit] = v;
       } else {
-        const float2 v = moments(a, centre + s1 / n, fmax(s2 - s1 * s1 / n, 0.0), n);
         a.mean[unit] = v.x;
         a.rstd[unit] = v.y;
       }
@@ -753,24 +812,18 @@ int launch_act(const GroupArgs& a, const Plan& p, cudaStream_t s) {
     group_affine_kernel<<<tiles, kBlock, 0, s>>>(a, p.ctas);
     return launch_check("group_affine_kernel");
   }
-  int st = BYSJ_OK;
-  if (affine)
-    st = cuda_check(cudaMemsetAsync(a.partial, 0,
-                                    sizeof(float2) * (a.chunks + a.frames.count) * a.channels, s),
-                    "group norm: zero the pieces");
-  if (st) return st;
   const unsigned chunks = static_cast<unsigned>(p.chunks);
   const size_t smem = fixed_smem<VEC, kChunkThreads>(a.channels, a.groups, BACKWARD);
-  st = launch_one(group_chunk_kernel<T, VEC, BACKWARD, ACT, false>, "group_chunk_kernel", chunks,
-                  kChunkThreads, smem, a, s);
+  int st = launch_one(group_chunk_kernel<T, VEC, BACKWARD, ACT, false>, "group_chunk_kernel",
+                      chunks, kChunkThreads, smem, a, s);
   if (st) return st;
   const int64_t units = a.frames.count * a.groups;
   group_join_kernel<BACKWARD>
       <<<static_cast<unsigned>((units < 65536 ? units : 65536) + tiles), kBlock, 0, s>>>(a, tiles);
   st = launch_check("group_join_kernel");
   if (st) return st;
-  return launch_one(group_chunk_kernel<T, VEC, BACKWARD, ACT, true>, "group_chunk_kernel", chunks,
-                    kChunkThreads, 0, a, s);
+  return launch_one(group_chunk_kernel<T, VEC, BACKWARD, ACT, true>, "group_chunk_kernel",
+                    chunks, kChunkThreads, 0, a, s);
 }
 
 template <typename T, int VEC, bool BACKWARD>
