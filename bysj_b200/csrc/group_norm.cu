@@ -78,6 +78,7 @@ struct GroupArgs {
   float2* affine;  // backward, frame kernel: [CTAs][channels] sum dz, sum dz xhat
   // chunks
   int64_t chunk_rows, chunks;
+  int64_t apply_rows;   // of a CTA of the result
   float2* partial;      // [chunks + frames][channels]
   float2* sums;         // backward: [frames][groups] mean(d), mean(d xhat)
 };
@@ -131,10 +132,11 @@ struct Raw {
   }
 };
 
-// A thread's rows of one or two arrays, kRows at a time.
-template <typename T, int VEC, bool TWO>
+// A thread's rows of one or two arrays, kRows at a time (of BYTES together).
+template <typename T, int VEC, bool TWO, int BYTES>
 struct Rows {
-  static constexpr int kRows = 32 / (VEC * sizeof(T) * (TWO ? 2 : 1)) * (VEC == 1 ? 1 : 2);
+  static constexpr int kRows =
+      VEC == 1 ? 8 : BYTES / static_cast<int>(VEC * sizeof(T) * (TWO ? 2 : 1));
   Raw<T, VEC> a[kRows], b[TWO ? kRows : 1];
   __device__ __forceinline__ void load(const T*& pa, const T*& pb, int64_t step) {
 #pragma unroll
@@ -164,10 +166,10 @@ struct Rows {
 
 // use(a, b) for n rows of a thread in order, the next kRows requested before
 // the last ones are used.
-template <typename T, int VEC, bool TWO, typename Use>
+template <typename T, int VEC, bool TWO, int BYTES, typename Use>
 __device__ __forceinline__ void each_row(const T* pa, const T* pb, int64_t step, int64_t n,
                                          Use use) {
-  using RowsT = Rows<T, VEC, TWO>;
+  using RowsT = Rows<T, VEC, TWO, BYTES>;
   constexpr int kRows = RowsT::kRows;
   const int rest = static_cast<int>(n % kRows);
   auto apply = [&](const RowsT& rows, int j) {
@@ -319,7 +321,7 @@ __device__ __forceinline__ void column_stats(const Tile<VEC, THREADS>& t, const 
     const T* pg = dy + t.ry * static_cast<int64_t>(channels) + t.c;
     const int64_t n = rows > t.ry ? (rows - t.ry + t.ty - 1) / t.ty : 0;  // of this thread
     int left = 64;  // terms of the inner sums before they join the outer ones
-    each_row<T, VEC, BACKWARD>(px, pg, step, n, [&](const float(&v)[VEC], const float(&g)[VEC]) {
+    each_row<T, VEC, BACKWARD, BACKWARD ? 128 : 64>(px, pg, step, n, [&](const float(&v)[VEC], const float(&g)[VEC]) {
       add(v, g);
       if (--left > 0) return;
       left = 64;
@@ -412,7 +414,7 @@ __device__ __forceinline__ void apply_rows(const Tile<VEC, THREADS>& t, const T*
   const T* px = x + at;
   const T* pg = dy + at;
   T* py = out + at;
-  each_row<T, VEC, BACKWARD>(px, pg, -step, n, [&](const float(&v)[VEC], const float(&g)[VEC]) {
+  each_row<T, VEC, BACKWARD, 64>(px, pg, -step, n, [&](const float(&v)[VEC], const float(&g)[VEC]) {
     float y[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -550,22 +552,25 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 }
 
 // Sums rows of channel pairs in a fixed order into the gradients of weight
-// and bias, 32 channels a CTA.
+// and bias: 8 channels a CTA, 32 rows at a time.
+constexpr int kAffineChannels = 8;
+
 __device__ __forceinline__ void affine_grad(const GroupArgs& a, int tile, const float2* rows,
                                             int64_t count) {
-  __shared__ float2 part[kWarpsPerBlock][kWarp];
-  const int warp = threadIdx.x / kWarp, c = tile * kWarp + lane_id();
+  constexpr int kAbreast = kBlock / kAffineChannels;
+  __shared__ float2 part[kAbreast][kAffineChannels];
+  const int rank = threadIdx.x / kAffineChannels, lane = threadIdx.x % kAffineChannels;
+  const int c = tile * kAffineChannels + lane;
   float s1 = 0.0f, s2 = 0.0f;
   if (c < a.channels)
-    add_terms(warp, static_cast<int>(count), kWarpsPerBlock, s1, s2,
+    add_terms(rank, static_cast<int>(count), kAbreast, s1, s2,
               [&](int i) { return rows[static_cast<int64_t>(i) * a.channels + c]; });
-  part[warp][lane_id()] = make_float2(s1, s2);
+  part[rank][lane] = make_float2(s1, s2);
   __syncthreads();
-  if (warp == 0 && c < a.channels) {
-    s1 = s2 = 0.0f;
-    for (int i = 0; i < kWarpsPerBlock; ++i) {
-      s1 += part[i][lane_id()].x;
-      s2 += part[i][lane_id()].y;
+  if (rank == 0 && c < a.channels) {
+    for (int i = 1; i < kAbreast; ++i) {
+      s1 += part[i][lane].x;
+      s2 += part[i][lane].y;
     }
     if (a.grad_bias) a.grad_bias[c] = s1;
     if (a.grad_weight) a.grad_weight[c] = s2;
@@ -620,9 +625,17 @@ struct Pieces {
   }
 };
 
+// CTAs of the kernel below on one SM.  In the statistics of the backward pass
+// more rows in flight for each thread do better than a third CTA (180001 x 96
+// float32: 35 us against 44); in the other kernels it is the other way round
+// (result of the backward pass, 393216 x 128 bfloat16: 59 us against 71).
+__host__ __device__ constexpr int chunk_ctas(bool backward, bool apply) {
+  return backward ? (apply ? 3 : 2) : 4;
+}
+
 // APPLY: y or dx; otherwise the pieces' numbers.  One chunk a CTA.
 template <typename T, int VEC, bool BACKWARD, int ACT, bool APPLY>
-__global__ void __launch_bounds__(kChunkThreads, BACKWARD ? 3 : 4)
+__global__ void __launch_bounds__(kChunkThreads, chunk_ctas(BACKWARD, APPLY))
     group_chunk_kernel(GroupArgs a) {
   constexpr int kThreads = kChunkThreads;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -631,7 +644,8 @@ __global__ void __launch_bounds__(kChunkThreads, BACKWARD ? 3 : 4)
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(BACKWARD ? a.grad_out : a.x);
   const int64_t chunk = blockIdx.x;
-  const int64_t r0 = chunk * a.chunk_rows, r1 = min(r0 + a.chunk_rows, a.frames.rows);
+  const int64_t chunk_rows = APPLY ? a.apply_rows : a.chunk_rows;
+  const int64_t r0 = chunk * chunk_rows, r1 = min(r0 + chunk_rows, a.frames.rows);
   const int64_t b0 = a.frames.of_row(r0);
   auto no_piece = [&](int64_t from, int64_t to) {  // numbers [from, to)
     if constexpr (!APPLY)
@@ -727,7 +741,7 @@ struct Plan {
   bool chunked = false;
   int ctas = 1;
   int threads = 256;  // frame kernel
-  int64_t chunk_rows = 1, chunks = 0;
+  int64_t chunk_rows = 1, chunks = 0, apply_rows = 1;
 };
 
 // Depends on sizes only, so that the workspace size follows from them; `item`
@@ -743,8 +757,12 @@ Plan make_plan(int64_t rows, int64_t channels, int64_t frames, int item, bool ba
   if (!p.chunked) return p;
   // one chunk for each resident CTA, of 16 KB at least
   const int64_t least = (16384 + row_bytes - 1) / row_bytes;
-  p.chunk_rows = (rows + sms * (backward ? 3 : 4) - 1) / (sms * (backward ? 3 : 4));
-  if (p.chunk_rows < least) p.chunk_rows = least;
+  const auto cut = [&](bool apply) {
+    const int64_t ctas = sms * chunk_ctas(backward, apply), each = (rows + ctas - 1) / ctas;
+    return each < least ? least : each;
+  };
+  p.chunk_rows = cut(false);
+  p.apply_rows = cut(true);
   p.chunks = (rows + p.chunk_rows - 1) / p.chunk_rows;
   return p;
 }
@@ -800,7 +818,7 @@ int launch_one(GroupKernel kernel, const char* name, unsigned ctas, int threads,
 template <typename T, int VEC, bool BACKWARD, int ACT>
 int launch_act(const GroupArgs& a, const Plan& p, cudaStream_t s) {
   const bool affine = BACKWARD && (a.grad_weight != nullptr || a.grad_bias != nullptr);
-  const int tiles = affine ? (a.channels + kWarp - 1) / kWarp : 0;
+  const int tiles = affine ? (a.channels + kAffineChannels - 1) / kAffineChannels : 0;
   if (!p.chunked) {
     const int st =
         p.threads == 512
@@ -823,7 +841,8 @@ int launch_act(const GroupArgs& a, const Plan& p, cudaStream_t s) {
   st = launch_check("group_join_kernel");
   if (st) return st;
   return launch_one(group_chunk_kernel<T, VEC, BACKWARD, ACT, true>, "group_chunk_kernel",
-                    chunks, kChunkThreads, 0, a, s);
+                    static_cast<unsigned>((a.frames.rows + p.apply_rows - 1) / p.apply_rows),
+                    kChunkThreads, 0, a, s);
 }
 
 template <typename T, int VEC, bool BACKWARD>
@@ -849,6 +868,7 @@ int launch(GroupArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t s
                 workspace_bytes);
   a.chunk_rows = p.chunk_rows;
   a.chunks = p.chunks;
+  a.apply_rows = p.apply_rows;
   return vectors ? launch_vec<T, 4, BACKWARD>(a, p, s) : launch_vec<T, 1, BACKWARD>(a, p, s);
 }
 

@@ -14,7 +14,7 @@ from typing import Any, Iterable, Sequence
 
 import torch
 
-from .native import _extension, require_dcu
+from .native import _entry, _extension, require_dcu
 
 BLOCK = 256
 
@@ -87,6 +87,7 @@ class AdamW:
         self.exp_avg = torch.zeros(length, dtype=dtype, device=device)
         self.exp_avg_sq = torch.zeros(length, dtype=dtype, device=device)
         self.exp_avg_scale = self.exp_avg_sq_scale = self.master = None
+        self._tensors = _extension("AdamWParams").AdamWParams(self.params, self.begins)
         if state_bits == 8:
             self.exp_avg_scale = torch.zeros(length // BLOCK, device=device)
             self.exp_avg_sq_scale = torch.zeros(length // BLOCK, device=device)
@@ -113,7 +114,7 @@ class AdamW:
         """
         if grads is None:
             grads = [p.grad for p in self.params]
-        else:
+        elif not isinstance(grads, list):
             grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError("AdamW needs one gradient (or None) for each parameter")
@@ -123,8 +124,8 @@ class AdamW:
             if grad_scale.numel() != 1:
                 raise ValueError("AdamW grad_scale must have one element")
         step, (beta1, beta2) = self.step_count + 1, self.betas
-        _extension("adamw_step").adamw_step(
-            self.params, grads, self.begins, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale,
+        _entry("adamw_step")(
+            self._tensors, grads, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale,
             self.exp_avg_sq_scale, self.master, grad_scale, beta1, beta2,
             1.0 - self.lr * self.weight_decay, self.lr / (1.0 - beta1 ** step),
             1.0 / math.sqrt(1.0 - beta2 ** step), self.eps)
@@ -139,7 +140,7 @@ class AdamW:
         """The moments as float32 buffers: the states themselves with 32 bits."""
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
-        return _extension("adamw_state_values").adamw_state_values(
+        return _entry("adamw_state_values")(
             self.exp_avg, self.exp_avg_sq, self.exp_avg_scale, self.exp_avg_sq_scale)
 
     _BUFFERS = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master")

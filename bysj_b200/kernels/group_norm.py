@@ -13,7 +13,7 @@ import math
 import torch
 
 from . import segment as _segment
-from .native import _extension, require_dcu
+from .native import _entry, require_dcu
 
 MAX_CHANNELS = 8192
 _ACTIVATIONS = {None: 0, "none": 0, "silu": 1, "sigmoid": 2}
@@ -77,11 +77,10 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     results repeat bit for bit.
     """
     eps = _validate(x, groups, weight, bias, eps, activation, offsets)
-    require_dcu(x, weight, bias, offsets)
+    require_dcu(x)  # the others share its device
     if offsets is not None and _segment._should_check(None):
         _segment.check_indices(offsets, x.shape[0], name="group norm")
-    return _extension("group_norm").group_norm(x, groups, weight, bias, eps,
-                                               _ACTIVATIONS[activation], offsets)
+    return _entry("group_norm")(x, groups, weight, bias, eps, _ACTIVATIONS[activation], offsets)
 
 
 __all__ = ["MAX_CHANNELS", "group_norm"]

@@ -80,4 +80,15 @@ def _extension(required_symbol: str):
     return extension
 
 
+_entries: dict = {}
+
+
+def _entry(symbol: str):
+    """The extension's entry point ``symbol``, looked up once per process."""
+    entry = _entries.get(symbol)
+    if entry is None:
+        entry = _entries[symbol] = getattr(_extension(symbol), symbol)
+    return entry
+
+
 __all__ = ["require_b200", "require_dcu"]

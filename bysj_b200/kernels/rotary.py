@@ -13,7 +13,7 @@ from typing import Sequence
 
 import torch
 
-from .native import _extension, require_dcu
+from .native import _entry, require_dcu
 
 MAX_AXES = 4
 
@@ -80,10 +80,9 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     ``positions`` (not for ``inv_freq``).
     """
     sections = _validate(q, k, positions, inv_freq, sections)
-    require_dcu(q, k, positions, inv_freq)
+    require_dcu(q)  # the others share its device
     other = q.new_empty((q.shape[0], 0, q.shape[2])) if k is None else k
-    yq, yk = _extension("rotary_axes").rotary_axes(q, other, positions, inv_freq, sections,
-                                                   bool(interleaved))
+    yq, yk = _entry("rotary_axes")(q, other, positions, inv_freq, sections, bool(interleaved))
     return yq, (None if k is None else yk)
 
 

@@ -13,7 +13,7 @@ from typing import NamedTuple
 import torch
 
 from . import segment as _segment
-from .native import _extension, require_dcu
+from .native import _entry, require_dcu
 
 MAX_EXPERTS = 1024
 MAX_K = 32
@@ -79,11 +79,10 @@ def route_experts(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = N
     ``weights``, ``balance`` and ``z`` are differentiable.
     """
     _validate(logits, k, mask, offsets)
-    require_dcu(logits, mask, offsets)
+    require_dcu(logits)  # the others share its device
     if offsets is not None and _segment._should_check(None):
         _segment.check_indices(offsets, logits.shape[0], name="router")
-    return Routing(*_extension("route_experts").route_experts(logits, k, mask, offsets,
-                                                              bool(renormalize)))
+    return Routing(*_entry("route_experts")(logits, k, mask, offsets, bool(renormalize)))
 
 
 __all__ = ["MAX_EXPERTS", "MAX_K", "Routing", "route_experts"]
