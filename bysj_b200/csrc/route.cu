@@ -100,18 +100,24 @@ __device__ __forceinline__ void copy_vec(T* to, const T* from) {
   else *to = *from;
 }
 
-// V cotangents from column c on (0 beyond the row's end).
-template <int V>
-__device__ __forceinline__ void load_cot(const float* s, int c, int experts, float (&v)[V]) {
+// Cotangents in shared memory, so that the L lanes of a row read 16 bytes each
+// side by side: vector n of V columns keeps its quarters apart, [n][V / 4][L][4].
+template <int V, int L>
+__device__ __forceinline__ int cot_place(int c) {
+  if constexpr (V <= 4) return c;
+  else return c / (V * L) * V * L + (c % V / 4 * L + c / V % L) * 4 + c % 4;
+}
+// Those of vector n of lane l.
+template <int V, int L>
+__device__ __forceinline__ void load_cot(const float* s, int n, int l, float (&v)[V]) {
   if constexpr (V >= 4) {
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
-      const float4 q = c < experts ? *reinterpret_cast<const float4*>(s + c + i)
-                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const float4 q = *reinterpret_cast<const float4*>(s + n * V * L + (i / 4 * L + l) * 4);
       v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
     }
   } else {
-    v[0] = c < experts ? s[c] : 0.0f;
+    v[0] = s[n * L + l];
   }
 }
 
@@ -146,6 +152,10 @@ struct Row {
     }
   }
   __device__ __forceinline__ float get(int i) const { return v[i / V].get(i % V); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) fill(v[n]);
+  }
   // Largest of the lane's logits (a NaN yields to a number).
   __device__ __forceinline__ float top() const {
     if constexpr (sizeof(T) == 2 && V == 8) {  // two at a time
@@ -654,7 +664,7 @@ __global__ void __launch_bounds__(kBlock) route_losses_kernel(RouteArgs a) {
 }
 
 // Shared memory, per CTA: the rows on their way out [warps][32 / L][E] and the
-// cotangents share[s, e] grad_balance [E].
+// cotangents share[s, e] grad_balance [M L] (see cot_place).
 template <typename T, int V, int NV, int L>
 __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
     route_backward_kernel(RouteArgs a) {
@@ -674,11 +684,12 @@ __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
   const int64_t t1 = min(t0 + a.tokens_per_cta, a.tokens);
 
   // What a token needs, requested one step ahead; slots l, l + L, ... of its k
-  // belong to lane l, the first of them here.
+  // belong to lane l, those of the first eight here.
+  constexpr int kMine = L >= 8 ? 1 : 8 / L;
   struct Fetch {
     RowT row;
-    float total, w, gw;
-    int slot, first;  // expert of slot l; of slot 0
+    float total, w[kMine], gw[kMine];
+    int slot[kMine], first;  // experts of the lane's slots; of slot 0
   };
   auto fetch = [&](int64_t t, int64_t hi) {
     Fetch f;
@@ -686,10 +697,14 @@ __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
     f.row.load(logits + t * E, l, E, in);
     f.total = in ? __ldg(a.denom + t) : 1.0f;
     f.first = in ? static_cast<int>(__ldg(a.chosen + t * k)) : -1;
-    const bool mine = gated && in && l < k;
-    f.slot = mine ? static_cast<int>(__ldg(a.chosen + t * k + l)) : -1;
-    f.w = mine ? __ldg(a.weights + t * k + l) : 0.0f;
-    f.gw = mine ? __ldg(a.grad_weights + t * k + l) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int j = l + i * L;
+      const bool mine = gated && in && j < k;
+      f.slot[i] = mine ? static_cast<int>(__ldg(a.chosen + t * k + j)) : -1;
+      f.w[i] = mine ? __ldg(a.weights + t * k + j) : 0.0f;
+      f.gw[i] = mine ? __ldg(a.grad_weights + t * k + j) : 0.0f;
+    }
     return f;
   };
 
@@ -701,20 +716,26 @@ __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
       continue;
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < E; c += kBlock) s_cot[c] = gb * __ldg(a.share + s * E + c);
+    for (int c = threadIdx.x; c < M * L; c += kBlock)
+      s_cot[cot_place<V, L>(c)] = c < E ? gb * __ldg(a.share + s * E + c) : 0.0f;
     __syncthreads();
     Fetch next = fetch(lo + warp * R + g, hi);
     for (int64_t base = lo + warp * R; base < hi; base += kWarpsPerBlock * R) {
       const int64_t t = base + g;
-      const Fetch f = next;
+      Fetch f = next;
       if (base + kWarpsPerBlock * R < hi) next = fetch(t + kWarpsPerBlock * R, hi);
-      const bool valid = f.first >= 0;
+      if (f.first < 0) {  // not a valid token: p = 0 everywhere
+        f.row.clear();
+        f.total = 1.0f;
+      }
       const float inv = 1.0f / f.total;
       const float top = row_max<L>(f.row.top());
       const float ref = top > -INFINITY ? top : 0.0f;
-      float along_w = f.w * f.gw;
-      if (gated && k > L && t < hi)
-        for (int j = l + L; j < k; j += L)
+      float along_w = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) along_w = fmaf(f.w[i], f.gw[i], along_w);
+      if (gated && k > kMine * L && t < hi)
+        for (int j = l + kMine * L; j < k; j += L)
           along_w += __ldg(a.weights + t * k + j) * __ldg(a.grad_weights + t * k + j);
       along_w = row_sum<L>(along_w);
       // p_e and the sum of p_e a_e; a weight that is p itself adds gw p at its expert
@@ -722,7 +743,7 @@ __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         float cot[V];
-        load_cot<V>(s_cot, (n * L + l) * V, E, cot);
+        load_cot<V, L>(s_cot, n, l, cot);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           p[n * V + i] = exp_from(f.row.get(n * V + i), ref) * inv;
@@ -736,25 +757,29 @@ __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
       for (int n = 0; n < NV; ++n) {
         const int c = (n * L + l) * V;
         float v[V];
-        load_cot<V>(s_cot, c, E, v);
+        load_cot<V, L>(s_cot, n, l, v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = valid ? p[n * V + i] * (v[i] + pull) : 0.0f;
+        for (int i = 0; i < V; ++i) v[i] = p[n * V + i] * (v[i] + pull);
         if (c < E) store_vec<V>(stage + c, v);
       }
       if (gated) {  // the chosen experts once more, with the weights' part
         __syncwarp();
-        for (int j = l; j < k; j += L) {
-          const bool head = j < L;
-          const int c = head ? f.slot : t < hi ? static_cast<int>(__ldg(a.chosen + t * k + j)) : -1;
-          if (c >= 0) {
-            const float gw = head ? f.gw : __ldg(a.grad_weights + t * k + j);
-            const float w = head ? f.w : __ldg(a.weights + t * k + j);
-            const float pe =
-                a.renormalize ? exp_from(load_f32(logits + t * E + c), ref) * inv : w;
-            store_value(stage + c, a.renormalize ? fmaf(pe, s_cot[c] + pull, w * (gw - along_w))
-                                                 : pe * (s_cot[c] + gw + pull));
+        auto fix = [&](int c, float w, float gw) {
+          const float pe = a.renormalize
+                               ? exp_from(load_f32(logits + t * E + c), ref) * inv
+                               : w;
+          const float cot = s_cot[cot_place<V, L>(c)];
+          store_value(stage + c, a.renormalize ? fmaf(pe, cot + pull, w * (gw - along_w))
+                                               : pe * (cot + gw + pull));
+        };
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+          if (f.slot[i] >= 0) fix(f.slot[i], f.w[i], f.gw[i]);
+        if (t < hi)
+          for (int j = l + kMine * L; j < k; j += L) {
+            const int c = static_cast<int>(__ldg(a.chosen + t * k + j));
+            if (c >= 0) fix(c, __ldg(a.weights + t * k + j), __ldg(a.grad_weights + t * k + j));
           }
-        }
       }
       __syncwarp();
       if (t < hi) {
@@ -771,23 +796,23 @@ __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
 }
 
 // Launch shapes by the number of experts: L lanes a token and M logits a lane.
-// Few lanes a token mean few shuffles; the forward networks take M = 32 (128
-// experts and k = 8, bfloat16: see the figures at the kernel), the other
-// kernels M = 16, which leaves registers for more warps.  Rows whose length is
+// Few lanes a token mean few shuffles: M = 32 for the networks.  The other
+// kernels take M = 16, which leaves registers for more warps (backward pass of
+// 500000 x 128 bfloat16: 87 us, 98 us with M = 32).  Rows whose length is
 // not a multiple of the vector width, or that are not aligned to 16 bytes, are
 // read one logit at a time.
 using RouteKernel = void (*)(RouteArgs);
 struct RouteShape {
   RouteKernel kernel;
-  int lanes;
+  int lanes, columns;  // of a token: lanes, and logits they hold
 };
 
 enum RoutePass { kForwardSlots, kForwardNetwork, kBackward };
 
 template <typename T, int V, int NV, int L, RoutePass P>
 RouteShape route_shape() {
-  if constexpr (P == kBackward) return {route_backward_kernel<T, V, NV, L>, L};
-  else return {route_forward_kernel<T, V, NV, L, P == kForwardNetwork ? 8 : 0>, L};
+  if constexpr (P == kBackward) return {route_backward_kernel<T, V, NV, L>, L, V * NV * L};
+  else return {route_forward_kernel<T, V, NV, L, P == kForwardNetwork ? 8 : 0>, L, V * NV * L};
 }
 
 template <typename T, RoutePass P>
@@ -996,7 +1021,7 @@ int bysj_route_backward(const void* logits, int dtype, int64_t tokens, int64_t n
   const RouteShape shape = route_pick_any(dtype, a.experts, logits, grad_logits, kBackward);
   const size_t rows = static_cast<size_t>(kWarpsPerBlock) * (kWarp / shape.lanes);
   a.stage_bytes = (rows * a.experts * (dtype == BYSJ_F32 ? 4 : 2) + 15) / 16 * 16;
-  const size_t smem = a.stage_bytes + sizeof(float) * a.experts;
+  const size_t smem = a.stage_bytes + sizeof(float) * shape.columns;
   st = allow_dynamic_smem(reinterpret_cast<const void*>(shape.kernel), smem);
   if (st) return st;
   shape.kernel<<<a.ctas, kBlock, smem, static_cast<cudaStream_t>(stream)>>>(a);
