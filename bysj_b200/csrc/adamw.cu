@@ -17,6 +17,12 @@
 // multiply-add), so a step gives the same bits as the formula evaluated one
 // operation at a time.
 //
+// 102 M float32 parameters, 32-bit states: 457 us, 28 B an element at 0.97 of the
+// measured copy bandwidth.  38.7 M bfloat16 parameters with masters and 8-bit
+// states: 159 us (18 B an element, 107 us at that bandwidth), bound by issue:
+// about 100 lane operations an element, of which the correctly rounded root and
+// quotient are a good part.  Values of 8-bit states: 72 us (59 us).
+//
 // 8-bit states.  m keeps a sign and a 7-bit magnitude with 3 mantissa bits
 // (a relative rounding of at most 1/16 down to 2^-16 of the block's
 // largest); sqrt(v) an 8-bit code with 4 mantissa bits (1/32).  The step

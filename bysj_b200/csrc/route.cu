@@ -27,6 +27,11 @@
 // such that all tokens fit 62 bits, 40 at most) and adds that to the frame's
 // total.  Integer atomics give the same sum in any order, so results repeat
 // bit for bit.
+//
+// 500000 x 128 bfloat16 logits, k = 8, renormalised: forward 94 us, bound by the
+// integer pipe of the comparators (122 warp instructions a token; the pass a slot
+// takes 217 and 168 us; HBM would need 27 us), backward 83 us, bound by issue
+// (HBM 49 us).  With an atomic for each probability the pair took 4.7 ms.
 #include "launch.cuh"
 
 namespace bysj {
