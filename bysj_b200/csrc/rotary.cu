@@ -182,8 +182,9 @@ __global__ void __launch_bounds__(kBlock, 3) rotary_kernel(RotaryArgs a) {
 #pragma unroll
             for (int i = 0; i < VP; ++i) {
               const float x1 = x.first(i), x2 = x.second(i);
-              y1[i] = x1 * cosine[i] - x2 * sine[i];
-              y2[i] = x2 * cosine[i] + x1 * sine[i];
+              // spelled out, so that every variant of the kernel gives the same bits
+              y1[i] = fmaf(x1, cosine[i], -__fmul_rn(x2, sine[i]));
+              y2[i] = fmaf(x2, cosine[i], __fmul_rn(x1, sine[i]));
               if constexpr (POS_GRAD)
                 dtheta[i] += y2[i] * saved.first(i) - y1[i] * saved.second(i);
             }

@@ -1272,6 +1272,9 @@ void adamw_step(const AdamWParams& tensors, const std::vector<OptTensor>& grads,
                           stream_of(exp_avg)),
           "adamw_step");
   }
+  // as an in-place operation: a graph that saved a parameter notices
+  for (size_t i = 0; i < params.size(); ++i)
+    if (grads[i]) params[i].unsafeGetTensorImpl()->bump_version();
 }
 
 std::tuple<Tensor, Tensor> adamw_state_values(Tensor exp_avg, Tensor exp_avg_sq,

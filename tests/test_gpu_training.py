@@ -526,6 +526,64 @@ def test_adamw_uses_parameter_gradients(cuda):
     assert p.grad is None
 
 
+# ---- alignment --------------------------------------------------------------------------
+
+def shifted(t):
+    """The same values one element past an aligned address."""
+    buffer = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    view = buffer[1:].view(t.shape)
+    view.copy_(t)
+    return view
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_unaligned_tensors_give_the_same(cuda, dtype):
+    gen = generator(31)
+    tol = half_ulp(dtype) * 2 + 64 * U
+    for rows in (40, 9000):  # one CTA, and pieces joined
+        x, g = normal(gen, rows, 64, dtype=dtype), normal(gen, rows, 64, dtype=dtype)
+        outs = []
+        for t, grad in ((x, g), (shifted(x), shifted(g))):
+            t = t.detach().requires_grad_()
+            y = K.group_norm(t[None], 8, activation="silu")
+            outs.append((y, *torch.autograd.grad(y, [t], grad[None])))
+        for a, b in zip(*outs):
+            close(a, f64(b), tol * (1.0 + np.abs(f64(b))))
+    x, g = normal(gen, 300, 128, dtype=dtype), normal(gen, 300, 8)
+    a, b = (t.detach().requires_grad_() for t in (x, shifted(x)))
+    ra, rb = K.route_experts(a, 8, renormalize=True), K.route_experts(b, 8, renormalize=True)
+    assert torch.equal(ra.experts, rb.experts) and torch.equal(ra.counts, rb.counts)
+    close(ra.weights, f64(rb.weights), 128 * U)
+    ga, = torch.autograd.grad(ra.weights, [a], g)
+    gb, = torch.autograd.grad(rb.weights, [b], g)
+    close(ga, f64(gb), 128 * U * 5 + 2 * half_ulp(dtype) * np.abs(f64(gb)))
+    q = normal(gen, 30, 4, 64, dtype=dtype)
+    pos, freq = torch.rand(30, 3, device="cuda"), torch.rand(32, device="cuda")
+    for inter in (False, True):
+        one, _ = K.rotary_axes(q, q, pos, freq, (16, 8, 8), interleaved=inter)
+        two, _ = K.rotary_axes(shifted(q), q, pos, freq, (16, 8, 8), interleaved=inter)
+        assert torch.equal(one, two)
+
+
+def test_group_norm_pieces_keep_frames_apart(cuda):
+    gen = generator(37)
+    x = normal(gen, 20000, 64)
+    given = torch.tensor([0, 7000, 7000, 7300, 20000], device="cuda")
+    first = K.group_norm(x, 8, activation="silu", offsets=given)
+    assert torch.equal(first, K.group_norm(x, 8, activation="silu", offsets=given))
+    x[7000:7300] = float("inf")
+    other = K.group_norm(x, 8, activation="silu", offsets=given)
+    assert torch.equal(other[:7000], first[:7000]) and torch.equal(other[7300:], first[7300:])
+
+
+def test_adamw_step_is_an_in_place_operation(cuda):
+    p = torch.ones(4, device="cuda", requires_grad=True)
+    loss = (p * p).sum()
+    K.AdamW([p]).step([torch.ones(4, device="cuda")])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 # ---- autograd ---------------------------------------------------------------------------
 
 def test_gradients_are_differentiable_once(cuda):
