@@ -17,11 +17,11 @@
 // multiply-add), so a step gives the same bits as the formula evaluated one
 // operation at a time.
 //
-// 102 M float32 parameters, 32-bit states: 457 us, 28 B an element at 0.97 of the
-// measured copy bandwidth.  38.7 M bfloat16 parameters with masters and 8-bit
-// states: 159 us (18 B an element, 107 us at that bandwidth), bound by issue:
+// 104.7 M float32 parameters, 32-bit states: 443 us, 28 B an element at the
+// measured copy bandwidth (448 us).  39.5 M bfloat16 parameters with masters and
+// 8-bit states: 160 us (16 B an element, 97 us at that bandwidth), bound by issue:
 // about 100 lane operations an element, of which the correctly rounded root and
-// quotient are a good part.  Values of 8-bit states: 72 us (59 us).
+// quotient are a good part.  Values of 8-bit states: 76 us (10 B, 60 us).
 //
 // 8-bit states.  m keeps a sign and a 7-bit magnitude with 3 mantissa bits
 // (a relative rounding of at most 1/16 down to 2^-16 of the block's
@@ -167,8 +167,13 @@ __device__ __forceinline__ unsigned pack4(const unsigned (&c)[4]) {
   return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 
+// Resident CTAs: with 32-bit states three leave 80 registers a thread and four 64;
+// three keep more of a lane's 16-byte loads in flight (104.7 M float32 parameters:
+// 443 against 452 us).  The 8-bit step is bound by issue and wants the warps, at
+// the price of 5 spilled registers (39.5 M bfloat16: 160 us with four, 181 with
+// three).
 template <typename T, int BITS, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kBlock, 4)
+__global__ void __launch_bounds__(kBlock, BITS == 8 ? 4 : 3)
     adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
   const int lane = lane_id();
   const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
