@@ -21,16 +21,31 @@
 // measured copy bandwidth (448 us).  39.5 M bfloat16 parameters with masters and
 // 8-bit states: 160 us (16 B an element, 97 us at that bandwidth), bound by issue:
 // about 100 lane operations an element, of which the correctly rounded root and
-// quotient are a good part.  Values of 8-bit states: 76 us (10 B, 60 us).
+// quotient are a good part.  With random rounding of sqrt(v) 202 us, of both 206
+// us: the generator's 28 multiplications for four elements.  Values of 8-bit
+// states: 76 us (10 B, 60 us).
 //
 // 8-bit states.  m keeps a sign and a 7-bit magnitude with 3 mantissa bits
 // (a relative rounding of at most 1/16 down to 2^-16 of the block's
 // largest); sqrt(v) an 8-bit code with 4 mantissa bits (1/32).  The step
 // divides by sqrt(v), so its root is what is kept: 2^-16 there spans 2^-32 of
-// v.  A positive v never becomes 0: its code is at least 1, so a rounded
-// second moment can only shorten a step, not divide by eps.  The scale is the
-// block's largest magnitude itself and value(top) = 1, so that element is
-// kept exactly and a decay by beta is carried by the scale.
+// v.  A positive v never becomes 0: its code is at least 1, so no rounding makes
+// a step divide by eps alone.  The scale is the block's largest magnitude itself
+// and value(top) = 1, so that element is kept exactly, and a decay by beta of the
+// whole block is carried by the scale.
+//
+// A step takes at most 1 - beta1 off m and (1 - beta2) / 2 off sqrt(v).  Where
+// that is less than half the gap between two codes, an element whose gradients
+// change beside others that do not would stay at its code for ever if it were
+// rounded to the nearest.  Such a moment is rounded at random instead, up with the
+// probability that keeps its mean: the code's bits plus a uniform number of one
+// unit, cut.  Random words come from a counter (the step and the element), so a
+// step repeats and resumes bit for bit.  m: where 1 - beta1 < 1/16 (half a gap is
+// up to 1/18 of m).  sqrt(v): where 1 - beta2 < 1/64; 6000 steps of random
+// gradients, half a block's changed by 0.1 or 4 after 2000, give sqrt(v) beside
+// 32-bit states within 0.84 .. 1.23 (nearest) and 0.73 .. 1.29 (random) at beta2 =
+// 0.97, 0.84 .. 1.24 and 0.74 .. 1.40 at 0.98, up to 3.6 and 1.36 at 0.99, up to
+// 9.7 and 2.2 at 0.999 (0.11 root mean square of its logarithm).
 #include "launch.cuh"
 
 namespace bysj {
@@ -61,6 +76,8 @@ struct AdamArgs {
   float* master;
   const float* grad_scale;
   bysj_adamw_hyper h;
+  uint64_t counter;            // of the step, for random rounding
+  bool random_m, random_v;     // round the moment's codes at random
 };
 
 // Kernel parameters hold 32,764 bytes; most models need far fewer entries and
@@ -122,15 +139,47 @@ __device__ __forceinline__ float value_v(unsigned word, int j, float scale) {
   return __fmul_rn(root, root);
 }
 
+// How a ratio is rounded to a code: to nearest (ties to even), or at random by a
+// 16-bit number, taken at the middle of its 2^-16.
+struct Rounding {
+  bool random;
+  unsigned r;
+  // Added below the last kept bit before the cut, in units of 2^-shift of it.
+  template <int SHIFT>
+  __device__ __forceinline__ unsigned addend(unsigned bits) const {
+    const unsigned nearest = (1u << (SHIFT - 1)) - 1u + ((bits >> SHIFT) & 1u);
+    return random ? (r << (SHIFT - 16)) | (1u << (SHIFT - 17)) : nearest;
+  }
+  // Part of the smallest code's value from which on a ratio below it takes it.
+  __device__ __forceinline__ float threshold() const {
+    return random ? static_cast<float>(131071u - 2u * r) * (1.0f / 131072.0f) : 0.5f;
+  }
+};
+
+// Four random words for the elements 4 quad .. 4 quad + 3 at step `counter`:
+// Philox 4x32 with seven rounds (Salmon, Moraes, Dror and Shaw, "Parallel random
+// numbers: as easy as 1, 2, 3", 2011).
+__device__ __forceinline__ uint4 random_words(uint64_t quad, uint64_t counter) {
+  uint4 c = make_uint4(static_cast<unsigned>(quad), static_cast<unsigned>(quad >> 32), 0u, 0u);
+  unsigned k0 = static_cast<unsigned>(counter), k1 = static_cast<unsigned>(counter >> 32);
+#pragma unroll
+  for (int round = 0; round < 7; ++round) {
+    const unsigned hi0 = __umulhi(0xd2511f53u, c.x), lo0 = 0xd2511f53u * c.x;
+    const unsigned hi1 = __umulhi(0xcd9e8d57u, c.z), lo1 = 0xcd9e8d57u * c.z;
+    c = make_uint4(hi1 ^ c.y ^ k0, lo1, hi0 ^ c.w ^ k1, lo0);
+    k0 += 0x9e3779b9u;
+    k1 += 0xbb67ae85u;
+  }
+  return c;
+}
+
 // Code of a ratio from the smallest code's value on: the bits of the float
-// rounded to MANT mantissa bits (to nearest, ties to even), counted down from
-// TOP.
+// rounded to MANT mantissa bits, counted down from TOP.
 template <int TOP, int MANT>
-__device__ __forceinline__ unsigned ratio_code(float ratio) {
+__device__ __forceinline__ unsigned ratio_code(float ratio, Rounding how) {
   constexpr int kShift = 23 - MANT;
   const unsigned bits = __float_as_uint(ratio);
-  return ((bits + ((1u << (kShift - 1)) - 1u) + ((bits >> kShift) & 1u)) >> kShift) -
-         ((127u << MANT) - TOP);
+  return ((bits + how.addend<kShift>(bits)) >> kShift) - ((127u << MANT) - TOP);
 }
 
 // Largest magnitude over the warp's block; for non-negative floats the order
@@ -152,15 +201,15 @@ __device__ __forceinline__ float inverse_scale(float scale) {
 // top code (and a NaN's block has a NaN scale, whatever its codes).
 constexpr float kLeastM = 1.25f / 65536.0f, kLeastV = 1.125f / 65536.0f;  // value(1)
 
-// Below the smallest code's value: to it or to 0, the nearer.
-__device__ __forceinline__ unsigned encode_m(float m, float inv) {
+// Below the smallest code's value: to it or to 0.
+__device__ __forceinline__ unsigned encode_m(float m, float inv, Rounding how) {
   const float ratio = fminf(__fmul_rn(fabsf(m), inv), 1.0f);
-  const unsigned code = ratio_code<kTopM, kMantM>(fmaxf(ratio, kLeastM));
-  return (ratio >= 0.5f * kLeastM ? code : 0u) | (m < 0.0f ? 128u : 0u);
+  const unsigned code = ratio_code<kTopM, kMantM>(fmaxf(ratio, kLeastM), how);
+  return (ratio >= how.threshold() * kLeastM ? code : 0u) | (m < 0.0f ? 128u : 0u);
 }
-__device__ __forceinline__ unsigned encode_v(float root, float inv) {
+__device__ __forceinline__ unsigned encode_v(float root, float inv, Rounding how) {
   const float ratio = fminf(__fmul_rn(root, inv), 1.0f);
-  const unsigned code = ratio_code<kTopV, kMantV>(fmaxf(ratio, kLeastV));
+  const unsigned code = ratio_code<kTopV, kMantV>(fmaxf(ratio, kLeastV), how);
   return root > 0.0f ? code : 0u;
 }
 __device__ __forceinline__ unsigned pack4(const unsigned (&c)[4]) {
@@ -171,9 +220,10 @@ __device__ __forceinline__ unsigned pack4(const unsigned (&c)[4]) {
 // three keep more of a lane's 16-byte loads in flight (104.7 M float32 parameters:
 // 443 against 452 us).  The 8-bit step is bound by issue and wants the warps, at
 // the price of 5 spilled registers (39.5 M bfloat16: 160 us with four, 181 with
-// three).
-template <typename T, int BITS, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kBlock, BITS == 8 ? 4 : 3)
+// three).  With random numbers it needs 72 to 78 registers and takes three.
+// RANDOM: a moment of the 8-bit states may be rounded at random.
+template <typename T, int BITS, bool MASTER, int CAP, bool RANDOM>
+__global__ void __launch_bounds__(kBlock, BITS == 8 && !RANDOM ? 4 : 3)
     adamw_kernel(const __grid_constant__ AdamArgs<CAP> a) {
   const int lane = lane_id();
   const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
@@ -278,12 +328,15 @@ __global__ void __launch_bounds__(kBlock, BITS == 8 ? 4 : 3)
 #pragma unroll
       for (int i = 0; i < kPerLane; i += 4) {
         unsigned codes_m[4], codes_v[4];
+        const int64_t at = state + element(lane, i);
+        uint4 words = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (RANDOM) words = random_words(static_cast<uint64_t>(at) / 4, a.counter);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          codes_m[j] = encode_m(m[i + j], im);
-          codes_v[j] = encode_v(root[i + j], iv);
+          const unsigned word = j == 0 ? words.x : j == 1 ? words.y : j == 2 ? words.z : words.w;
+          codes_m[j] = encode_m(m[i + j], im, {RANDOM && a.random_m, word & 0xffffu});
+          codes_v[j] = encode_v(root[i + j], iv, {RANDOM && a.random_v, word >> 16});
         }
-        const int64_t at = state + element(lane, i);
         *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.exp_avg) + at) = pack4(codes_m);
         *reinterpret_cast<unsigned*>(static_cast<uint8_t*>(a.exp_avg_sq) + at) = pack4(codes_v);
       }
@@ -330,7 +383,7 @@ __global__ void __launch_bounds__(kBlock)
   }
 }
 
-template <typename T, int BITS, bool MASTER, int CAP>
+template <typename T, int BITS, bool MASTER, int CAP, bool RANDOM>
 int launch_chunk(const bysj_adamw_tensor* tensors, int64_t count, AdamArgs<CAP>& a,
                  cudaStream_t s) {
   a.count = 0;
@@ -349,11 +402,11 @@ int launch_chunk(const bysj_adamw_tensor* tensors, int64_t count, AdamArgs<CAP>&
   int64_t blocks = (a.work_blocks + kWarpsPerBlock - 1) / kWarpsPerBlock;
   const int64_t cap = static_cast<int64_t>(current_device_info().sm_count) * 16;
   if (blocks > cap) blocks = cap;
-  adamw_kernel<T, BITS, MASTER, CAP><<<static_cast<unsigned>(blocks), kBlock, 0, s>>>(a);
+  adamw_kernel<T, BITS, MASTER, CAP, RANDOM><<<static_cast<unsigned>(blocks), kBlock, 0, s>>>(a);
   return launch_check("adamw_kernel");
 }
 
-template <typename T, int BITS, bool MASTER, int CAP>
+template <typename T, int BITS, bool MASTER, int CAP, bool RANDOM>
 int launch_all(const bysj_adamw_tensor* tensors, int64_t count, const AdamArgs<1>& base,
                cudaStream_t s) {
   AdamArgs<CAP> a;
@@ -364,43 +417,43 @@ int launch_all(const bysj_adamw_tensor* tensors, int64_t count, const AdamArgs<1
   a.master = base.master;
   a.grad_scale = base.grad_scale;
   a.h = base.h;
+  a.counter = base.counter;
+  a.random_m = base.random_m;
+  a.random_v = base.random_v;
   for (int64_t at = 0; at < count; at += CAP) {
     const int64_t part = count - at < CAP ? count - at : CAP;
-    const int st = launch_chunk<T, BITS, MASTER, CAP>(tensors + at, part, a, s);
+    const int st = launch_chunk<T, BITS, MASTER, CAP, RANDOM>(tensors + at, part, a, s);
     if (st != BYSJ_OK) return st;
   }
   return BYSJ_OK;
 }
 
+template <typename T, int BITS, bool RANDOM>
+int launch_bits(const bysj_adamw_tensor* tensors, int64_t count, const AdamArgs<1>& base,
+                cudaStream_t s) {
+  const bool small = count <= kSmallTable;
+  if (base.master != nullptr)
+    return small ? launch_all<T, BITS, true, kSmallTable, RANDOM>(tensors, count, base, s)
+                 : launch_all<T, BITS, true, kLargeTable, RANDOM>(tensors, count, base, s);
+  return small ? launch_all<T, BITS, false, kSmallTable, RANDOM>(tensors, count, base, s)
+               : launch_all<T, BITS, false, kLargeTable, RANDOM>(tensors, count, base, s);
+}
+
 template <typename T>
 int launch_type(const bysj_adamw_tensor* tensors, int64_t count, int bits,
                 const AdamArgs<1>& base, cudaStream_t s) {
-  const bool master = base.master != nullptr, small = count <= kSmallTable;
-  if (bits == 32) {
-    if (master)
-      return small ? launch_all<T, 32, true, kSmallTable>(tensors, count, base, s)
-                   : launch_all<T, 32, true, kLargeTable>(tensors, count, base, s);
-    return small ? launch_all<T, 32, false, kSmallTable>(tensors, count, base, s)
-                 : launch_all<T, 32, false, kLargeTable>(tensors, count, base, s);
-  }
-  if (master)
-    return small ? launch_all<T, 8, true, kSmallTable>(tensors, count, base, s)
-                 : launch_all<T, 8, true, kLargeTable>(tensors, count, base, s);
-  return small ? launch_all<T, 8, false, kSmallTable>(tensors, count, base, s)
-               : launch_all<T, 8, false, kLargeTable>(tensors, count, base, s);
+  if (bits == 32) return launch_bits<T, 32, false>(tensors, count, base, s);
+  return base.random_m || base.random_v ? launch_bits<T, 8, true>(tensors, count, base, s)
+                                        : launch_bits<T, 8, false>(tensors, count, base, s);
 }
 
-}  // namespace
-}  // namespace bysj
+// Moments of 8-bit states that a step moves by less than half a code.
+constexpr float kSlowM = 1.0f / 16.0f, kSlowV = 1.0f / 64.0f;
 
-using namespace bysj;
-
-extern "C" {
-
-int bysj_adamw_step(const bysj_adamw_tensor* tensors, int64_t n_tensors, int dtype,
-                    int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
-                    float* exp_avg_sq_scale, float* master, const float* grad_scale,
-                    const bysj_adamw_hyper* hyper, void* stream) {
+int adamw_step(const bysj_adamw_tensor* tensors, int64_t n_tensors, int dtype, int state_bits,
+               void* exp_avg, void* exp_avg_sq, float* exp_avg_scale, float* exp_avg_sq_scale,
+               float* master, const float* grad_scale, const bysj_adamw_hyper* hyper,
+               const uint64_t* counter, void* stream) {
   clear_error();
   if (dtype != BYSJ_F32 && dtype != BYSJ_BF16)
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw: unknown dtype %d", dtype);
@@ -422,6 +475,14 @@ int bysj_adamw_step(const bysj_adamw_tensor* tensors, int64_t n_tensors, int dty
       (state_bits == 8 && (exp_avg_scale == nullptr || exp_avg_sq_scale == nullptr)))
     return fail(BYSJ_ERR_INVALID_ARGUMENT, "adamw: NULL state");
   AdamArgs<1> base{};
+  if (state_bits == 8) {
+    base.random_m = hyper->one_minus_beta1 < kSlowM;
+    base.random_v = hyper->one_minus_beta2 < kSlowV;
+    if ((base.random_m || base.random_v) && counter == nullptr)
+      return fail(BYSJ_ERR_INVALID_ARGUMENT,
+                  "adamw: 8-bit states at these betas need bysj_adamw_step_counted");
+  }
+  if (counter != nullptr) base.counter = *counter;
   base.exp_avg = exp_avg;
   base.exp_avg_sq = exp_avg_sq;
   base.exp_avg_scale = exp_avg_scale;
@@ -432,6 +493,30 @@ int bysj_adamw_step(const bysj_adamw_tensor* tensors, int64_t n_tensors, int dty
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == BYSJ_F32 ? launch_type<float>(tensors, n_tensors, state_bits, base, s)
                            : launch_type<__nv_bfloat16>(tensors, n_tensors, state_bits, base, s);
+}
+
+}  // namespace
+}  // namespace bysj
+
+using namespace bysj;
+
+extern "C" {
+
+int bysj_adamw_step(const bysj_adamw_tensor* tensors, int64_t n_tensors, int dtype,
+                    int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
+                    float* exp_avg_sq_scale, float* master, const float* grad_scale,
+                    const bysj_adamw_hyper* hyper, void* stream) {
+  return adamw_step(tensors, n_tensors, dtype, state_bits, exp_avg, exp_avg_sq, exp_avg_scale,
+                    exp_avg_sq_scale, master, grad_scale, hyper, nullptr, stream);
+}
+
+int bysj_adamw_step_counted(const bysj_adamw_tensor* tensors, int64_t n_tensors, int dtype,
+                            int state_bits, void* exp_avg, void* exp_avg_sq,
+                            float* exp_avg_scale, float* exp_avg_sq_scale, float* master,
+                            const float* grad_scale, const bysj_adamw_hyper* hyper,
+                            uint64_t counter, void* stream) {
+  return adamw_step(tensors, n_tensors, dtype, state_bits, exp_avg, exp_avg_sq, exp_avg_scale,
+                    exp_avg_sq_scale, master, grad_scale, hyper, &counter, stream);
 }
 
 int bysj_adamw_state_values(const uint8_t* exp_avg, const uint8_t* exp_avg_sq,

@@ -1210,7 +1210,7 @@ struct AdamWParams {
 void adamw_step(const AdamWParams& tensors, const std::vector<OptTensor>& grads, Tensor exp_avg,
                 Tensor exp_avg_sq, OptTensor exp_avg_scale, OptTensor exp_avg_sq_scale,
                 OptTensor master, OptTensor grad_scale, double beta1, double beta2, double decay,
-                double size, double correct, double eps) {
+                double size, double correct, double eps, int64_t step) {
   const std::vector<Tensor>& params = tensors.params;
   const std::vector<int64_t>& begins = tensors.begins;
   TORCH_CHECK(params.size() == grads.size(),
@@ -1262,14 +1262,14 @@ void adamw_step(const AdamWParams& tensors, const std::vector<OptTensor>& grads,
   c10::cuda::CUDAGuard guard(exp_avg.device());
   for (int i = 0; i < 2; ++i) {
     if (table[i].empty()) continue;
-    check(bysj_adamw_step(table[i].data(), static_cast<int64_t>(table[i].size()),
-                          i ? BYSJ_BF16 : BYSJ_F32, bytes ? 8 : 32, exp_avg.data_ptr(),
-                          exp_avg_sq.data_ptr(),
-                          bytes ? exp_avg_scale->data_ptr<float>() : nullptr,
-                          bytes ? exp_avg_sq_scale->data_ptr<float>() : nullptr,
-                          master ? master->data_ptr<float>() : nullptr,
-                          grad_scale ? grad_scale->data_ptr<float>() : nullptr, &hyper,
-                          stream_of(exp_avg)),
+    check(bysj_adamw_step_counted(table[i].data(), static_cast<int64_t>(table[i].size()),
+                                  i ? BYSJ_BF16 : BYSJ_F32, bytes ? 8 : 32, exp_avg.data_ptr(),
+                                  exp_avg_sq.data_ptr(),
+                                  bytes ? exp_avg_scale->data_ptr<float>() : nullptr,
+                                  bytes ? exp_avg_sq_scale->data_ptr<float>() : nullptr,
+                                  master ? master->data_ptr<float>() : nullptr,
+                                  grad_scale ? grad_scale->data_ptr<float>() : nullptr, &hyper,
+                                  static_cast<uint64_t>(step), stream_of(exp_avg)),
           "adamw_step");
   }
   // as an in-place operation: a graph that saved a parameter notices

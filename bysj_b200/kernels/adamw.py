@@ -34,9 +34,15 @@ class AdamW:
     ``weight_decay`` are plain attributes, so a schedule may assign them
     between steps.  ``state_bits``: 32, or 8 for one byte per element and
     moment: the first as sign and 7-bit magnitude, the root of the second in 8
-    bits, both relative to the largest of 256 elements (rounding errors of at
-    most 1/16 and 1/32 of a value).  A non-finite gradient makes the moments
-    of its whole block NaN there, of its element alone with 32 bits.
+    bits, both relative to the largest of 256 elements.  A step rounds them to
+    the nearest code (errors of at most 1/16 and 1/32 of a value).  A moment
+    that a step moves by less than half a code (``beta1 > 15/16``, ``beta2 >
+    63/64``, as the default) is rounded at random without bias instead, so
+    that it keeps following its gradients; the root of the second moment then
+    differs from that of 32-bit states by about 11 % root mean square.  The
+    random numbers come from the step and the element: equal runs give equal
+    bits.  A non-finite gradient makes the moments of its whole block NaN
+    there, of its element alone with 32 bits.
     ``master_weights`` keeps float32 weights beside the parameters;
     call :meth:`sync_master` after assigning parameters by hand.
 
@@ -128,7 +134,7 @@ class AdamW:
             self._tensors, grads, self.exp_avg, self.exp_avg_sq, self.exp_avg_scale,
             self.exp_avg_sq_scale, self.master, grad_scale, beta1, beta2,
             1.0 - self.lr * self.weight_decay, self.lr / (1.0 - beta1 ** step),
-            1.0 / math.sqrt(1.0 - beta2 ** step), self.eps)
+            1.0 / math.sqrt(1.0 - beta2 ** step), self.eps, step)
         self.step_count = step
 
     def zero_grad(self) -> None:

@@ -586,6 +586,12 @@ BYSJ_API int bysj_route_backward(const void* logits, int dtype, int64_t tokens,
  * code c > 0 stands for scale * value(c), value(top) = 1, each step one unit
  * in the last mantissa bit (value = float with the bits
  * (c - top + (127 << mantissa)) << (23 - mantissa)); code 0 for 0.
+ * A moment whose decay a step is less than half a code (8-bit states with
+ * one_minus_beta1 < 1/16 or one_minus_beta2 < 1/64) would stop following its
+ * gradients if it were rounded to the nearest code: bysj_adamw_step refuses
+ * such values (BYSJ_ERR_INVALID_ARGUMENT).  bysj_adamw_step_counted rounds that
+ * moment's codes at random without bias, by a generator of `counter` and the
+ * element: pass the number of the step.  Otherwise the two are the same.
  * tensors is read on the host. */
 #define BYSJ_ADAMW_BLOCK 256
 typedef struct bysj_adamw_tensor {
@@ -606,6 +612,12 @@ BYSJ_API int bysj_adamw_step(const bysj_adamw_tensor* tensors, int64_t n_tensors
                              float* exp_avg_scale, float* exp_avg_sq_scale, float* master,
                              const float* grad_scale, const bysj_adamw_hyper* hyper,
                              void* stream);
+BYSJ_API int bysj_adamw_step_counted(const bysj_adamw_tensor* tensors, int64_t n_tensors,
+                                     int dtype, int state_bits, void* exp_avg, void* exp_avg_sq,
+                                     float* exp_avg_scale, float* exp_avg_sq_scale,
+                                     float* master, const float* grad_scale,
+                                     const bysj_adamw_hyper* hyper, uint64_t counter,
+                                     void* stream);
 /* The float32 values that 8-bit states stand for (blocks * BYSJ_ADAMW_BLOCK
  * elements each): m = scale value, v = (scale value)^2. */
 BYSJ_API int bysj_adamw_state_values(const uint8_t* exp_avg, const uint8_t* exp_avg_sq,

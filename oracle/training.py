@@ -178,16 +178,54 @@ def adamw_f32(p, g, m, v, step, lr, betas, eps, weight_decay, grad_scale=None):
     return p, m, v, root
 
 
-def encode(x, top, values):
+def philox4x32(counter, key, rounds):
+    """Philox 4x32 (Salmon et al., 2011) of counters [n, 4] and one 64-bit key."""
+    c = [np.asarray(counter, np.uint64)[:, i] for i in range(4)]
+    low = np.uint64(0xFFFFFFFF)
+    k = [key & 0xFFFFFFFF, key >> 32]
+    for _ in range(rounds):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> np.uint64(32)) ^ c[1] ^ np.uint64(k[0]), b & low,
+             (a >> np.uint64(32)) ^ c[3] ^ np.uint64(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return np.stack(c, 1)
+
+
+def rounding_noise(step, length, betas):
+    """Numbers in (0, 1) that round the codes of m and of sqrt(v) at ``step``, [length / BLOCK, BLOCK].
+
+    ``None`` for a moment that a step decays by at least half a code, which
+    is rounded to the nearest.
+    """
+    quads = np.zeros((length // 4, 4), np.uint64)
+    quads[:, 0] = np.arange(length // 4)
+    words = philox4x32(quads, step, 7).reshape(-1, BLOCK)
+    noise = [((words >> np.uint64(16 * i) & np.uint64(0xFFFF)) + 0.5) / 65536.0 for i in range(2)]
+    return [n if 1.0 - beta < least else None
+            for n, beta, least in zip(noise, betas, (1 / 16, 1 / 64))]
+
+
+def encode(x, top, values, noise=None):
     """Codes of non-negative float32 blocks [n, BLOCK] by nearest value, and their scales.
 
     A tie goes to the even mantissa (the odd code: the top code is odd).  The
-    ratio is the float32 product with the float32 inverse of the scale.
+    ratio is the float32 product with the float32 inverse of the scale.  With
+    ``noise`` in (0, 1) a ratio between two values takes the upper one where
+    the part of the gap above it does not exceed the noise.
     """
     scale = x.max(1)
     with np.errstate(divide="ignore"):
         inverse = np.where(scale > 0, np.float32(1.0) / scale, np.float32(0.0)).astype(np.float32)
     ratio = (x * inverse[:, None]).astype(np.float64)
+    if noise is not None:
+        ratio = np.minimum(ratio, 1.0)
+        lower = np.searchsorted(values, ratio, side="right") - 1
+        upper = np.minimum(lower + 1, top)
+        gap = np.where(upper > lower, values[upper] - values[lower], 1.0)
+        code = np.where((ratio - values[lower]) / gap + noise >= 1.0, upper, lower)
+        if top == 255:
+            code = np.where(x > 0, np.maximum(code, 1), 0)
+        return code.astype(np.uint8), scale
     middle = (values[1:] + values[:-1]) / 2
     code = np.searchsorted(middle, ratio, side="left")
     tie = (code < top) & (ratio == middle[np.minimum(code, top - 1)]) & (code % 2 == 0)
@@ -202,4 +240,5 @@ def decode(code, scale, values):
 
 
 __all__ = ["BLOCK", "VALUES_M", "VALUES_V", "adamw", "adamw_f32", "code_values", "decode",
-           "encode", "group_norm", "rotary", "rotary_position_grad", "route"]
+           "encode", "group_norm", "philox4x32", "rotary", "rotary_position_grad",
+           "rounding_noise", "route"]

@@ -1,0 +1,146 @@
+"""Training-step operators where they can go wrong, on the GPU (B200).
+
+Long runs of the optimizer, outliers and infinities, masked places that hold
+anything, and launch shapes that only large or many-framed inputs take.
+Tolerances are derived at each test; ``U`` and ``B`` are the unit roundoffs of
+float32 and bfloat16.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from bysj_b200 import kernels as K  # noqa: E402
+from oracle import training as O  # noqa: E402
+
+U, B = torch.finfo(torch.float32).eps / 2, torch.finfo(torch.bfloat16).eps / 2
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def close(got, want, tol):
+    got = f64(got) if isinstance(got, torch.Tensor) else got
+    assert got.shape == want.shape
+    worst = np.max(np.abs(got - want) - tol) if got.size else -1.0
+    assert worst <= 0.0, f"off by {worst} beyond the tolerance"
+
+
+def normal(gen, *shape, dtype=F32, scale=1.0):
+    return (torch.randn(*shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+def generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+# ---- AdamW: 8-bit states over many steps -------------------------------------------------
+
+@pytest.mark.parametrize("before,after", [(1.0, 0.1), (1.0, 4.0), (0.05, 0.2)])
+def test_adamw_8bit_second_moment_follows_at_the_default_betas(cuda, before, after):
+    """sqrt(v) of 8-bit states stays near that of 32-bit states while half a block's gradients change.
+
+    A step moves sqrt(v) by (1 - beta2) / 2 = 0.05 % of it at most (downwards), against gaps of 1/31 to
+    1/16 between codes.  Rounded at random without bias, a step adds a variance of its move times the
+    gap: over s steps at most s * 0.0005 / 16 to log sqrt(v) where nothing renews it (4000 steps here:
+    0.35^2), 0.12^2 where gradients do.  Means over 8192 elements stay within the gap's second-order
+    effect (1/32) and the skew of the logarithm (0.35^2 / 2).
+    """
+    gen, n = generator(41), 64 * 256
+    size = torch.ones(64, 256, device="cuda")
+    params = [torch.zeros(n, device="cuda") for _ in range(2)]
+    byte, full = K.AdamW(params[:1], state_bits=8), K.AdamW(params[1:])
+    for step in range(6000):
+        if step in (0, 2000):
+            size[:, 128:] = after if step else before
+        g = normal(gen, 64, 256).mul_(size).view(-1)
+        byte.step([g])
+        full.step([g])
+    ratio = (byte.state_values()[1].sqrt() / full.exp_avg_sq.sqrt()).view(64, 256).log()
+    for part in (ratio[:, :128], ratio[:, 128:]):
+        assert float(part.square().mean().sqrt()) < 0.35 + 0.05
+        assert abs(float(part.mean())) < 0.35 ** 2 / 2 + 1 / 32
+    # the first moment is exact to its codes: 1/16 a step, renewed by a tenth
+    m = byte.state_values()[0] - full.exp_avg
+    assert float(m.square().mean().sqrt()) < 0.1 * float(full.exp_avg.square().mean().sqrt())
+
+
+def test_adamw_8bit_first_moment_decays_when_its_gradients_stop(cuda):
+    """At beta1 = 0.95 a step takes 5 % off m, less than half the gap between codes 8 and 9.
+
+    After 400 steps without a gradient m is 0.95^400 = 1.2e-9 of what it was; rounding without bias
+    keeps that mean, so of 8192 elements one above 1e-3 has a probability of 1e-2.
+    """
+    gen, n = generator(43), 64 * 256
+    opt = K.AdamW([torch.zeros(n, device="cuda")], betas=(0.95, 0.95), state_bits=8)
+    g = normal(gen, 64, 256)
+    for step in range(450):
+        if step == 50:
+            g[:, 128:] = 0.0
+        opt.step([g.view(-1)])
+    m = opt.state_values()[0].view(64, 256)
+    assert float(m[:, 128:].abs().max()) < 1e-3
+    # the others keep their constant gradient: within a gap of it
+    close(m[:, :128], f64(g[:, :128]), f64(g[:, :128].abs()) / 8 + 2.0 ** -16 * 5)
+
+
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.95, 0.95), (0.97, 0.9999)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_adamw_8bit_random_rounding_bit_for_bit(cuda, betas, dtype):
+    gen, sizes = generator(47), [(700,), (1,), (3, 256), (0,), (31, 33)]
+    hyper = dict(lr=0.01, betas=betas, eps=1e-8, weight_decay=0.1)
+    params = [normal(gen, *s, dtype=dtype) for s in sizes]
+    opt = K.AdamW(params, **hyper, state_bits=8, master_weights=dtype == BF16)
+    length = opt.exp_avg.numel()
+
+    def packed(tensors):
+        out = np.zeros(length, np.float32)
+        for t, begin in zip(tensors, opt.begins):
+            out[begin:begin + t.numel()] = t.detach().float().cpu().numpy().reshape(-1)
+        return out
+
+    p, m, v = packed(params), np.zeros(length, np.float32), np.zeros(length, np.float32)
+    for step in range(1, 5):
+        grads = [normal(gen, *s, dtype=dtype) for s in sizes]
+        if step == 2:
+            for g in grads:
+                g.mul_(torch.exp(normal(gen, *g.shape, scale=5.0)).to(dtype))
+                g[..., ::3] = 0.0
+        opt.step(grads)
+        p, m, v, root = O.adamw_f32(p, packed(grads), m, v, step, **hyper)
+        noise_m, noise_v = O.rounding_noise(step, length, betas)
+        whole = m.reshape(-1, O.BLOCK)
+        code, scale = O.encode(np.abs(whole), 127, O.VALUES_M, noise_m)
+        np.testing.assert_array_equal(
+            opt.exp_avg.cpu().numpy(),
+            np.where(whole < 0, code + 128, code).astype(np.uint8).reshape(-1))
+        m = (np.where(whole < 0, -1, 1) * O.decode(code, scale, O.VALUES_M)).astype(
+            np.float32).reshape(-1)
+        code, scale = O.encode(root.reshape(-1, O.BLOCK), 255, O.VALUES_V, noise_v)
+        np.testing.assert_array_equal(opt.exp_avg_sq.cpu().numpy(), code.reshape(-1))
+        v = O.decode(code, scale, O.VALUES_V).reshape(-1) ** 2
+        for t, begin in zip(params, opt.begins):
+            part = torch.from_numpy(p[begin:begin + t.numel()])
+            assert torch.equal(t.cpu().reshape(-1), part.to(dtype))
+
+
+def test_adamw_8bit_random_rounding_repeats_and_resumes(cuda):
+    gen = generator(53)
+    start, grads = normal(gen, 1000), [normal(gen, 1000) for _ in range(6)]
+    one, two = start.clone(), start.clone()
+    a = K.AdamW([one], state_bits=8)
+    for g in grads:
+        a.step([g])
+    b = K.AdamW([two], state_bits=8)
+    for g in grads[:3]:
+        b.step([g])
+    c = K.AdamW([two], state_bits=8)
+    c.load_state_dict(b.state_dict())
+    for g in grads[3:]:
+        c.step([g])
+    assert torch.equal(one, two) and torch.equal(a.exp_avg_sq, c.exp_avg_sq)
