@@ -828,6 +828,17 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors,
   return false;
 }
 
+// A tangent would be dropped, which reads as a derivative of zero.
+void refuse_tangents(const char* op, std::initializer_list<const Tensor*> tensors,
+                     std::initializer_list<const OptTensor*> optional) {
+  const auto check_one = [op](const Tensor& t) {
+    TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), op, " has no forward-mode derivative");
+  };
+  for (const Tensor* t : tensors) check_one(*t);
+  for (const OptTensor* t : optional)
+    if (t->has_value()) check_one(**t);
+}
+
 // Gradients that cannot be differentiated again: with create_graph, an attempt
 // to go through them raises.
 variable_list once(variable_list grads, const char* op) {
@@ -949,6 +960,7 @@ class RotaryFunction : public torch::autograd::Function<RotaryFunction> {
 std::tuple<Tensor, Tensor> rotary_axes(const Tensor& q, const Tensor& k, const Tensor& positions,
                                        const Tensor& inv_freq,
                                        const std::vector<int64_t>& sections, bool interleaved) {
+  refuse_tangents("rotary_axes", {&q, &k, &positions, &inv_freq}, {});
   if (!wants_grad({&q, &k, &positions}, {})) {
     auto [yq, yk, none] = rotary_turn(q, k, positions, inv_freq, sections, interleaved, false,
                                       std::nullopt, std::nullopt);
@@ -1073,6 +1085,7 @@ class GroupNormFunction : public torch::autograd::Function<GroupNormFunction> {
 Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight,
                   const OptTensor& bias, double eps, int64_t activation,
                   const OptTensor& offsets) {
+  refuse_tangents("group_norm", {&x}, {&weight, &bias});
   if (!wants_grad({&x}, {&weight, &bias}))
     return std::get<0>(group_norm_forward(x, groups, weight, bias, eps, activation, offsets));
   return GroupNormFunction::apply(x, weight, bias, offsets, groups, eps, activation);
@@ -1184,6 +1197,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_experts(const Tensor& l
                                                                  const OptTensor& mask,
                                                                  const OptTensor& offsets,
                                                                  bool renormalize) {
+  refuse_tangents("route_experts", {&logits}, {});
   if (!wants_grad({&logits}, {})) {
     const Routed r = route_forward(logits, k, mask, offsets, renormalize);
     return {r.weights, r.experts, r.counts, r.balance, r.z};

@@ -144,3 +144,40 @@ def test_adamw_8bit_random_rounding_repeats_and_resumes(cuda):
     for g in grads[3:]:
         c.step([g])
     assert torch.equal(one, two) and torch.equal(a.exp_avg_sq, c.exp_avg_sq)
+
+
+# ---- derivatives other than backward ---------------------------------------------------------
+
+def operator_calls(gen):
+    x = normal(gen, 40, 8)
+    q, pos, freq = normal(gen, 5, 2, 8), torch.rand(5, 2, device="cuda"), torch.rand(4, device="cuda")
+    w = torch.ones(8, device="cuda")
+    return [
+        (lambda t: K.group_norm(t, 2, w), x),
+        (lambda t: K.group_norm(x, 2, t, t), w),
+        (lambda t: K.route_experts(t, 2).weights, x),
+        (lambda t: K.rotary_axes(t, q, pos, freq, (2, 2))[0], q),
+        (lambda t: K.rotary_axes(q, t, pos, freq, (2, 2))[1], q),
+        (lambda t: K.rotary_axes(q, None, t, freq, (2, 2))[0], pos),
+        (lambda t: K.rotary_axes(q, None, pos, t, (2, 2))[0], freq),
+    ]
+
+
+@pytest.mark.parametrize("grad_enabled", [True, False])
+def test_forward_mode_derivatives_are_refused(cuda, grad_enabled):
+    import torch.autograd.forward_ad as fwd
+
+    for call, x in operator_calls(generator(59)):
+        with fwd.dual_level(), torch.set_grad_enabled(grad_enabled):
+            dual = fwd.make_dual(x, torch.ones_like(x))
+            with pytest.raises(RuntimeError, match="jvp|forward-mode"):
+                call(dual)
+
+
+def test_function_transforms_are_refused(cuda):
+    for call, x in operator_calls(generator(61)):
+        for transform in (lambda f: torch.func.vmap(f)(x[None]),
+                          lambda f: torch.func.jvp(f, (x,), (torch.ones_like(x),)),
+                          lambda f: torch.func.grad(lambda t: f(t).sum())(x)):
+            with pytest.raises(RuntimeError):
+                transform(call)
