@@ -22,9 +22,11 @@
 //
 // Sums are float32, of a few tens of terms at a time (rows of a thread, threads
 // of a channel, pieces of a frame), so their rounding does not grow with the
-// rows; float64 arithmetic cost tens of microseconds a kernel here.  Squares are
-// taken about a value near the mean, which costs the variance no digits
-// wherever the mean lies.  No atomics: results repeat bit for bit.
+// rows; float64 arithmetic cost tens of microseconds a kernel here.  The variance
+// loses no digits to outliers or to channels that lie apart: a thread takes
+// squares about the mean of its own rows nearby, and means and squares of threads,
+// pieces and channels are joined as such, where only squares add.  No atomics:
+// results repeat bit for bit.
 //
 // Bound by HBM in the results, by instruction issue and loads in flight in the
 // statistics.  16 frames of 24576 x 128 bfloat16 with SiLU: forward 34 us
@@ -173,10 +175,10 @@ struct Rows {
 };
 
 // use(a, b) for n rows of a thread in order, the next kRows requested before
-// the last ones are used.
-template <typename T, int VEC, bool TWO, int BYTES, typename Use>
+// the last ones are used, which batch(rows, their number) sees first.
+template <typename T, int VEC, bool TWO, int BYTES, typename Batch, typename Use>
 __device__ __forceinline__ void each_row(const T* pa, const T* pb, int64_t step, int64_t n,
-                                         Use use) {
+                                         Batch batch, Use use) {
   using RowsT = Rows<T, VEC, TWO, BYTES>;
   constexpr int kRows = RowsT::kRows;
   const int rest = static_cast<int>(n % kRows);
@@ -193,9 +195,11 @@ __device__ __forceinline__ void each_row(const T* pa, const T* pb, int64_t step,
     const RowsT now = next;
     if (n >= 2 * kRows) next.load(pa, pb, step);
     else next.load(pa, pb, step, rest);
+    batch(now, kRows);
 #pragma unroll
     for (int j = 0; j < kRows; ++j) apply(now, j);
   }
+  if (rest > 0) batch(next, rest);
 #pragma unroll
   for (int j = 0; j < kRows - 1; ++j)
     if (j < rest) apply(next, j);
@@ -260,14 +264,17 @@ struct Columns {
   }
 };
 
-// A channel's pair from its sums over `rows` rows; forward sums are about the
-// pivot.
-template <bool BACKWARD>
-__device__ __forceinline__ float2 channel_value(float s1, float s2, int64_t rows, float pivot) {
-  if constexpr (BACKWARD) return make_float2(s1, s2);
-  const float mean = s1 / static_cast<float>(rows);
-  return make_float2(pivot + mean, fmaxf(fmaf(-s1, mean, s2), 0.0f));
-}
+// Number, mean and sum of squares about the mean of some values.  Joining two of
+// them only adds squares, so no digits cancel wherever the means lie.
+struct Moments {
+  float n = 0.0f, mean = 0.0f, m2 = 0.0f;
+  __device__ __forceinline__ void join(const Moments& o) {
+    const float sum = n + o.n, part = o.n > 0.0f ? __fdividef(o.n, sum) : 0.0f, d = o.mean - mean;
+    mean = fmaf(d, part, mean);
+    m2 += fmaf(d * (n * part), d, o.m2);  // d first: its square may overflow beside n = 0
+    n = sum;
+  }
+};
 
 // Adds n terms term(i) for i = first, first + step, ...: eight at a time, the
 // eights then to the sum, so that the rounding grows with n / 8 + 8 terms.
@@ -288,28 +295,67 @@ __device__ __forceinline__ void add_terms(int first, int n, int step, float& s1,
   }
 }
 
+// Terms of a thread's inner sums before they join the outer ones; a multiple of
+// the rows that each_row takes at a time.
+constexpr int kInner = 64;
+
 // Channel sums over a slab's rows into chan[] (forward: mean and the sum of
 // squares about it; backward: sum dz, sum dz xhat).  Ends synchronised.
+//
+// Forward: a thread sums kInner rows at a time about a pivot, the mean of its rows
+// before them; they move the pivot by off = s1 / rows so far, and what squares about
+// the old pivot exceed those about the new one is s1 off.  The first pivot is the
+// mean of the first batch of rows (of four or eight: an outlier there enters it by a
+// quarter or less, so that squares cancel by a factor of 5 at most).
 template <typename T, int VEC, int THREADS, bool BACKWARD, int ACT>
 __device__ __forceinline__ void column_stats(const Tile<VEC, THREADS>& t, const T* x, const T* dy,
                                              int64_t rows, int channels, const Columns<VEC>& q,
                                              float* scratch, float2* level, float2* chan) {
-  float s1[VEC], s2[VEC], pivot[VEC], o1[VEC], o2[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = o1[i] = o2[i] = pivot[i] = 0.0f;
   if (t.on) {
-    if constexpr (!BACKWARD) {  // about the mean of the first rows
-      const int count = rows < 4 ? static_cast<int>(rows) : 4;
-      for (int r = 0; r < count; ++r) {
-        float v[VEC];
-        load_vec<VEC>(x + r * static_cast<int64_t>(channels) + t.c, v);
+    float s1[VEC], s2[VEC], o1[VEC], o2[VEC];  // inner and outer sums; forward: o1 is the pivot
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) pivot[i] += v[i];
+    for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = o1[i] = o2[i] = 0.0f;
+    const int64_t step = static_cast<int64_t>(t.ty) * channels;
+    const T* px = x + t.ry * static_cast<int64_t>(channels) + t.c;
+    const T* pg = dy + t.ry * static_cast<int64_t>(channels) + t.c;
+    const int64_t n = rows > t.ry ? (rows - t.ry + t.ty - 1) / t.ty : 0;  // of this thread
+    int terms = 0;      // of the inner sums
+    float done = 0.0f;  // forward: rows of the outer ones
+    auto flush = [&] {
+      done += static_cast<float>(terms);
+      const float inv = 1.0f / done;
+      terms = 0;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if constexpr (BACKWARD) {
+          o1[i] += s1[i];
+          o2[i] += s2[i];
+        } else {
+          const float off = s1[i] * inv;
+          o1[i] += off;
+          o2[i] += fmaf(-s1[i], off, s2[i]);
+        }
+        s1[i] = s2[i] = 0.0f;
       }
+    };
+    auto batch = [&](const auto& now, int count) {
+      if constexpr (BACKWARD) return;
+      if (terms == 0) {  // the first of all
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) pivot[i] /= static_cast<float>(count);
-    }
-    auto add = [&](const float (&v)[VEC], const float (&g)[VEC]) {
+        for (int j = 0; j < now.kRows; ++j) {
+          if (j >= count) continue;
+          float v[VEC];
+          now.a[j].get(v);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) o1[i] += v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o1[i] /= static_cast<float>(count);
+      }
+      if (terms == kInner) flush();
+      terms += count;
+    };
+    each_row<T, VEC, BACKWARD, BACKWARD ? 128 : 64>(px, pg, step, n, batch, [&](const float(&v)[VEC], const float(&g)[VEC]) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         if constexpr (BACKWARD) {
@@ -318,67 +364,69 @@ __device__ __forceinline__ void column_stats(const Tile<VEC, THREADS>& t, const 
           s1[i] += dz;
           s2[i] = fmaf(dz, xhat, s2[i]);
         } else {
-          const float d = v[i] - pivot[i];
+          const float d = v[i] - o1[i];
           s1[i] += d;
           s2[i] = fmaf(d, d, s2[i]);
         }
       }
-    };
-    const int64_t step = static_cast<int64_t>(t.ty) * channels;
-    const T* px = x + t.ry * static_cast<int64_t>(channels) + t.c;
-    const T* pg = dy + t.ry * static_cast<int64_t>(channels) + t.c;
-    const int64_t n = rows > t.ry ? (rows - t.ry + t.ty - 1) / t.ty : 0;  // of this thread
-    int left = 64;  // terms of the inner sums before they join the outer ones
-    each_row<T, VEC, BACKWARD, BACKWARD ? 128 : 64>(px, pg, step, n, [&](const float(&v)[VEC], const float(&g)[VEC]) {
-      add(v, g);
-      if (--left > 0) return;
-      left = 64;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        o1[i] += s1[i];
-        o2[i] += s2[i];
-        s1[i] = s2[i] = 0.0f;
-      }
+      if constexpr (BACKWARD)
+        if (++terms == kInner) flush();
     });
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      s1[i] += o1[i];
-      s2[i] += o2[i];
-    }
+    if (terms > 0) flush();
     float* place = scratch + t.ry * t.width + t.c - t.c0;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      place[i] = s1[i];
-      place[THREADS * VEC + i] = s2[i];
-      if (t.ry == 0) chan[t.c + i].x = pivot[i];
+      place[i] = o1[i];
+      place[THREADS * VEC + i] = o2[i];
     }
   }
   __syncthreads();
   // THREADS / width parts of the rows side by side, then the parts in order
   const int parts = t.width < THREADS ? THREADS / t.width : 1;
   const int share = (t.ty + parts - 1) / parts;
+  // forward: rows of thread row r, and of all before it
+  const int64_t each = rows / t.ty;
+  const int more = static_cast<int>(rows - each * t.ty);
+  const auto before = [&](int r) { return each * r + min(r, more); };
   for (int i = threadIdx.x; i < parts * t.width; i += THREADS) {
     const int part = i / t.width, c = i - part * t.width;
-    float a1 = 0.0f, a2 = 0.0f;
-    for (int r = part * share; r < min((part + 1) * share, t.ty); ++r) {
-      a1 += scratch[r * t.width + c];
-      a2 += scratch[THREADS * VEC + r * t.width + c];
-    }
-    if (parts > 1) {
-      level[i] = make_float2(a1, a2);
+    const int end = min((part + 1) * share, t.ty);
+    float2 v;
+    if constexpr (BACKWARD) {
+      v = make_float2(0.0f, 0.0f);
+      for (int r = part * share; r < end; ++r) {
+        v.x += scratch[r * t.width + c];
+        v.y += scratch[THREADS * VEC + r * t.width + c];
+      }
     } else {
-      chan[t.c0 + c] = channel_value<BACKWARD>(a1, a2, rows, chan[t.c0 + c].x);
+      Moments m;
+      for (int r = part * share; r < end; ++r)
+        m.join({static_cast<float>(r < more ? each + 1 : each), scratch[r * t.width + c],
+                scratch[THREADS * VEC + r * t.width + c]});
+      v = make_float2(m.mean, m.m2);
     }
+    if (parts > 1) level[i] = v;
+    else chan[t.c0 + c] = v;
   }
   __syncthreads();
   if (parts > 1) {
     for (int c = threadIdx.x; c < t.width; c += THREADS) {
-      float a1 = 0.0f, a2 = 0.0f;
-      for (int part = 0; part < parts; ++part) {
-        a1 += level[part * t.width + c].x;
-        a2 += level[part * t.width + c].y;
+      if constexpr (BACKWARD) {
+        float2 v = make_float2(0.0f, 0.0f);
+        for (int part = 0; part < parts; ++part) {
+          v.x += level[part * t.width + c].x;
+          v.y += level[part * t.width + c].y;
+        }
+        chan[t.c0 + c] = v;
+      } else {
+        Moments m;
+        for (int part = 0; part < parts; ++part) {
+          const float2 v = level[part * t.width + c];
+          const int from = min(part * share, t.ty), to = min(from + share, t.ty);
+          m.join({static_cast<float>(before(to) - before(from)), v.x, v.y});
+        }
+        chan[t.c0 + c] = make_float2(m.mean, m.m2);
       }
-      chan[t.c0 + c] = channel_value<BACKWARD>(a1, a2, rows, chan[t.c0 + c].x);
     }
     __syncthreads();
   }
@@ -422,7 +470,8 @@ __device__ __forceinline__ void apply_rows(const Tile<VEC, THREADS>& t, const T*
   const T* px = x + at;
   const T* pg = dy + at;
   T* py = out + at;
-  each_row<T, VEC, BACKWARD, 64>(px, pg, -step, n, [&](const float(&v)[VEC], const float(&g)[VEC]) {
+  const auto nothing = [](const auto&, int) {};
+  each_row<T, VEC, BACKWARD, 64>(px, pg, -step, n, nothing, [&](const float(&v)[VEC], const float(&g)[VEC]) {
     float y[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -588,16 +637,12 @@ __device__ __forceinline__ void affine_grad(const GroupArgs& a, int tile, const 
 constexpr int kChunkThreads = 256;
 static_assert(kChunkThreads == kBlock, "affine_grad and block_sum run in both kernels");
 
-// The pieces of a frame, for one channel: terms whose sums (and n, all values
-// of the group) give its group's numbers.  Backward: sum d, sum d xhat; forward:
-// the sum and the sum of squares about `centre`, the first piece's mean of the
-// group's first channel.
-template <bool BACKWARD>
+// The pieces of a frame: what each of its channels left there.
 struct Pieces {
   const GroupArgs& a;
   int64_t r0, r1, first;
   int count;
-  float n;
+  float n;                // values of a group
   const float2* partial;  // the first piece's channels
   __device__ Pieces(const GroupArgs& args, int64_t b) : a(args) {
     r0 = a.frames.begin(b);
@@ -607,31 +652,54 @@ struct Pieces {
     n = static_cast<float>(r1 - r0) * static_cast<float>(a.group_channels);
     partial = a.partial + (first + b) * a.channels;
   }
-  __device__ float centre(int g) const { return BACKWARD ? 0.0f : partial[g * a.group_channels].x; }
-  // Pieces from, from + step, ... of channel c into s1 and s2.
-  __device__ void add(int c, float middle, int from, int step, float& s1, float& s2) const {
-    const float w = BACKWARD && a.weight ? __ldg(a.weight + c) : 1.0f;
-    add_terms(from, count, step, s1, s2, [&](int p) {
-      float2 v = partial[static_cast<int64_t>(p) * a.channels + c];
-      if constexpr (BACKWARD) {
-        v.x *= w;
-        v.y *= w;
-      } else {
+  __device__ __forceinline__ float2 at(int p, int c) const {
+    return partial[static_cast<int64_t>(p) * a.channels + c];
+  }
+  // Forward: pieces from, from + step, ... of channel c joined to m, eight at a time.
+  __device__ void join(int c, int from, int step, Moments& m) const {
+    for (int p = from; p < count;) {
+      Moments eight;
+#pragma unroll
+      for (int u = 0; u < 8; ++u, p += step) {
+        if (p >= count) continue;
         const int64_t chunk = first + p;
         const float rows = static_cast<float>(
             static_cast<int>(min((chunk + 1) * a.chunk_rows, r1) - max(chunk * a.chunk_rows, r0)));
-        const float d = v.x - middle;
-        v = make_float2(rows * d, fmaf(rows * d, d, v.y));
+        const float2 v = at(p, c);
+        eight.join({rows, v.x, v.y});
       }
-      return v;
+      m.join(eight);
+    }
+  }
+  // Backward: their sums of d and d xhat, d = dz w.
+  __device__ void add(int c, int from, int step, float& s1, float& s2) const {
+    const float w = a.weight ? __ldg(a.weight + c) : 1.0f;
+    add_terms(from, count, step, s1, s2, [&](int p) {
+      const float2 v = at(p, c);
+      return make_float2(v.x * w, v.y * w);
     });
   }
-  __device__ float2 numbers(int g, float s1, float s2) const {
-    s1 /= n;
-    if constexpr (BACKWARD) return make_float2(s1, s2 / n);
-    else return moments(a, centre(g) + s1, fmaf(-s1, s1, s2 / n));
-  }
 };
+
+// The block's moments joined in a fixed order; on thread 0.
+template <int LANES>
+__device__ __forceinline__ void lanes_join(Moments& v) {
+#pragma unroll
+  for (int d = LANES / 2; d > 0; d >>= 1)
+    v.join({__shfl_down_sync(kFull, v.n, d), __shfl_down_sync(kFull, v.mean, d),
+            __shfl_down_sync(kFull, v.m2, d)});
+}
+__device__ __forceinline__ Moments block_join(Moments v, Moments* scratch) {
+  lanes_join<kWarp>(v);
+  __syncthreads();
+  if (lane_id() == 0) scratch[threadIdx.x / kWarp] = v;
+  __syncthreads();
+  if (threadIdx.x < kWarp) {
+    v = threadIdx.x < kWarpsPerBlock ? scratch[threadIdx.x] : Moments();
+    lanes_join<kWarpsPerBlock>(v);
+  }
+  return v;
+}
 
 // CTAs of the kernel below on one SM.  In the statistics of the backward pass
 // more rows in flight for each thread do better than a third CTA (180001 x 96
@@ -702,7 +770,9 @@ __global__ void __launch_bounds__(kBlock) group_affine_kernel(GroupArgs a, int c
 // first `tiles` CTAs take the gradients of weight and bias, from all pieces.
 template <bool BACKWARD>
 __global__ void __launch_bounds__(kBlock) group_join_kernel(GroupArgs a, int tiles) {
-  __shared__ float scratch[kWarpsPerBlock];
+  using Part = std::conditional_t<BACKWARD, float, Moments>;
+  __shared__ __align__(16) unsigned char memory[kWarpsPerBlock * sizeof(Part)];
+  Part* scratch = reinterpret_cast<Part*>(memory);
   if constexpr (BACKWARD) {
     if (static_cast<int>(blockIdx.x) < tiles) {
       affine_grad(a, blockIdx.x, a.partial, a.chunks + a.frames.count);
@@ -718,20 +788,22 @@ __global__ void __launch_bounds__(kBlock) group_join_kernel(GroupArgs a, int til
         if (threadIdx.x == 0) a.mean[unit] = a.rstd[unit] = 0.0f;
       continue;
     }
-    const Pieces<BACKWARD> pieces(a, b);
+    const Pieces pieces(a, b);
     const int width = a.group_channels < kBlock ? a.group_channels : kBlock;
     const int lanes = kBlock / width, rank = threadIdx.x / width;
-    float s1 = 0.0f, s2 = 0.0f;
-    if (rank < lanes)
-      for (int c = threadIdx.x % width; c < a.group_channels; c += width)
-        pieces.add(c0 + c, pieces.centre(g), rank, lanes, s1, s2);
-    s1 = block_sum(s1, scratch);
-    s2 = block_sum(s2, scratch);
-    if (threadIdx.x == 0) {
-      const float2 v = pieces.numbers(g, s1, s2);
-      if constexpr (BACKWARD) {
-        a.sums[unit] = v;
-      } else {
+    const int c_first = rank < lanes ? threadIdx.x % width : a.group_channels;
+    if constexpr (BACKWARD) {
+      float s1 = 0.0f, s2 = 0.0f;
+      for (int c = c_first; c < a.group_channels; c += width) pieces.add(c0 + c, rank, lanes, s1, s2);
+      s1 = block_sum(s1, scratch);
+      s2 = block_sum(s2, scratch);
+      if (threadIdx.x == 0) a.sums[unit] = make_float2(s1 / pieces.n, s2 / pieces.n);
+    } else {
+      Moments m;
+      for (int c = c_first; c < a.group_channels; c += width) pieces.join(c0 + c, rank, lanes, m);
+      m = block_join(m, scratch);
+      if (threadIdx.x == 0) {
+        const float2 v = moments(a, m.mean, m.m2 / pieces.n);
         a.mean[unit] = v.x;
         a.rstd[unit] = v.y;
       }

@@ -181,3 +181,76 @@ def test_function_transforms_are_refused(cuda):
                           lambda f: torch.func.grad(lambda t: f(t).sum())(x)):
             with pytest.raises(RuntimeError):
                 transform(call)
+
+
+# ---- group norm: outliers, infinities, launch shapes -------------------------------------------
+
+def chunk_rows(rows, row_bytes):
+    """Rows of a forward statistics chunk: one for each of four resident CTAs an SM, of 16 KB at least."""
+    ctas = torch.cuda.get_device_properties(0).multi_processor_count * 4
+    return max(-(-rows // ctas), -(-16384 // row_bytes))
+# rows, channels, groups, lengths, where -> value, dtype
+OUTLIERS = {
+    "first row": (200000, 160, 1, None, [(0, 0, 3000.0)], F32),
+    "first row, few channels": (196608, 4, 1, None, [(0, None, 1000.0)], F32),
+    "first rows of every frame": (98304, 8, 2, [1000, 40000, 57304], [(0, None, 300.0)], F32),
+    "group's first channel": (20000, 1024, 1, None, [(None, 0, 1000.0)], F32),
+    "group's last channel": (20000, 64, 4, None, [(None, 63, 1000.0)], F32),
+    "small frame": (4000, 4, 1, None, [(0, None, 3000.0)], F32),
+    "bfloat16": (100000, 64, 8, None, [(0, None, 1024.0)], BF16),
+}
+
+
+@pytest.mark.parametrize("name", OUTLIERS)
+def test_group_norm_variance_beside_outliers(cuda, name):
+    rows, channels, groups, lengths, places, dtype = OUTLIERS[name]
+    gen = generator(rows)
+    x = normal(gen, rows, channels)
+    offsets = np.concatenate([[0], np.cumsum([rows] if lengths is None else lengths)])
+    for row, channel, value in places:
+        at = slice(None) if channel is None else channel
+        if row is None:
+            x[:, at] += value
+        else:
+            x[torch.from_numpy(offsets[:-1] + row).cuda(), at] = value
+    x = x.to(dtype)
+    check_norm(x, groups, offsets, dtype)
+
+
+@pytest.mark.parametrize("before", [1, 2, 5])
+def test_group_norm_variance_of_a_frame_that_begins_at_the_end_of_a_chunk(cuda, before):
+    rows, channels = 200000, 8
+    edge = 40 * chunk_rows(rows, channels * 4)
+    offsets = np.array([0, edge - before, rows])
+    x = normal(generator(before), rows, channels)
+    x[edge - before] = 1000.0
+    check_norm(x, 2, offsets, F32)
+
+
+def check_norm(x, groups, offsets, dtype):
+    """z = (x - mean) rstd beside the float64 definition.
+
+    mean: the weighted mean of partial means, each within a few units of the values' size, rstd: sums of
+    squares about means, 64 terms and a few levels of joining: 96 units relative.  z itself is one
+    multiply-add, whose constant has the mean's rounding.
+    """
+    channels = x.shape[-1]
+    y = K.group_norm(x, groups, offsets=torch.from_numpy(offsets).cuda())
+    flat = x.double()
+    for a, b in zip(offsets[:-1], offsets[1:]):
+        v = flat[a:b].reshape(b - a, groups, -1)
+        mean = v.mean((0, 2), keepdim=True)
+        rstd = 1.0 / torch.sqrt((v - mean).square().mean((0, 2), keepdim=True) + 1e-5)
+        z = (v - mean) * rstd
+        size = 1.0 + v.abs() * rstd + v.abs().mean((0, 2), keepdim=True) * rstd
+        tol = 96 * U * (size + z.abs()) + (B if dtype == BF16 else 0.0) * z.abs()
+        off = (y[a:b].double().reshape(v.shape) - z).abs() - tol
+        assert float(off.max()) <= 0.0, f"off by {float(off.max())} beyond the tolerance"
+
+
+def test_group_norm_one_large_frame_among_small_ones(cuda):
+    gen = generator(71)
+    lengths = np.full(400, 3)
+    lengths[200] = 30000
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    check_norm(normal(gen, int(offsets[-1]), 16), 2, offsets, F32)
