@@ -510,8 +510,10 @@ struct Smem {
   }
 };
 
+// A variance that is not a number (an infinity among the values) stays one: the mean
+// alone may be infinite, which an activation turns into a number.
 __device__ __forceinline__ float2 moments(const GroupArgs& a, float mean, float variance) {
-  return make_float2(mean, 1.0f / sqrtf(fmaxf(variance, 0.0f) + a.eps));
+  return make_float2(mean, 1.0f / sqrtf((variance < 0.0f ? 0.0f : variance) + a.eps));
 }
 
 // Statistics of one tile's thread: mean and rstd of frame b, and its sums.

@@ -248,6 +248,23 @@ def check_norm(x, groups, offsets, dtype):
         assert float(off.max()) <= 0.0, f"off by {float(off.max())} beyond the tolerance"
 
 
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("rows", [40, 9000])
+@pytest.mark.parametrize("activation", [None, "sigmoid", "silu"])
+def test_group_norm_infinities_show(cuda, value, rows, activation):
+    # a frame and group that hold one have no mean: all of it is NaN, nothing else is touched
+    x = normal(generator(67), 3 * rows, 16)
+    offsets = torch.tensor([0, rows, 2 * rows, 3 * rows], device="cuda")
+    whole = K.group_norm(x, 4, activation=activation, offsets=offsets)
+    for place in (rows, rows + rows // 2, 2 * rows - 1):
+        bad = x.clone()
+        bad[place, 5] = value
+        y = K.group_norm(bad, 4, activation=activation, offsets=offsets)
+        assert torch.isnan(y[rows:2 * rows, 4:8]).all()
+        y[rows:2 * rows, 4:8] = whole[rows:2 * rows, 4:8]
+        assert torch.equal(y, whole)
+
+
 def test_group_norm_one_large_frame_among_small_ones(cuda):
     gen = generator(71)
     lengths = np.full(400, 3)
