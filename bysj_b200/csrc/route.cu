@@ -30,7 +30,7 @@
 //
 // 500000 x 128 bfloat16 logits, k = 8, renormalised: forward 94 us, bound by the
 // integer pipe of the comparators (122 warp instructions a token; the pass a slot
-// takes 217 and 168 us; HBM would need 27 us), backward 83 us, bound by issue
+// takes 217 and 168 us; HBM would need 27 us), backward 84 us, bound by issue
 // (HBM 49 us).  With an atomic for each probability the pair took 4.7 ms.
 #include "launch.cuh"
 
@@ -103,6 +103,11 @@ __device__ __forceinline__ void copy_vec(T* to, const T* from) {
   if constexpr (V * sizeof(T) == 16)
     *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
   else *to = *from;
+}
+template <int V, typename T>
+__device__ __forceinline__ void zero_vec(T* to) {
+  if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4*>(to) = make_uint4(0u, 0u, 0u, 0u);
+  else *to = T(0.0f);
 }
 
 // Cotangents in shared memory, so that the L lanes of a row read 16 bytes each
@@ -729,7 +734,7 @@ __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
       const int64_t t = base + g;
       Fetch f = next;
       if (base + kWarpsPerBlock * R < hi) next = fetch(t + kWarpsPerBlock * R, hi);
-      if (f.first < 0) {  // not a valid token: p = 0 everywhere
+      if (f.first < 0) {  // not a valid token: its gradient is 0 whatever comes back
         f.row.clear();
         f.total = 1.0f;
       }
@@ -738,10 +743,12 @@ __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
       const float ref = top > -INFINITY ? top : 0.0f;
       float along_w = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) along_w = fmaf(f.w[i], f.gw[i], along_w);
+      for (int i = 0; i < kMine; ++i)  // an empty slot's cotangent may hold anything
+        along_w = fmaf(f.w[i], f.slot[i] >= 0 ? f.gw[i] : 0.0f, along_w);
       if (gated && k > kMine * L && t < hi)
         for (int j = l + kMine * L; j < k; j += L)
-          along_w += __ldg(a.weights + t * k + j) * __ldg(a.grad_weights + t * k + j);
+          if (__ldg(a.chosen + t * k + j) >= 0)
+            along_w += __ldg(a.weights + t * k + j) * __ldg(a.grad_weights + t * k + j);
       along_w = row_sum<L>(along_w);
       // p_e and the sum of p_e a_e; a weight that is p itself adds gw p at its expert
       float p[M], along = 0.0f;
@@ -791,7 +798,9 @@ __global__ void __launch_bounds__(kBlock, V * NV <= 16 ? 3 : 2)
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
           const int c = (n * L + l) * V;
-          if (c < E) copy_vec<V>(out + t * E + c, stage + c);
+          if (c >= E) continue;
+          if (f.first >= 0) copy_vec<V>(out + t * E + c, stage + c);
+          else zero_vec<V>(out + t * E + c);
         }
       }
       __syncwarp();

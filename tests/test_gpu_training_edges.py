@@ -271,3 +271,32 @@ def test_group_norm_one_large_frame_among_small_ones(cuda):
     lengths[200] = 30000
     offsets = np.concatenate([[0], np.cumsum(lengths)])
     check_norm(normal(gen, int(offsets[-1]), 16), 2, offsets, F32)
+
+
+# ---- router: masked places, launch shapes ---------------------------------------------------------
+
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("dtype,experts,k", [(F32, 8, 2), (BF16, 64, 4), (F32, 33, 12)])
+def test_router_cotangents_of_masked_tokens_and_empty_slots_have_no_effect(cuda, renormalize, dtype,
+                                                                          experts, k):
+    gen, nan = generator(73), float("nan")
+    x = normal(gen, 50, experts)
+    x[10:20, 1:] = float("-inf")   # one expert each, the other slots empty
+    x[20:25] = float("-inf")       # none at all
+    x = x.to(dtype).requires_grad_()
+    mask = torch.ones(50, dtype=torch.bool, device="cuda")
+    mask[30:40] = False
+    r = K.route_experts(x, k, mask=mask, renormalize=renormalize)
+    cotangents = [normal(gen, 50, k), torch.tensor(0.7, device="cuda"), torch.tensor(0.1, device="cuda")]
+    want, = torch.autograd.grad([r.weights, r.balance, r.z], [x], cotangents, retain_graph=True)
+    empty = r.experts < 0
+    for value in (nan, float("inf")):
+        spoiled = [cotangents[0].masked_fill(empty, value), *cotangents[1:]]
+        got, = torch.autograd.grad([r.weights, r.balance, r.z], [x], spoiled, retain_graph=True)
+        assert torch.equal(got, want)
+    # a loss that is lost leaves the tokens alone that were left out of it
+    spoiled = [cotangents[0], torch.tensor(nan, device="cuda"), torch.tensor(nan, device="cuda")]
+    got, = torch.autograd.grad([r.weights, r.balance, r.z], [x], spoiled)
+    out = ~mask
+    out[20:25] = True
+    assert (got[out] == 0.0).all() and torch.isnan(got[~out]).any(1).all()
