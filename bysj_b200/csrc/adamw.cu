@@ -21,9 +21,9 @@
 // measured copy bandwidth (448 us).  39.5 M bfloat16 parameters with masters and
 // 8-bit states: 160 us (16 B an element, 97 us at that bandwidth), bound by issue:
 // about 100 lane operations an element, of which the correctly rounded root and
-// quotient are a good part.  With random rounding of sqrt(v) 202 us, of both 206
-// us: the generator's 28 multiplications for four elements.  Values of 8-bit
-// states: 76 us (10 B, 60 us).
+// quotient are a good part.  Random rounding adds 39 us for sqrt(v), 41 us for both:
+// the generator's 28 multiplications for four elements.  Values of 8-bit states: 76
+// us (10 B, 60 us).
 //
 // 8-bit states.  m keeps a sign and a 7-bit magnitude with 3 mantissa bits
 // (a relative rounding of at most 1/16 down to 2^-16 of the block's
@@ -198,13 +198,14 @@ __device__ __forceinline__ float inverse_scale(float scale) {
 
 // Ratios are at most 1 up to a rounding that the code drops, unless the scale
 // is so small that its inverse is infinite: then every value but 0 takes the
-// top code (and a NaN's block has a NaN scale, whatever its codes).
+// top code (0 times it is not a number and compares as below the least).  A block
+// with a NaN or an infinity has it for its scale, and no finite value of any code.
 constexpr float kLeastM = 1.25f / 65536.0f, kLeastV = 1.125f / 65536.0f;  // value(1)
 
 // Below the smallest code's value: to it or to 0.
 __device__ __forceinline__ unsigned encode_m(float m, float inv, Rounding how) {
-  const float ratio = fminf(__fmul_rn(fabsf(m), inv), 1.0f);
-  const unsigned code = ratio_code<kTopM, kMantM>(fmaxf(ratio, kLeastM), how);
+  const float ratio = __fmul_rn(fabsf(m), inv);
+  const unsigned code = ratio_code<kTopM, kMantM>(fminf(fmaxf(ratio, kLeastM), 1.0f), how);
   return (ratio >= how.threshold() * kLeastM ? code : 0u) | (m < 0.0f ? 128u : 0u);
 }
 __device__ __forceinline__ unsigned encode_v(float root, float inv, Rounding how) {

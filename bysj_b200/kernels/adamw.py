@@ -41,8 +41,8 @@ class AdamW:
     that it keeps following its gradients; the root of the second moment then
     differs from that of 32-bit states by about 11 % root mean square.  The
     random numbers come from the step and the element: equal runs give equal
-    bits.  A non-finite gradient makes the moments of its whole block NaN
-    there, of its element alone with 32 bits.
+    bits.  A non-finite gradient leaves no finite moment in its whole block
+    there, in its element alone with 32 bits.
     ``master_weights`` keeps float32 weights beside the parameters;
     call :meth:`sync_master` after assigning parameters by hand.
 

@@ -214,9 +214,10 @@ def encode(x, top, values, noise=None):
     the part of the gap above it does not exceed the noise.
     """
     scale = x.max(1)
-    with np.errstate(divide="ignore"):
+    with np.errstate(divide="ignore", over="ignore", invalid="ignore"):
         inverse = np.where(scale > 0, np.float32(1.0) / scale, np.float32(0.0)).astype(np.float32)
-    ratio = (x * inverse[:, None]).astype(np.float64)
+        ratio = (x * inverse[:, None]).astype(np.float64)
+    ratio[x == 0] = 0.0  # also where the inverse is infinite
     if noise is not None:
         ratio = np.minimum(ratio, 1.0)
         lower = np.searchsorted(values, ratio, side="right") - 1

@@ -146,6 +146,20 @@ def test_adamw_8bit_random_rounding_repeats_and_resumes(cuda):
     assert torch.equal(one, two) and torch.equal(a.exp_avg_sq, c.exp_avg_sq)
 
 
+# ---- AdamW: what a step is given -----------------------------------------------------------
+
+def test_adamw_zero_stays_zero_beside_tiny_values(cuda):
+    # the inverse of a scale below 2^-128 is infinite: its product with 0 must not become a code
+    p = torch.zeros(300, device="cuda")
+    g = torch.zeros(300, device="cuda")
+    g[:100], g[100:200] = 1e-39, -1e-39
+    opt = K.AdamW([p], state_bits=8, betas=(0.9, 0.95))
+    opt.step([g])
+    m = opt.state_values()[0]
+    assert float(m[:256].abs().max()) > 0.0  # the block holds something
+    assert (opt.exp_avg[200:] == 0).all() and (m[200:] == 0.0).all()
+
+
 # ---- derivatives other than backward ---------------------------------------------------------
 
 def operator_calls(gen):

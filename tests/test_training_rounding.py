@@ -100,3 +100,13 @@ def test_c_entry_without_a_counter_refuses_slow_moments():
                                      one_minus_beta2, 1.0, 0.01, 1.0, 1e-8)
         assert lib.bysj_adamw_step(table, 1, 0, 8, at, at, at, at, None, None, hyper, None) == 1
         assert b"bysj_adamw_step_counted" in lib.bysj_last_error()
+
+
+@pytest.mark.parametrize("noise", [None, 0.75])
+def test_zero_beside_values_whose_scale_has_no_finite_inverse(noise):
+    x = np.zeros((1, O.BLOCK), np.float32)
+    x[0, :2] = 1e-39, 1e-40
+    noise = None if noise is None else np.full(x.shape, noise)
+    for top, values in ((127, O.VALUES_M), (255, O.VALUES_V)):
+        code, scale = O.encode(x, top, values, noise)
+        assert (code[0, :2] == top).all() and (code[0, 2:] == 0).all() and scale[0] == x[0, 0]
