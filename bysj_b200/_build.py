@@ -166,6 +166,10 @@ def build_extension(verbose: bool = True) -> Path:
         "-ltorch_python",
         f"-L{PACKAGE}",
         "-lbysj_b200",
+        # torch's own C++ runtime, by name: a compiler that finds only the static one
+        # would put a second copy into the module, whose streams crash on numbers
+        # (their locale facets are found by the other copy's identifiers)
+        "-l:libstdc++.so.6",
         "-Wl,-rpath,$ORIGIN",
         *[f"-Wl,-rpath,{p}" for p in libdirs],
     ]

@@ -1216,7 +1216,8 @@ struct AdamWParams {
   std::vector<int64_t> begins;
   AdamWParams(std::vector<Tensor> p, std::vector<int64_t> b)
       : params(std::move(p)), begins(std::move(b)) {
-    TORCH_CHECK(params.size() == begins.size(), "AdamW needs one begin for each parameter");
+    TORCH_CHECK(params.size() == begins.size(), "AdamW needs one begin for each parameter: ",
+                params.size(), " parameters, ", begins.size(), " begins");
   }
 };
 
