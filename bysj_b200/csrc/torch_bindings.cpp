@@ -1261,10 +1261,10 @@ void adamw_step(const AdamWParams& tensors, const std::vector<OptTensor>& grads,
     if (!grads[i]) continue;
     const Tensor &p = params[i], &g = *grads[i];
     const int dt = value_dtype(p, "AdamW parameter");
-    TORCH_CHECK(g.scalar_type() == p.scalar_type() && g.numel() == p.numel() &&
+    TORCH_CHECK(g.scalar_type() == p.scalar_type() && g.sizes() == p.sizes() &&
                     g.device() == p.device() && p.device() == exp_avg.device() &&
                     g.is_contiguous(),
-                "AdamW gradient ", i, " must be contiguous with the parameter's dtype, size and "
+                "AdamW gradient ", i, " must be contiguous with the parameter's dtype, shape and "
                 "device");
     const int64_t begin = begins[i], n = p.numel();
     TORCH_CHECK(begin >= 0 && begin % BYSJ_ADAMW_BLOCK == 0 &&

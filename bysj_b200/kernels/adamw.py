@@ -113,7 +113,7 @@ class AdamW:
              grad_scale: torch.Tensor | None = None) -> None:
         """Step every parameter that has a gradient, in place.
 
-        ``grads``: one tensor (or ``None``: skip) per parameter, of its dtype;
+        ``grads``: one tensor (or ``None``: skip) per parameter, of its dtype and shape;
         default the parameters' ``.grad``.  ``grad_scale``: a float32 CUDA
         tensor of one element that multiplies every gradient (a clip factor or
         the inverse of a loss scale), read on the device.

@@ -160,6 +160,15 @@ def test_adamw_zero_stays_zero_beside_tiny_values(cuda):
     assert (opt.exp_avg[200:] == 0).all() and (m[200:] == 0.0).all()
 
 
+def test_adamw_gradient_of_another_shape_is_refused(cuda):
+    p = torch.ones(3, 4, device="cuda")
+    opt = K.AdamW([p])
+    for shape in ((4, 3), (12,), (3, 4, 1)):
+        with pytest.raises(RuntimeError, match="shape"):
+            opt.step([torch.ones(shape, device="cuda")])
+    assert opt.step_count == 0 and torch.equal(p, torch.ones_like(p))
+
+
 # ---- derivatives other than backward ---------------------------------------------------------
 
 def operator_calls(gen):
