@@ -1213,11 +1213,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_experts(const Tensor& l
 // begin (a multiple of BYSJ_ADAMW_BLOCK).
 struct AdamWParams {
   std::vector<Tensor> params;
-  std::vector<int64_t> begins;
+  std::vector<int64_t> begins, sizes;
   AdamWParams(std::vector<Tensor> p, std::vector<int64_t> b)
       : params(std::move(p)), begins(std::move(b)) {
     TORCH_CHECK(params.size() == begins.size(), "AdamW needs one begin for each parameter: ",
                 params.size(), " parameters, ", begins.size(), " begins");
+    for (const Tensor& t : params) sizes.push_back(t.numel());
   }
 };
 
@@ -1267,6 +1268,9 @@ void adamw_step(const AdamWParams& tensors, const std::vector<OptTensor>& grads,
                 "AdamW gradient ", i, " must be contiguous with the parameter's dtype, shape and "
                 "device");
     const int64_t begin = begins[i], n = p.numel();
+    // its states end where those of the next one begin
+    TORCH_CHECK(n == tensors.sizes[i], "AdamW parameter ", i, " changed its shape: ",
+                tensors.sizes[i], " elements when handed over, now ", n);
     TORCH_CHECK(begin >= 0 && begin % BYSJ_ADAMW_BLOCK == 0 &&
                     begin + (n + BYSJ_ADAMW_BLOCK - 1) / BYSJ_ADAMW_BLOCK * BYSJ_ADAMW_BLOCK <=
                         length,

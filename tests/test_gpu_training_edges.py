@@ -169,6 +169,14 @@ def test_adamw_gradient_of_another_shape_is_refused(cuda):
     assert opt.step_count == 0 and torch.equal(p, torch.ones_like(p))
 
 
+def test_adamw_parameter_that_changed_its_size_is_refused(cuda):
+    p, q = torch.ones(4, device="cuda"), torch.ones(300, device="cuda")
+    opt = K.AdamW([p, q])
+    p.data = torch.ones(400, device="cuda")  # its states would reach into those of q
+    with pytest.raises(RuntimeError, match="shape"):
+        opt.step([torch.ones(400, device="cuda"), None])
+
+
 # ---- derivatives other than backward ---------------------------------------------------------
 
 def operator_calls(gen):
