@@ -55,7 +55,7 @@ class AdamW:
                  betas: Sequence[float] = (0.9, 0.999), eps: float = 1.0e-8,
                  weight_decay: float = 1.0e-2, *, state_bits: int = 32,
                  master_weights: bool = False) -> None:
-        self.params = list(params)
+        self._params = tuple(params)
         if not self.params:
             raise ValueError("AdamW needs at least one parameter")
         for p in self.params:
@@ -100,6 +100,11 @@ class AdamW:
         if master_weights:
             self.master = torch.zeros(length, device=device)
             self.sync_master()
+
+    @property
+    def params(self) -> tuple[torch.Tensor, ...]:
+        """The parameters, fixed when the optimizer is made."""
+        return self._params
 
     @torch.no_grad()
     def sync_master(self) -> None:

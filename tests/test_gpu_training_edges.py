@@ -177,6 +177,16 @@ def test_adamw_parameter_that_changed_its_size_is_refused(cuda):
         opt.step([torch.ones(400, device="cuda"), None])
 
 
+def test_adamw_params_cannot_be_replaced_behind_its_back(cuda):
+    p = torch.ones(4, device="cuda")
+    opt = K.AdamW([p])
+    with pytest.raises(TypeError):
+        opt.params[0] = torch.zeros(4, device="cuda")
+    with pytest.raises(AttributeError):
+        opt.params = [torch.zeros(4, device="cuda")]
+    assert opt.params[0] is p
+
+
 # ---- derivatives other than backward ---------------------------------------------------------
 
 def operator_calls(gen):
