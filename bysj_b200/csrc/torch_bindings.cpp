@@ -6,6 +6,7 @@
 // happens here.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/CUDAEvent.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -1279,6 +1280,9 @@ void adamw_step(const AdamWParams& tensors, const std::vector<OptTensor>& grads,
         {p.data_ptr(), g.data_ptr(), n, begin / BYSJ_ADAMW_BLOCK});
   }
   c10::cuda::CUDAGuard guard(exp_avg.device());
+  TORCH_CHECK(at::cuda::currentStreamCaptureStatus() == at::cuda::CaptureStatus::None,
+              "AdamW steps cannot be captured in a graph: a replay would repeat this step's bias "
+              "corrections");
   for (int i = 0; i < 2; ++i) {
     if (table[i].empty()) continue;
     check(bysj_adamw_step_counted(table[i].data(), static_cast<int64_t>(table[i].size()),

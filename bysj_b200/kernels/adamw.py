@@ -121,7 +121,8 @@ class AdamW:
         ``grads``: one tensor (or ``None``: skip) per parameter, of its dtype and shape;
         default the parameters' ``.grad``.  ``grad_scale``: a float32 CUDA
         tensor of one element that multiplies every gradient (a clip factor or
-        the inverse of a loss scale), read on the device.
+        the inverse of a loss scale), read on the device.  A step is refused while
+        the stream is captured: its bias corrections are values of this call.
         """
         if grads is None:
             grads = [p.grad for p in self.params]

@@ -187,6 +187,23 @@ def test_adamw_params_cannot_be_replaced_behind_its_back(cuda):
     assert opt.params[0] is p
 
 
+def test_adamw_step_is_not_captured(cuda):
+    # the bias corrections and the step count are values of the call: a replay would repeat them
+    p, g = torch.ones(4, device="cuda"), torch.ones(4, device="cuda")
+    opt = K.AdamW([p])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = p + 1.0
+        with pytest.raises(RuntimeError, match="captur"):
+            opt.step([g])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert opt.step_count == 0 and torch.equal(p, torch.ones_like(p)) and float(y[0]) == 2.0
+    opt.step([g])
+    assert opt.step_count == 1
+
+
 # ---- derivatives other than backward ---------------------------------------------------------
 
 def operator_calls(gen):
