@@ -1262,6 +1262,8 @@ void adamw_step(const AdamWParams& tensors, const std::vector<OptTensor>& grads,
   for (size_t i = 0; i < params.size(); ++i) {
     if (!grads[i]) continue;
     const Tensor &p = params[i], &g = *grads[i];
+    TORCH_CHECK(!p.is_inference() || c10::InferenceMode::is_enabled(), "AdamW parameter ", i,
+                " is an inference tensor: step it in inference mode");
     const int dt = value_dtype(p, "AdamW parameter");
     TORCH_CHECK(g.scalar_type() == p.scalar_type() && g.sizes() == p.sizes() &&
                     g.device() == p.device() && p.device() == exp_avg.device() &&

@@ -204,6 +204,18 @@ def test_adamw_step_is_not_captured(cuda):
     assert opt.step_count == 1
 
 
+def test_adamw_inference_tensor_is_refused_before_the_step(cuda):
+    with torch.inference_mode():
+        p = torch.ones(4, device="cuda")
+    opt = K.AdamW([p])
+    with pytest.raises(RuntimeError, match="inference"):
+        opt.step([torch.ones(4, device="cuda")])
+    assert torch.equal(p.cpu(), torch.ones(4)) and float(opt.exp_avg.abs().max()) == 0.0
+    with torch.inference_mode():
+        opt.step([torch.ones(4, device="cuda")])
+    assert opt.step_count == 1
+
+
 # ---- derivatives other than backward ---------------------------------------------------------
 
 def operator_calls(gen):
