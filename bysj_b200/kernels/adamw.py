@@ -69,6 +69,10 @@ class AdamW:
             raise ValueError("all AdamW parameters must share a device")
         if len({id(p) for p in self.params}) != len(self.params):
             raise ValueError("AdamW parameters must be different tensors")
+        ranges = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in self.params
+                        if p.numel())
+        if any(at + size > after for (at, size), (after, _) in zip(ranges, ranges[1:])):
+            raise ValueError("AdamW parameters must not share memory")
         if state_bits not in (8, 32):
             raise ValueError("AdamW state_bits must be 8 or 32")
         self.lr, self.eps, self.weight_decay = float(lr), float(eps), float(weight_decay)
