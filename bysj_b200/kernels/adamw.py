@@ -172,17 +172,19 @@ class AdamW:
     @torch.no_grad()
     def load_state_dict(self, state: dict[str, Any]) -> None:
         """Copy the buffers of a :meth:`state_dict` of the same layout into this one."""
+        step = int(state["step"])
         for name in self._BUFFERS:
             own, given = getattr(self, name), state[name]
             if (own is None) != (given is None):
                 raise ValueError(f"AdamW state {name} is present on one side only")
-            if own is not None and (given.dtype != own.dtype or given.shape != own.shape):
+            if own is not None and (not isinstance(given, torch.Tensor) or
+                                    given.dtype != own.dtype or given.shape != own.shape):
                 raise ValueError(f"AdamW state {name} must be {own.dtype} of shape "
                                  f"{tuple(own.shape)}")
         for name in self._BUFFERS:
             if state[name] is not None:
                 getattr(self, name).copy_(state[name])
-        self.step_count = int(state["step"])
+        self.step_count = step
 
 
 __all__ = ["AdamW", "BLOCK"]

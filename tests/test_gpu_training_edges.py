@@ -187,6 +187,18 @@ def test_adamw_params_cannot_be_replaced_behind_its_back(cuda):
     assert opt.params[0] is p
 
 
+@pytest.mark.parametrize("change,error", [(dict(step=None), TypeError), (dict(exp_avg_sq=[0.0]), ValueError),
+                                          (dict(exp_avg_sq=torch.zeros(3)), ValueError),
+                                          (dict(master=torch.zeros(256)), ValueError)])
+def test_adamw_state_that_does_not_fit_changes_nothing(cuda, change, error):
+    p = torch.ones(4, device="cuda")
+    opt, other = K.AdamW([p]), K.AdamW([p.clone()])
+    other.step([torch.ones(4, device="cuda")])
+    with pytest.raises(error):
+        opt.load_state_dict({**other.state_dict(), **change})
+    assert opt.step_count == 0 and float(opt.exp_avg.abs().max()) == 0.0
+
+
 def test_adamw_step_is_not_captured(cuda):
     # the bias corrections and the step count are values of the call: a replay would repeat them
     p, g = torch.ones(4, device="cuda"), torch.ones(4, device="cuda")
