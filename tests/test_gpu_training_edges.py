@@ -347,6 +347,38 @@ def test_group_norm_infinities_show(cuda, value, rows, activation):
         assert torch.equal(y, whole)
 
 
+@pytest.mark.parametrize("frames", [200, 2000])
+@pytest.mark.parametrize("dtype,channels", [(F32, 24), (BF16, 64), (F32, 7)])
+def test_group_norm_many_small_frames(cuda, frames, dtype, channels):
+    """More frames than CTAs are launched: a CTA walks over several and adds up their affine gradients.
+
+    Values as in the one-frame tests (z within 16 units of its size and the mean's); an affine gradient
+    sums n terms of either sign with that error, over a few hundred rows a CTA and the CTAs in order.
+    """
+    gen, rng = generator(frames), np.random.default_rng(frames)
+    lengths = rng.integers(0, 12, frames)
+    lengths[:3] = 0, 1, 0
+    offsets = np.concatenate([[0], np.cumsum(lengths)])
+    rows, groups = int(offsets[-1]), 1 if channels == 7 else 4
+    x, grad = normal(gen, rows, channels, dtype=dtype), normal(gen, rows, channels, dtype=dtype)
+    w, b = torch.rand(channels, generator=gen, device="cuda") + 0.5, normal(gen, channels, scale=0.3)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = K.group_norm(x, groups, w, b, activation="silu", offsets=torch.from_numpy(offsets).cuda())
+    grads = torch.autograd.grad(y, leaves, grad)
+    want, (gx, gw, gb) = O.group_norm(f64(x), offsets, groups, f64(w), f64(b), 1e-5, "silu", f64(grad))
+    half = B if dtype == BF16 else 0.0
+    # a frame of six values and more: 1 / std below 20 for these
+    v = [f64(x)[i:j].reshape(j - i, groups, -1) for i, j in zip(offsets[:-1], offsets[1:]) if j > i]
+    rstd = max(1.0 / np.sqrt(t.var((0, 2)) + 1e-5).min() for t in v)
+    off = 16 * U * (2.0 + rstd)
+    xhat = max(2.0, np.sqrt(12.0 * channels / groups))
+    close(y, want, off * 1.5 * xhat + half * np.abs(want))
+    d = np.abs(f64(grad)).max() * 1.1 * 1.5
+    close(grads[0], gx, rstd * off * d * (2.0 + 2.0 * xhat * xhat) * 1.5 + half * np.abs(gx))
+    for got, ref in ((grads[1], gw), (grads[2], gb)):
+        close(got, ref, 4 * np.sqrt(rows) * off * d * xhat * 1.5 + 4 * U * np.sqrt(rows) * np.abs(ref))
+
+
 def test_group_norm_one_large_frame_among_small_ones(cuda):
     gen = generator(71)
     lengths = np.full(400, 3)
@@ -382,3 +414,128 @@ def test_router_cotangents_of_masked_tokens_and_empty_slots_have_no_effect(cuda,
     out = ~mask
     out[20:25] = True
     assert (got[out] == 0.0).all() and torch.isnan(got[~out]).any(1).all()
+
+
+def check_route(x, k, lengths, mask, renormalize, seed):
+    """Against the float64 definition, with the bounds of the other router tests."""
+    tokens, experts = x.shape
+    gen = generator(seed)
+    offsets = None if lengths is None else np.concatenate([[0], np.cumsum(lengths)])
+    given = None if offsets is None else torch.from_numpy(offsets).cuda()
+    grads = (normal(gen, tokens, k), torch.tensor(0.7 * tokens, device="cuda"),
+             torch.tensor(0.1 * tokens, device="cuda"))
+    x = x.clone().requires_grad_()
+    r = K.route_experts(x, k, mask=mask, offsets=given, renormalize=renormalize)
+    grad, = torch.autograd.grad([r.weights, r.balance, r.z], [x], list(grads))
+    want = O.route(f64(x), k, None if mask is None else mask.cpu().numpy(), offsets, renormalize,
+                   (f64(grads[0]), float(grads[1]), float(grads[2])))
+    np.testing.assert_array_equal(r.experts.cpu().numpy(), want[1])
+    counts = r.counts.cpu().numpy()
+    np.testing.assert_array_equal(counts if offsets is not None else counts[None], want[2])
+    rel = (16 + experts / 8) * U
+    close(r.weights, want[0], 2 * rel * want[0])
+    close(r.balance.reshape(1), np.array([want[3]]), rel * abs(want[3]) + 1e-9)
+    top = np.abs(f64(x)[np.isfinite(f64(x))]).max() + np.log(experts)
+    close(r.z.reshape(1), np.array([want[4]]), rel * top * 2.0 * np.sqrt(want[4]) + U * want[4])
+    valid = (want[1][:, 0] >= 0).astype(np.int64)
+    edges = np.array([0, tokens]) if offsets is None else offsets
+    n = np.maximum([valid[a:b].sum() for a, b in zip(edges[:-1], edges[1:])], 1)
+    scale = np.abs(f64(grads[0])).max() + \
+        float(grads[1]) * (experts / k * want[2].max(1) / n ** 2).max() + \
+        float(grads[2]) * 2.0 / max(valid.sum(), 1) * (top + 5.0)
+    half = B if x.dtype == BF16 else 0.0
+    close(grad, want[5], 4 * rel * scale + half * np.abs(want[5]))
+
+
+@pytest.mark.parametrize("ties", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("experts,k", [(512, 8), (1024, 8), (1024, 3), (264, 5), (24, 4), (32, 3),
+                                       (20, 7), (28, 1), (8, 8), (256, 2)])
+def test_router_launch_shapes(cuda, experts, k, dtype, ties):
+    x = normal(generator(experts + k), 90, experts, scale=2.0)
+    check_route((torch.round(x) if ties else x).to(dtype), k, None, None, True, 79)
+
+
+@pytest.mark.parametrize("frames,experts", [(100, 256), (300, 64), (2000, 16)])
+def test_router_losses_of_many_frames(cuda, frames, experts):
+    # more cells than the forward kernel's last CTA takes: a kernel of several CTAs joins the losses
+    rng = np.random.default_rng(frames)
+    lengths = rng.integers(0, 7, frames)
+    tokens = int(lengths.sum())
+    gen = generator(frames)
+    x = normal(gen, tokens, experts, scale=1.5)
+    mask = torch.rand(tokens, generator=gen, device="cuda") < 0.8
+    check_route(x, 2, lengths, mask, False, 83)
+
+
+# ---- rotary: long positions -----------------------------------------------------------------------
+
+def test_rotary_long_positions(cuda):
+    """Angles of thousands of turns: the float32 product is off by a unit roundoff of the angle."""
+    gen = generator(89)
+    q = normal(gen, 50, 2, 16)
+    pos = torch.randint(0, 1 << 17, (50, 2), generator=gen, device="cuda")
+    freq = torch.rand(8, generator=gen, device="cuda") + 0.05
+    y, _ = K.rotary_axes(q, None, pos, freq, (4, 4))
+    want = O.rotary(f64(q), f64(pos), f64(freq), (4, 4))
+    theta = float(pos.max()) * float(freq.max())
+    close(y, want, (U * theta + 8 * U) * 2.0 * float(q.abs().max()))
+
+
+# ---- graphs and threads ----------------------------------------------------------------------------
+
+def test_forward_and_backward_are_captured(cuda):
+    gen = generator(97)
+    x = normal(gen, 1200, 64).requires_grad_()
+    pos = torch.rand(1200, 3, device="cuda").requires_grad_()
+    offsets, freq = torch.tensor([0, 500, 1200]).cuda(), torch.rand(6, device="cuda")
+    g = normal(gen, 1200, 64)
+
+    def step():
+        q, k = K.rotary_axes(x.view(1200, 4, 16), x.view(1200, 4, 16), pos, freq, (2, 2, 2))
+        y = K.group_norm((q + k).reshape(1200, 64), 8, activation="silu", offsets=offsets)
+        r = K.route_experts(y, 4, offsets=offsets, renormalize=True)
+        loss = (y * g).sum() + (r.weights * g[:, :4]).sum() + r.balance + r.z
+        return (loss.detach(), *torch.autograd.grad(loss, [x, pos]))
+
+    want = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, expected in zip(out, want):
+            assert torch.equal(got, expected)
+
+
+def test_operators_called_from_two_threads(cuda):
+    from concurrent.futures import ThreadPoolExecutor
+
+    gen = generator(101)
+    inputs = [normal(gen, 3000, 64) for _ in range(2)]
+
+    def work(x):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            out = []
+            for _ in range(20):
+                t = x.clone().requires_grad_()
+                y = K.group_norm(t, 8, activation="silu",
+                                 offsets=torch.tensor([0, 1000, 3000], device="cuda"))
+                r = K.route_experts(y, 4, renormalize=True)
+                out.append((y, r.weights, *torch.autograd.grad(r.weights.sum() + r.z + y.sum(), [t])))
+            torch.cuda.current_stream().synchronize()
+            return out
+
+    torch.cuda.synchronize()
+    want = [work(x)[0] for x in inputs]
+    with ThreadPoolExecutor(2) as pool:
+        results = list(pool.map(work, inputs))
+    for outs, first in zip(results, want):
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, first))
