@@ -1215,11 +1215,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_experts(const Tensor& l
 struct AdamWParams {
   std::vector<Tensor> params;
   std::vector<int64_t> begins, sizes;
+  bool inference = false;  // one of them is an inference tensor
   AdamWParams(std::vector<Tensor> p, std::vector<int64_t> b)
       : params(std::move(p)), begins(std::move(b)) {
     TORCH_CHECK(params.size() == begins.size(), "AdamW needs one begin for each parameter: ",
                 params.size(), " parameters, ", begins.size(), " begins");
-    for (const Tensor& t : params) sizes.push_back(t.numel());
+    for (const Tensor& t : params) {
+      sizes.push_back(t.numel());
+      inference = inference || t.is_inference();
+    }
   }
 };
 
@@ -1230,6 +1234,8 @@ void adamw_step(const AdamWParams& tensors, const std::vector<OptTensor>& grads,
                 double size, double correct, double eps, int64_t step) {
   const std::vector<Tensor>& params = tensors.params;
   const std::vector<int64_t>& begins = tensors.begins;
+  TORCH_CHECK(!tensors.inference || c10::InferenceMode::is_enabled(),
+              "AdamW parameters that are inference tensors can be stepped in inference mode only");
   TORCH_CHECK(params.size() == grads.size(),
               "AdamW needs one gradient (or None) for each parameter");
   cuda_tensor(exp_avg, "AdamW exp_avg");
@@ -1262,8 +1268,6 @@ void adamw_step(const AdamWParams& tensors, const std::vector<OptTensor>& grads,
   for (size_t i = 0; i < params.size(); ++i) {
     if (!grads[i]) continue;
     const Tensor &p = params[i], &g = *grads[i];
-    TORCH_CHECK(!p.is_inference() || c10::InferenceMode::is_enabled(), "AdamW parameter ", i,
-                " is an inference tensor: step it in inference mode");
     const int dt = value_dtype(p, "AdamW parameter");
     TORCH_CHECK(g.scalar_type() == p.scalar_type() && g.sizes() == p.sizes() &&
                     g.device() == p.device() && p.device() == exp_avg.device() &&

@@ -117,7 +117,6 @@ class AdamW:
             for p, begin in zip(self.params, self.begins):
                 self.master[begin:begin + p.numel()] = p.reshape(-1)
 
-    @torch.no_grad()
     def step(self, grads: Sequence[torch.Tensor | None] | None = None, *,
              grad_scale: torch.Tensor | None = None) -> None:
         """Step every parameter that has a gradient, in place.
@@ -129,10 +128,10 @@ class AdamW:
         the stream is captured: its bias corrections are values of this call.
         """
         if grads is None:
-            grads = [p.grad for p in self.params]
+            grads = [p.grad for p in self._params]
         elif not isinstance(grads, list):
             grads = list(grads)
-        if len(grads) != len(self.params):
+        if len(grads) != len(self._params):
             raise ValueError("AdamW needs one gradient (or None) for each parameter")
         if grad_scale is not None:
             if not isinstance(grad_scale, torch.Tensor) or grad_scale.dtype != torch.float32:
