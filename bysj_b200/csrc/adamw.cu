@@ -22,8 +22,8 @@
 // 8-bit states: 160 us (16 B an element, 97 us at that bandwidth), bound by issue:
 // about 100 lane operations an element, of which the correctly rounded root and
 // quotient are a good part.  Random rounding adds 39 us for sqrt(v), 41 us for both:
-// the generator's 28 multiplications for four elements.  Values of 8-bit states: 76
-// us (10 B, 60 us).
+// an eighth more instructions, and registers for three CTAs on an SM instead of
+// four.  Values of 8-bit states: 75 us (10 B, 60 us).
 //
 // 8-bit states.  m keeps a sign and a 7-bit magnitude with 3 mantissa bits
 // (a relative rounding of at most 1/16 down to 2^-16 of the block's

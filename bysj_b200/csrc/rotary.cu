@@ -13,9 +13,10 @@
 // or 4 (float32) pairs of one 16-byte vector in registers and turns them in
 // every HS-th head of q and k, four heads requested at a time.  Consecutive
 // threads take consecutive vectors, then consecutive heads, so a warp reads and
-// writes whole lines.  Bound by HBM and the loads in flight: 98304 tokens of 16 +
-// 4 heads of 64 bfloat16 channels (506 MB) in 105 us, 0.73 of the measured copy
-// bandwidth.  Angles evaluated by each lane for its own pairs took 178 us; a
+// writes whole lines.  98304 tokens of 16 + 4 heads of 64 bfloat16 channels (506 MB)
+// take 105 us, 0.73 of the measured copy bandwidth: a CTA's loads begin after its
+// angles and a barrier, so neither HBM (54 % of its peak) nor issue (49 %) is full.
+// Angles evaluated by each lane for its own pairs took 178 us; a
 // fourth CTA on an SM, with half the loads in flight for each thread, 114 us.
 #include "launch.cuh"
 

@@ -811,8 +811,8 @@ std::tuple<Tensor, Tensor, Tensor> gie_zonal_scatter_backward(Tensor grad_output
 // ---- autograd of the training-step operators -----------------------------------
 //
 // Their gradients are autograd nodes in C++: a node called through Python costs
-// about 60 us more for a forward and backward call, several times what the
-// kernels of a small frame take.
+// 27 us more for a forward and backward call of a small frame (118 against 91 us),
+// about what its kernels take.
 
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;

@@ -30,9 +30,10 @@ class AdamW:
     """Decoupled-weight-decay Adam over a fixed list of parameters.
 
     ``params``: contiguous float32 or bfloat16 CUDA tensors on one device
-    (mixed dtypes are stepped in two launches).  ``lr``, ``betas``, ``eps`` and
-    ``weight_decay`` are plain attributes, so a schedule may assign them
-    between steps.  ``state_bits``: 32, or 8 for one byte per element and
+    that share no memory (mixed dtypes are stepped in two launches).  ``lr``,
+    ``betas``, ``eps`` and ``weight_decay`` are plain attributes, so a schedule
+    may assign them between steps; weights with another decay need an optimizer
+    of their own.  ``state_bits``: 32, or 8 for one byte per element and
     moment: the first as sign and 7-bit magnitude, the root of the second in 8
     bits, both relative to the largest of 256 elements.  A step rounds them to
     the nearest code (errors of at most 1/16 and 1/32 of a value).  A moment

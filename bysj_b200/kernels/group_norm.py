@@ -69,12 +69,17 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     ``x`` float32 or bfloat16, contiguous, channels last: ``(B, ..., C)``, a
     frame per leading entry, or with ``offsets`` int64 ``(B + 1,)`` packed
     ``(T, ..., C)``, frame ``b`` holding ``x[offsets[b]:offsets[b + 1]]``
-    (empty frames allowed).  ``mean`` and the biased variance run over all of
-    a frame's values in each of ``groups`` equal channel groups.  ``weight`` /
+    (empty frames allowed).  ``offsets`` cover ``x``: from 0, never falling, to
+    ``T``; rows of no frame are left unwritten (checked with
+    ``DPA4_CHECK_GROUPING=1``).  ``mean`` and the biased variance run over all of
+    a frame's values in each of ``groups`` equal channel groups; an infinity
+    or NaN among them makes all of them NaN.  ``weight`` /
     ``bias`` float32 ``(C,)`` or ``None``; ``activation`` ``None``, ``"silu"``
-    or ``"sigmoid"``.  Statistics and arithmetic are float32 or wider, with
-    one rounding to the output.  Gradients for ``x``, ``weight`` and ``bias``;
-    results repeat bit for bit.
+    or ``"sigmoid"``.  Statistics and arithmetic are float32, with one rounding
+    to the output.  Gradients for ``x``, ``weight`` and ``bias``, once (second
+    and forward-mode derivatives raise); results repeat bit for bit.  Whether a
+    CTA takes whole frames goes by their mean size: a long frame among many
+    short ones is slow.
     """
     eps = _validate(x, groups, weight, bias, eps, activation, offsets)
     require_dcu(x)  # the others share its device

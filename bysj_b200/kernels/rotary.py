@@ -4,8 +4,9 @@
 of every head of ``q`` and ``k`` by ``positions[t, axis] * inv_freq[pair]``,
 each axis (x, y, z of an atom; time, height, width of a grid) owning a section
 of the pairs.  Both tensors go through one launch.  Float positions are
-differentiable, so an energy that depends on coordinates through its
-attention scores gives forces.  No reference counterpart.
+differentiable once, so an energy that depends on coordinates through its
+attention scores gives forces (but a loss of those forces no gradient).  No
+reference counterpart.
 """
 from __future__ import annotations
 
@@ -76,8 +77,11 @@ def rotary_axes(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
     ``P = sum(sections) <= D / 2``.  Pair ``p`` is channels ``(p, p + P)``, or
     ``(2p, 2p + 1)`` when ``interleaved``; channels from ``2P`` on are copied.
     The angle is a float32 product and sine, cosine and rotation are float32,
-    with one rounding to the output.  Gradients for ``q``, ``k`` and float
-    ``positions`` (not for ``inv_freq``).
+    with one rounding to the output: at an angle of ``a`` radians the product's
+    rounding is ``a 2^-24``, and int64 positions beyond ``2^24`` are rounded to
+    float32 first.  Gradients for ``q``, ``k`` and float ``positions`` (not for
+    ``inv_freq``), once: a second derivative (a loss of forces that come from
+    positions) raises, as a forward-mode derivative does.
     """
     sections = _validate(q, k, positions, inv_freq, sections)
     require_dcu(q)  # the others share its device

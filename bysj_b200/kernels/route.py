@@ -70,13 +70,16 @@ def route_experts(logits: torch.Tensor, k: int, *, mask: torch.Tensor | None = N
     slots are ``-1`` with weight 0.  ``weights`` is ``p`` at the chosen
     experts, divided by its sum with ``renormalize``.  Tokens with a false
     ``mask`` (or without a logit above ``-inf``) are left out of everything,
-    whatever their logits hold.
+    whatever their logits and their cotangents hold; so are empty slots.
 
     ``balance``: the mean over frames (``offsets`` int64 ``(S + 1,)``; without
     it all tokens are one) with ``n > 0`` tokens of
     ``E / (k n^2) sum_e counts_e sum_t p_te``, 1 when the load is even;
     ``counts`` is a constant to it.  ``z``: the mean of ``logsumexp^2``.
-    ``weights``, ``balance`` and ``z`` are differentiable.
+    ``weights``, ``balance`` and ``z`` are differentiable, once (second and
+    forward-mode derivatives raise).  ``offsets`` cover the tokens, from 0, never
+    falling, to ``T`` (checked with ``DPA4_CHECK_GROUPING=1``): tokens before the
+    first count with the first frame, tokens after the last with the last.
     """
     _validate(logits, k, mask, offsets)
     require_dcu(logits)  # the others share its device
