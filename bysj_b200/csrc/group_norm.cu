@@ -267,11 +267,14 @@ struct Columns {
 };
 
 // Number, mean and sum of squares about the mean of some values.  Joining two of
-// them only adds squares, so no digits cancel wherever the means lie.
+// them only adds squares, so no digits cancel wherever the means lie.  The part is
+// an approximate quotient, of which a difference of means is taken; beside nothing
+// it is 1 or 0 exactly, so that a mean keeps its bits.
 struct Moments {
   float n = 0.0f, mean = 0.0f, m2 = 0.0f;
   __device__ __forceinline__ void join(const Moments& o) {
-    const float sum = n + o.n, part = o.n > 0.0f ? __fdividef(o.n, sum) : 0.0f, d = o.mean - mean;
+    const float sum = n + o.n, d = o.mean - mean;
+    const float part = o.n > 0.0f ? (n > 0.0f ? __fdividef(o.n, sum) : 1.0f) : 0.0f;
     mean = fmaf(d, part, mean);
     m2 += fmaf(d * (n * part), d, o.m2);  // d first: its square may overflow beside n = 0
     n = sum;
